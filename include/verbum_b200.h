@@ -199,6 +199,154 @@ VB_API vb_status vb_argmax_rows(const float* logits, int rows, int64_t n, int* o
                          void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Paged serving: a ragged batch of new tokens over a paged KV cache.        */
+/* The reference's cache is one contiguous [max_seq, KVH*D] block of a single */
+/* sequence (core/include/verbum/generate.h:19-30); here a pool of pages is   */
+/* shared by sequences of any lengths, and the calls below are its            */
+/* cuda_cache_append + cuda_rope + cuda_attn_decode (cuda_backend.h:29-42)    */
+/* for all of them at once.  Asynchronous on `stream`, no allocation; all     */
+/* memory belongs to the current device.                                      */
+/* ------------------------------------------------------------------------ */
+
+/* Element types of the paged calls and of vb_logits_process. */
+enum { VB_F32 = 0, VB_F16 = 1, VB_BF16 = 2 };
+
+/* A pool of pages: element (page, offset, kv head, d) of K is at
+ * k + page*stride_page + offset*stride_pos + head*stride_head + d (elements),
+ * V likewise at v.  Any order of the axes in memory; rows of head_dim elements
+ * are contiguous, bases and strides multiples of 16 bytes.  head_dim is 64 or
+ * 128, dtype VB_F32, VB_F16 or VB_BF16, page_size any positive number. */
+typedef struct {
+    void* k;
+    void* v;
+    int dtype;
+    int num_pages;
+    int page_size;
+    int kv_heads;
+    int head_dim;
+    int64_t stride_page, stride_pos, stride_head;
+} vb_paged_cache;
+
+/* Bits of vb_paged_batch.status. */
+enum {
+    VB_PAGED_BAD_ROWS = 1, /* a sequence's rows are not within 0..tokens, or more than max_new */
+    VB_PAGED_BAD_LEN = 2,  /* a length is negative or above max_len */
+    VB_PAGED_BAD_PAGE = 4  /* a page id outside 0..num_pages-1 */
+};
+
+/* New tokens of `batch` sequences, packed: sequence b owns rows
+ * q_start[b] .. q_start[b+1]-1 (none is fine) of the `tokens` rows; its cache
+ * holds lens[b] positions INCLUDING the new ones; table[b*table_stride + j] is
+ * the page of its positions j*page_size .. (j+1)*page_size-1.  Row i of a
+ * sequence with n new tokens has position p = lens[b] - n + i.  A row with
+ * p < 0 (left padding, or a sequence of length 0) has no position: nothing is
+ * appended for it and its attention is empty.  Rows behind the last sequence's
+ * are left as they were in every output.
+ * q_start [batch+1], lens [batch] and table are device arrays, read by the
+ * kernels only (a captured graph replays with their contents of that moment);
+ * max_new and max_len bound what they say.  The kernels check them: a sequence
+ * with bad rows is not computed, one with a bad length counts as length 0, a
+ * bad page is not written and reads as zeros, and each sets its bit in
+ * *status (a device word that the caller clears; NULL: not reported).  Pages
+ * that receive new tokens must belong to one sequence of the batch. */
+typedef struct {
+    int batch;
+    int tokens;
+    int max_new;
+    int max_len;
+    const int* q_start;
+    const int* lens;
+    const int* table;
+    int table_stride;
+    int* status;
+} vb_paged_batch;
+
+/* Position rotation and norm of vb_paged_append; all zero = neither.
+ * cos_tab / sin_tab: f32 [rope_positions, rot], the tables of vb_rope (their
+ * rows' first rot/2 entries are read); the first `rot` dims (a multiple of 16,
+ * at most head_dim) of q and k are rotated in pairs (d, d + rot/2), or
+ * (2d, 2d + 1) when interleaved.  q_norm / k_norm: f32 [head_dim] weights of
+ * the per-head RMS norm before the rotation, or NULL. */
+typedef struct {
+    const float* cos_tab;
+    const float* sin_tab;
+    int rope_positions;
+    int rot;
+    int interleaved;
+    const float* q_norm;
+    const float* k_norm;
+    float eps;
+} vb_paged_rope;
+
+/* Appends the new tokens' k and v [tokens][kv_heads][D] to their sequences'
+ * pages, k normed and rotated on the way, and writes q [tokens][heads][D],
+ * normed and rotated the same way, to q_out (q and q_out both NULL: keys and
+ * values only; q_out may equal q, with the same strides).  io is the type of q,
+ * q_out, k and v: the cache's own, or VB_F32 with a VB_BF16 cache.  Strides are in elements, per row
+ * and per head.  The rotation is the arithmetic of vb_rope, the norm that of
+ * vb_rmsnorm. */
+VB_API vb_status vb_paged_append(const vb_paged_cache* cache, const vb_paged_batch* batch,
+                                 const vb_paged_rope* rope, int io, int heads, const void* q,
+                                 int64_t q_row, int64_t q_head, void* q_out, int64_t qo_row,
+                                 int64_t qo_head, const void* k, int64_t k_row, int64_t k_head,
+                                 const void* v, int64_t v_row, int64_t v_head, void* stream);
+
+/* Causal attention of the new tokens over their sequences' pages (appended
+ * before): row with position p sees positions j <= p, with window > 0 only
+ * j > p - window.  out [tokens][heads][D] = softmax(scale * q.k) v; an empty
+ * row gives zeros.  lse (f32 [tokens][heads], may be NULL) gets the natural
+ * logarithm of the sum of exp(scale * q.k), -inf for an empty row.  heads is a
+ * multiple of kv_heads; query heads h*G .. h*G + G-1 read KV head h.  io as in
+ * vb_paged_append.  workspace: vb_paged_attn_workspace_bytes() bytes (the same
+ * for every io and window), 16-byte aligned, no initial contents; calls that
+ * may overlap need their own. */
+VB_API size_t vb_paged_attn_workspace_bytes(const vb_paged_cache* cache,
+                                            const vb_paged_batch* batch, int heads);
+VB_API vb_status vb_paged_attn(const vb_paged_cache* cache, const vb_paged_batch* batch, int io,
+                               int heads, const void* q, int64_t q_row, int64_t q_head,
+                               void* out, int64_t o_row, int64_t o_head, float* lse, float scale,
+                               int window, void* workspace, size_t workspace_bytes, void* stream);
+
+/* What vb_logits_process applies to a row of logits, in this order; NULL
+ * leaves a part out.  All arrays are on the device.
+ *  history: row r's tokens are hist_ids[hist_start[r] .. hist_start[r+1]-1]
+ *    (of hist_total), the first prompt_len[r] of them its prompt (NULL: none).
+ *    repetition[r]: logits of tokens in the history are divided by it when
+ *    positive, multiplied by it otherwise.  frequency[r] times the number of
+ *    times a token stands in the history behind the prompt, and presence[r]
+ *    once if it does at all, are subtracted.
+ *  bias: bias_vals[i] is added to the logit of bias_ids[i], for i in
+ *    bias_start[r] .. bias_start[r+1]-1 (of bias_total); of an id that stands
+ *    there more than once the sum, taken in the order of the list.
+ *  mask: bit t % 32 of word mask[r*mask_stride + t/32] is 0: token t's logit
+ *    becomes -inf, whatever it was.
+ * Ids outside 0 .. vocab-1 (padding) are skipped. */
+typedef struct {
+    const int* hist_start;
+    const int* hist_ids;
+    int64_t hist_total;
+    const int* prompt_len;
+    const float* repetition;
+    const float* frequency;
+    const float* presence;
+    const int* bias_start;
+    const int* bias_ids;
+    const float* bias_vals;
+    int64_t bias_total;
+    const uint32_t* mask;
+    int64_t mask_stride;
+} vb_logits_rules;
+
+/* Penalties, biases and grammar mask on logits [rows][vocab] (type dtype, row
+ * strides in elements) on the way to Sampler::sample
+ * (core/src/generate.cpp:197-252, which has none of them): out gets the
+ * processed rows and may equal logits (with the same stride).  Computed in
+ * f32, rounded once; the same result for the same input, always. */
+VB_API vb_status vb_logits_process(const void* logits, int64_t stride_in, void* out,
+                                   int64_t stride_out, int dtype, int rows, int64_t vocab,
+                                   const vb_logits_rules* rules, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Synthetic weights (host): seeded N(0, std) f32 fill, identical for a given  */
 /* (seed, offset) whatever the thread count.                                 */
 /* ------------------------------------------------------------------------ */

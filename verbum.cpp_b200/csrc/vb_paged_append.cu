@@ -1,0 +1,186 @@
+// vb_paged_append.cu -- new keys and values into a paged cache, with the
+// per-head RMS norm and the position rotation on the way; q rotated in the
+// same launch (kernels/cuda_ops.cu's rope and cache_append, and
+// generate.cpp:52-64, for a ragged batch).
+//
+// Bound by memory: q, k, v are read and q, K, V written once, nothing else is
+// moved but the rotation's angles.  A thread holds 16 elements of one head row
+// -- the 8 + 8 whose pairs rotate together -- so a row's norm is a sum over
+// D / 16 neighbouring lanes and every access is 16 bytes or two of them.
+#include "vb_kernels.cuh"
+#include "vb_paged.cuh"
+
+namespace vb {
+namespace {
+
+struct AppendArgs {
+    PagedView p;
+    vb_paged_rope rope;
+    const char *q, *kn, *vn;
+    char* qo;
+    int64_t q_row, q_head, qo_row, qo_head, k_row, k_head, v_row, v_head;  // bytes
+    int heads;      // 0: no q
+    int row_units;  // (heads + 2 * kv_heads) * (D / 16), the threads of one token
+};
+
+constexpr int kAppendThreads = 256;
+
+template <typename IO, typename KV, int D>
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __grid_constant__ AppendArgs a) {
+    constexpr int U = D / 16;  // threads of a head row
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31;
+    const int64_t g = (int64_t)blockIdx.x * kAppendThreads + threadIdx.x;
+    // the warp's first row's sequence by a warp-wide search; later rows are a few sequences on
+    const int64_t g0 = g - lane;
+    const int t0 = (int)(g0 / a.row_units);
+    if (t0 >= a.p.tokens) return;  // the whole warp is behind the last token
+    int b = paged_find_seq(a.p.q_start, a.p.batch, t0, lane);
+    const int t = (int)(g / a.row_units);
+    const int unit = (int)(g - (int64_t)t * a.row_units);
+    const int head = unit / U, u = unit % U;
+    while (b + 1 < a.p.batch && a.p.q_start[b + 1] <= t) b++;
+    bool live = t < a.p.tokens;
+    int pos = -1;
+    if (live) {
+        const PagedSeq s = paged_seq(a.p, b);
+        live = s.ok && t >= s.start && t < s.start + s.n;
+        pos = s.len - s.n + (t - s.start);
+        live = live && pos >= 0;
+    }
+    const bool is_q = head < a.heads, is_k = !is_q && head < a.heads + a.p.kv_heads;
+    const int h = is_q ? head : is_k ? head - a.heads : head - a.heads - a.p.kv_heads;
+    // the unit's two chunks of 8 elements
+    const int rot = a.rope.rot;
+    const bool turn = !(!is_q && !is_k) && 16 * u < rot;
+    const int c0 = turn && !a.rope.interleaved ? 8 * u : 16 * u;
+    const int c1 = turn && !a.rope.interleaved ? rot / 2 + 8 * u : 16 * u + 8;
+    float x[8], y[8];
+    if (live) {
+        const char* src = is_q ? a.q + t * a.q_row + h * a.q_head
+                          : is_k ? a.kn + t * a.k_row + h * a.k_head
+                                 : a.vn + t * a.v_row + h * a.v_head;
+        Eight<IO>::load(src + c0 * sizeof(IO), x);
+        Eight<IO>::load(src + c1 * sizeof(IO), y);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = y[e] = 0.f;
+    }
+    const float* w = is_q ? a.rope.q_norm : is_k ? a.rope.k_norm : nullptr;
+    if (a.rope.q_norm || a.rope.k_norm) {  // warp-uniform: every lane takes part in the sum
+        // a double sum of squares, as vb_rmsnorm's
+        double ss = 0.0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) ss += (double)x[e] * x[e] + (double)y[e] * y[e];
+#pragma unroll
+        for (int o = U / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (w) {
+            const float sc = rms_scale(ss, D, a.rope.eps);
+            float wx[8], wy[8];
+            Eight<float>::load(w + c0, wx);
+            Eight<float>::load(w + c1, wy);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                x[e] = __fmul_rn(__fmul_rn(x[e], sc), wx[e]);
+                y[e] = __fmul_rn(__fmul_rn(y[e], sc), wy[e]);
+            }
+        }
+    }
+    if (!live) return;
+    if (turn) {
+        float c[8], s[8];
+        Eight<float>::load(a.rope.cos_tab + (size_t)pos * rot + 8 * u, c);
+        Eight<float>::load(a.rope.sin_tab + (size_t)pos * rot + 8 * u, s);
+        if (!a.rope.interleaved) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float lo = __fsub_rn(__fmul_rn(x[e], c[e]), __fmul_rn(y[e], s[e]));
+                y[e] = __fadd_rn(__fmul_rn(y[e], c[e]), __fmul_rn(x[e], s[e]));
+                x[e] = lo;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const float lo = __fsub_rn(__fmul_rn(x[e], c[e / 2]), __fmul_rn(x[e + 1], s[e / 2]));
+                x[e + 1] = __fadd_rn(__fmul_rn(x[e + 1], c[e / 2]), __fmul_rn(x[e], s[e / 2]));
+                x[e] = lo;
+                const float l2 = __fsub_rn(__fmul_rn(y[e], c[4 + e / 2]), __fmul_rn(y[e + 1], s[4 + e / 2]));
+                y[e + 1] = __fadd_rn(__fmul_rn(y[e + 1], c[4 + e / 2]), __fmul_rn(y[e], s[4 + e / 2]));
+                y[e] = l2;
+            }
+        }
+    }
+    if (is_q) {
+        char* dst = a.qo + t * a.qo_row + h * a.qo_head;
+        Eight<IO>::store(dst + c0 * sizeof(IO), x);
+        Eight<IO>::store(dst + c1 * sizeof(IO), y);
+    } else {
+        const int64_t off = paged_offset(a.p, b, pos);
+        if (off < 0) return;
+        char* dst = const_cast<char*>(is_k ? a.p.k : a.p.v) + off + h * a.p.stride_head;
+        Eight<KV>::store(dst + c0 * sizeof(KV), x);
+        Eight<KV>::store(dst + c1 * sizeof(KV), y);
+    }
+}
+
+template <typename IO, typename KV>
+vb_status launch_append(const AppendArgs& a, int D, unsigned grid, cudaStream_t s) {
+    const cudaError_t e =
+        D == 128 ? launch_pdl(paged_append_kernel<IO, KV, 128>, dim3(grid), dim3(kAppendThreads), 0, s, a)
+                 : launch_pdl(paged_append_kernel<IO, KV, 64>, dim3(grid), dim3(kAppendThreads), 0, s, a);
+    if (e != cudaSuccess) return cuda_fail(e, "paged_append_kernel");
+    VB_LAUNCH_CHECK("paged_append_kernel");
+    return VB_OK;
+}
+
+}  // namespace
+}  // namespace vb
+
+using namespace vb;
+
+extern "C" vb_status vb_paged_append(const vb_paged_cache* cache, const vb_paged_batch* batch,
+                                     const vb_paged_rope* rope, int io, int heads, const void* q, int64_t q_row,
+                                     int64_t q_head, void* q_out, int64_t qo_row, int64_t qo_head, const void* k,
+                                     int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head,
+                                     void* stream) {
+    AppendArgs a{};
+    if ((q == nullptr) != (q_out == nullptr)) return fail(VB_ERR_ARG, "paged_append: q and q_out come together");
+    const vb_status st = paged_view(cache, batch, io, q ? heads : cache ? cache->kv_heads : 0, "paged_append", &a.p);
+    if (st) return st;
+    if (batch->tokens == 0 || batch->batch == 0) return VB_OK;
+    if (!k || !v) return fail(VB_ERR_ARG, "paged_append: null pointer");
+    const int es = paged_elem_bytes(io), D = cache->head_dim;
+    if ((q && (!paged_aligned(q, q_row, q_head, es) || !paged_aligned(q_out, qo_row, qo_head, es))) ||
+        !paged_aligned(k, k_row, k_head, es) || !paged_aligned(v, v_row, v_head, es))
+        return fail(VB_ERR_UNSUPPORTED, "paged_append: 16-byte alignment required");
+    if (q == q_out && q && (q_row != qo_row || q_head != qo_head))
+        return fail(VB_ERR_ARG, "paged_append: q in place needs equal strides");
+    if (rope) a.rope = *rope;
+    if (a.rope.rot) {
+        if (a.rope.rot < 0 || a.rope.rot % 16 || a.rope.rot > D)
+            return fail(VB_ERR_UNSUPPORTED, "paged_append: rot must be a multiple of 16, at most head_dim");
+        if (!a.rope.cos_tab || !a.rope.sin_tab) return fail(VB_ERR_ARG, "paged_append: null rotation table");
+        if (!paged_aligned(a.rope.cos_tab, 0, 0, 4) || !paged_aligned(a.rope.sin_tab, 0, 0, 4))
+            return fail(VB_ERR_UNSUPPORTED, "paged_append: 16-byte alignment required");
+        if (batch->max_len > a.rope.rope_positions) return fail(VB_ERR_ROPE, "position is outside the rope table");
+    }
+    if (!paged_aligned(a.rope.q_norm, 0, 0, 4) || !paged_aligned(a.rope.k_norm, 0, 0, 4))
+        return fail(VB_ERR_UNSUPPORTED, "paged_append: 16-byte alignment required");
+    a.q = static_cast<const char*>(q);
+    a.qo = static_cast<char*>(q_out);
+    a.kn = static_cast<const char*>(k);
+    a.vn = static_cast<const char*>(v);
+    a.q_row = q_row * es, a.q_head = q_head * es, a.qo_row = qo_row * es, a.qo_head = qo_head * es;
+    a.k_row = k_row * es, a.k_head = k_head * es, a.v_row = v_row * es, a.v_head = v_head * es;
+    a.heads = q ? heads : 0;
+    a.row_units = (a.heads + 2 * a.p.kv_heads) * (D / 16);
+    const int64_t blocks = ((int64_t)batch->tokens * a.row_units + kAppendThreads - 1) / kAppendThreads;
+    if (blocks > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_append: too many rows");
+    cudaStream_t s = as_stream(stream);
+    const unsigned grid = (unsigned)blocks;
+    if (io == VB_F32 && cache->dtype == VB_F32) return launch_append<float, float>(a, D, grid, s);
+    if (io == VB_F32) return launch_append<float, __nv_bfloat16>(a, D, grid, s);
+    if (io == VB_F16) return launch_append<__half, __half>(a, D, grid, s);
+    return launch_append<__nv_bfloat16, __nv_bfloat16>(a, D, grid, s);
+}

@@ -1,0 +1,656 @@
+// vb_paged_attn.cu -- causal attention of each sequence's new tokens over its
+// pages (generate.cpp:73-105 applied at every new position of a ragged batch).
+//
+// For the rows of one KV head (new tokens x the G query heads that share it)
+// s_j = q . k_j, m = max s, l = sum e^(s_j - m), out = sum e^(s_j - m) v_j / l,
+// kept as a running (m, l, sum) while one pass goes over the keys, so K and V
+// are read once for all G heads.
+#include <algorithm>
+#include <atomic>
+
+#include "vb_kernels.cuh"
+#include "vb_paged.cuh"
+#include "vb_pipe.cuh"
+#include "vb_tc.cuh"
+
+namespace vb {
+
+vb_status paged_view(const vb_paged_cache* c, const vb_paged_batch* b, int io, int heads, const char* who,
+                     PagedView* out) {
+    const std::string w = std::string(who) + ": ";
+    if (!c || !b || !c->k || !c->v) return fail(VB_ERR_ARG, w + "null pointer");
+    const int es = paged_elem_bytes(c->dtype);
+    if (!es || !paged_elem_bytes(io)) return fail(VB_ERR_ARG, w + "unknown element type");
+    if (io != c->dtype && !(io == VB_F32 && c->dtype == VB_BF16))
+        return fail(VB_ERR_UNSUPPORTED, w + "rows have the cache's type, or f32 with a bf16 cache");
+    if (c->head_dim != 64 && c->head_dim != 128) return fail(VB_ERR_UNSUPPORTED, w + "head_dim must be 64 or 128");
+    if (c->num_pages <= 0 || c->page_size <= 0 || c->kv_heads <= 0) return fail(VB_ERR_ARG, w + "non-positive shape");
+    if (heads <= 0 || heads % c->kv_heads) return fail(VB_ERR_ARG, w + "heads must be a multiple of kv_heads");
+    if (c->stride_page < 0 || c->stride_pos < 0 || c->stride_head < 0) return fail(VB_ERR_ARG, w + "negative stride");
+    if (!paged_aligned(c->k, c->stride_pos, c->stride_head, es) || !paged_aligned(c->v, c->stride_page, 0, es))
+        return fail(VB_ERR_UNSUPPORTED, w + "16-byte alignment required");
+    if (b->batch < 0 || b->tokens < 0 || b->max_new < 0 || b->max_len < 0 || b->table_stride < 0)
+        return fail(VB_ERR_ARG, w + "negative size");
+    if (b->batch && b->tokens) {
+        if (!b->q_start || !b->lens || (b->max_len && !b->table)) return fail(VB_ERR_ARG, w + "null pointer");
+        if (b->max_len > (int64_t)b->table_stride * c->page_size)
+            return fail(VB_ERR_ARG, w + "max_len is more than the table's pages hold");
+    }
+    PagedView& p = *out;
+    p.k = static_cast<const char*>(c->k);
+    p.v = static_cast<const char*>(c->v);
+    p.num_pages = c->num_pages;
+    p.page_size = c->page_size;
+    p.kv_heads = c->kv_heads;
+    p.page_shift = -1;
+    for (int i = 0; i < 31; i++)
+        if (c->page_size == 1 << i) p.page_shift = i;
+    p.stride_page = c->stride_page * es;
+    p.stride_pos = c->stride_pos * es;
+    p.stride_head = c->stride_head * es;
+    p.batch = b->batch;
+    p.tokens = b->tokens;
+    p.max_new = std::min(b->max_new, b->tokens);
+    p.max_len = b->max_len;
+    p.q_start = b->q_start;
+    p.lens = b->lens;
+    p.table = b->table;
+    p.table_stride = b->table_stride;
+    p.status = b->status;
+    return VB_OK;
+}
+
+namespace {
+
+struct AttnView {
+    PagedView p;
+    const char* q;
+    char* out;
+    int64_t q_row, q_head, o_row, o_head;  // bytes
+    float* lse;
+    int heads, group;   // group: query heads per KV head
+    float scale_log2;   // scale * log2(e): the softmax runs in base 2
+    int window;
+    int row_tiles;      // tiles of a KV head's rows in a sequence of max_new tokens
+    int splits, split_len;
+    float* part;        // [split][token][head][D] sums of a split, relative to its maximum
+    float2* part_ml;    // [split][token][head] (maximum in base 2, sum of weights)
+};
+
+// The keys that rows r0 .. r0 + count - 1 (of n * G) of a sequence see.
+struct KeyRange {
+    int lo, hi;  // positions lo .. hi - 1
+    int base;    // lo rounded down: where the first split starts
+};
+__device__ __forceinline__ KeyRange key_range(const AttnView& a, const PagedSeq& s, int r0, int count) {
+    const int r1 = min(r0 + count, s.n * a.group) - 1;
+    const int p0 = s.len - s.n + r0 / a.group, p1 = s.len - s.n + r1 / a.group;
+    KeyRange k;
+    k.hi = max(p1 + 1, 0);
+    k.lo = a.window > 0 ? max(p0 - a.window + 1, 0) : 0;
+    k.lo = min(k.lo, k.hi);
+    k.base = k.lo & ~15;
+    return k;
+}
+__device__ __forceinline__ int splits_used(const AttnView& a, const KeyRange& k) {
+    return max(1, (k.hi - k.base + a.split_len - 1) / a.split_len);
+}
+
+__device__ __forceinline__ void cp_async16(unsigned dst, const void* src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(unsigned addr, uint32_t* r) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(unsigned addr, uint32_t* r) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ float4 lds128(unsigned addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
+// d (16 x 8, f32) += a (16 x 16) b (16 x 8)
+template <typename T>
+__device__ __forceinline__ void mma16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16<__nv_bfloat16>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16<__half>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// d (16 x 8, f32) += a (16 x 8) b (8 x 8), tf32 operands
+__device__ __forceinline__ void mma8(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A pair of f32 as NT bf16 pairs whose sum it is: three hold all 24 bits of an
+// f32 (8 each), so products with bf16 values lose nothing.
+template <typename T, int NT>
+__device__ __forceinline__ void split_terms(float a, float b, uint32_t* t) {
+    t[0] = pack2<T>(a, b);
+    if constexpr (NT > 1) {
+#pragma unroll
+        for (int i = 1; i < NT; i++) {
+            a -= __uint_as_float(t[i - 1] << 16);
+            b -= __uint_as_float(t[i - 1] & 0xffff0000u);
+            t[i] = pack2<T>(a, b);
+        }
+    }
+}
+// x = hi + lo with hi a tf32 number (nearest) and lo the rest; the tensor core
+// reads the first 11 bits of lo.
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+    lo = __float_as_uint(x - __uint_as_float(hi));
+}
+
+constexpr int kFewWarps = 4;
+constexpr int kBK = 16;  // keys a warp takes at a time
+
+template <typename KV, int D>
+struct FewCfg {
+    static constexpr int kRowBytes = D * (int)sizeof(KV);
+    static constexpr int kBlockBytes = kBK * kRowBytes;  // K or V of a block
+    // three stages of 8 KB (D = 128, 16 bits) a warp: 96 KB in flight per CTA, two CTAs on an SM
+    static constexpr int kStages = sizeof(KV) == 4 && D == 128 ? 3 : kRowBytes == 128 ? 6 : 3;
+    static constexpr int kWarpBytes = kStages * 2 * kBlockBytes;
+    static constexpr int kMerge = kFewWarps * 16 * (D + 4) * 4;  // the warps' sums, rows padded by 16 bytes
+    static constexpr int kSmem = kFewWarps * kWarpBytes > kMerge ? kFewWarps * kWarpBytes : kMerge;
+};
+
+// Attention of 16 rows of a KV head: grid (split, KV head, row tile, sequence)
+// in one axis, 4 warps.  The warps share the rows and take turns at blocks of
+// 16 keys, each with a ring of its own in shared memory (no barrier in the
+// loop); at the end they join their (m, l, sum).
+//
+// Bound by memory when a tile holds all rows of its KV head (decoding).  16-bit
+// caches: one m16n8k16 product per 16 keys x 8 dims.  f32 rows over a bf16
+// cache: q and the weights as three bf16 terms.  f32 cache: hi/lo tf32 pairs,
+// three products.  Where the result is f32 a block's P.V is summed apart and
+// added to the running sum by an FMA: the tensor core's own accumulation
+// truncates, which over thousands of keys would show.
+template <typename IO, typename KV, int D>
+__global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __grid_constant__ AttnView a) {
+    using C = FewCfg<KV, D>;
+    constexpr bool kF32 = sizeof(KV) == 4;
+    constexpr bool kExact = sizeof(IO) == 4;
+    constexpr int NT = !kF32 && kExact ? 3 : 1;  // bf16 terms of an f32 operand
+    constexpr int NK = D / 16;
+    extern __shared__ __align__(1024) char smem[];
+    __shared__ float2 ml[kFewWarps][16];
+    pdl_wait();
+    pdl_trigger();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+    int64_t idx = blockIdx.x;
+    const int split = (int)(idx % a.splits);
+    idx /= a.splits;
+    const int kvh = (int)(idx % a.p.kv_heads);
+    idx /= a.p.kv_heads;
+    const int r0 = (int)(idx % a.row_tiles) * 16, b = (int)(idx / a.row_tiles);
+    const PagedSeq s = paged_seq(a.p, b);
+    const int rows = s.n * a.group;
+    if (r0 >= rows) return;
+    const KeyRange kr = key_range(a, s, r0, 16);
+    if (split >= splits_used(a, kr)) return;
+    const int k_begin = kr.base + split * a.split_len, k_end = min(k_begin + a.split_len, kr.hi);
+    const int blocks = max(0, (k_end - k_begin + kBK - 1) / kBK);
+    const int mine = blocks > warp ? (blocks - warp + kFewWarps - 1) / kFewWarps : 0;  // blocks warp, warp + 4, ...
+
+    const unsigned ring = smem_addr(smem) + warp * C::kWarpBytes;
+    const int64_t head_off = (int64_t)kvh * a.p.stride_head;
+    // lane l looks up the place of key l % 16 of a block; -1: outside, read as zeros
+    auto look_up = [&](int i) -> int64_t {
+        const int key = k_begin + (warp + i * kFewWarps) * kBK + (lane & 15);
+        return i < mine && key >= kr.lo && key < k_end ? paged_offset(a.p, b, key) : -1;
+    };
+    // 16-byte chunk c of row r sits at chunk c ^ swz(r): the loads below touch 8 rows (or 2 and 4) at once
+    auto swz = [](int r) { return kF32 ? (((r >> 1) & 3) ^ ((r & 1) << 1)) << 1 : r & 7; };
+    auto fetch = [&](int i, int64_t off) {
+        if (i < mine) {
+            constexpr int RC = C::kRowBytes / 16, RPI = 32 / RC;
+            const unsigned st = ring + (unsigned)(i % C::kStages) * 2 * C::kBlockBytes;
+#pragma unroll
+            for (int it = 0; it < kBK / RPI; it++) {
+                const int r = it * RPI + lane / RC, c = lane % RC;
+                const int64_t o = __shfl_sync(0xffffffffu, off, r);
+                const unsigned dst = st + r * C::kRowBytes + ((c ^ swz(r)) << 4);
+                const int64_t at = o < 0 ? 0 : o + head_off + c * 16;
+                cp_async16(dst, a.p.k + at, o >= 0);
+                cp_async16(dst + C::kBlockBytes, a.p.v + at, o >= 0);
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < C::kStages - 1; i++) fetch(i, look_up(i));
+    int64_t next = look_up(C::kStages - 1);
+
+    // rows g and g + 8 of the tile: token, query head, position
+    int pos[2];
+    const char* qp[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int r = r0 + g + 8 * i;
+        pos[i] = r < rows ? s.len - s.n + r / a.group : -1;
+        const int rr = min(r, rows - 1);
+        qp[i] = a.q + (int64_t)(s.start + rr / a.group) * a.q_row + (int64_t)(kvh * a.group + rr % a.group) * a.q_head;
+    }
+    // q fragments.  f32 cache: dims 16 kk + 4 t4 .. + 3 of both rows (the order of
+    // the dims inside a product is free as long as K's is the same).  16 bits: the
+    // m16n8k16 layout, dims 16 kk + 2 t4, + 1, + 8, + 9.
+    float qf[kF32 ? NK : 1][8];
+    uint32_t qh[kF32 ? 1 : NK][NT][4];
+    if constexpr (kF32) {
+#pragma unroll
+        for (int kk = 0; kk < NK; kk++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const float4 x = *reinterpret_cast<const float4*>(qp[i] + (16 * kk + 4 * t4) * 4);
+                qf[kk][4 * i] = x.x, qf[kk][4 * i + 1] = x.y, qf[kk][4 * i + 2] = x.z, qf[kk][4 * i + 3] = x.w;
+            }
+    } else {
+#pragma unroll
+        for (int kk = 0; kk < NK; kk++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {  // a0 (g, lo), a1 (g + 8, lo), a2 (g, hi), a3 (g + 8, hi)
+                const char* x = qp[j & 1] + (16 * kk + 2 * t4 + 8 * (j >> 1)) * sizeof(IO);
+                if constexpr (kExact) {
+                    const float2 f = *reinterpret_cast<const float2*>(x);
+                    uint32_t tt[NT];
+                    split_terms<KV, NT>(f.x, f.y, tt);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) qh[kk][n][j] = tt[n];
+                } else {
+                    qh[kk][0][j] = *reinterpret_cast<const uint32_t*>(x);
+                }
+            }
+    }
+
+    float o[D / 8][4];
+#pragma unroll
+    for (int n = 0; n < D / 8; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[n][e] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    for (int i = 0; i < mine; i++) {
+        cp_async_wait<C::kStages - 2>();
+        __syncwarp();
+        fetch(i + C::kStages - 1, next);
+        next = look_up(i + C::kStages);
+        const unsigned kb = ring + (unsigned)(i % C::kStages) * 2 * C::kBlockBytes, vb = kb + C::kBlockBytes;
+        const int key0 = k_begin + (warp + i * kFewWarps) * kBK;
+        // S: 16 rows x 16 keys as two n-tiles; the small terms in an accumulator of their own
+        float sc[2][4] = {}, sl[2][4] = {};
+        if constexpr (kF32) {
+#pragma unroll
+            for (int kk = 0; kk < NK; kk++) {
+                uint32_t qhi[8], qlo[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) split_tf32(qf[kk][e], qhi[e], qlo[e]);
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    const int r = 8 * n + g;
+                    const float4 kx = lds128(kb + r * C::kRowBytes + (((4 * kk + t4) ^ swz(r)) << 4));
+                    const float kv[4] = {kx.x, kx.y, kx.z, kx.w};
+                    uint32_t khi[4], klo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) split_tf32(kv[e], khi[e], klo[e]);
+#pragma unroll
+                    for (int h = 0; h < 4; h += 2) {
+                        const uint32_t ah[4] = {qhi[h], qhi[4 + h], qhi[h + 1], qhi[5 + h]};
+                        const uint32_t al[4] = {qlo[h], qlo[4 + h], qlo[h + 1], qlo[5 + h]};
+                        mma8(sc[n], ah, khi[h], khi[h + 1]);
+                        mma8(sl[n], ah, klo[h], klo[h + 1]);
+                        mma8(sl[n], al, khi[h], khi[h + 1]);
+                    }
+                }
+            }
+        } else {
+            const int r = (lane & 7) + ((lane >> 4) << 3), cc = (lane >> 3) & 1;
+#pragma unroll
+            for (int kk = 0; kk < NK; kk++) {
+                uint32_t kx[4];
+                ldsm4(kb + r * C::kRowBytes + (((2 * kk + cc) ^ swz(r)) << 4), kx);
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    mma16<KV>(sc[n], qh[kk][0], kx[2 * n], kx[2 * n + 1]);
+#pragma unroll
+                    for (int x = 1; x < NT; x++) mma16<KV>(sl[n], qh[kk][x], kx[2 * n], kx[2 * n + 1]);
+                }
+            }
+        }
+        // weights: rows g (e 0, 1) and g + 8 (e 2, 3), keys key0 + 8 n + 2 t4 + (e & 1)
+        float mx[2] = {m[0], m[1]};
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int key = key0 + 8 * n + 2 * t4 + (e & 1), p = pos[e >> 1];
+                float x = (sc[n][e] + sl[n][e]) * a.scale_log2;
+                if (key > p || key >= k_end || (a.window > 0 && key <= p - a.window)) x = -INFINITY;
+                sc[n][e] = x;
+                mx[e >> 1] = fmaxf(mx[e >> 1], x);
+            }
+        float alpha[2];
+#pragma unroll
+        for (int i2 = 0; i2 < 2; i2++) {
+            mx[i2] = fmaxf(mx[i2], __shfl_xor_sync(0xffffffffu, mx[i2], 1));
+            mx[i2] = fmaxf(mx[i2], __shfl_xor_sync(0xffffffffu, mx[i2], 2));
+            const float mb = mx[i2] == -INFINITY ? 0.f : mx[i2];
+            alpha[i2] = ex2_approx(m[i2] - mb);
+            m[i2] = mx[i2];
+            mx[i2] = mb;
+            l[i2] *= alpha[i2];
+        }
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                sc[n][e] = ex2_approx(sc[n][e] - mx[e >> 1]);
+                l[e >> 1] += sc[n][e];
+            }
+        // P.V
+        if constexpr (kF32) {
+            // keys 8 kt + 2 t4 and + 1 of the block are the product's k = t4 and t4 + 4, dims
+            // 32 nn + 4 g + j its column g for j = 0..3: the same order in P and V
+            uint32_t ph[2][4], pl[2][4];
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++) {
+                split_tf32(sc[kt][0], ph[kt][0], pl[kt][0]);
+                split_tf32(sc[kt][2], ph[kt][1], pl[kt][1]);
+                split_tf32(sc[kt][1], ph[kt][2], pl[kt][2]);
+                split_tf32(sc[kt][3], ph[kt][3], pl[kt][3]);
+            }
+#pragma unroll
+            for (int nn = 0; nn < D / 32; nn++) {
+                float pv[4][4] = {};
+#pragma unroll
+                for (int kt = 0; kt < 2; kt++) {
+                    const int ra = 8 * kt + 2 * t4;
+                    const float4 va = lds128(vb + ra * C::kRowBytes + (((8 * nn + g) ^ swz(ra)) << 4));
+                    const float4 vc = lds128(vb + (ra + 1) * C::kRowBytes + (((8 * nn + g) ^ swz(ra + 1)) << 4));
+                    const float x0[4] = {va.x, va.y, va.z, va.w}, x1[4] = {vc.x, vc.y, vc.z, vc.w};
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        uint32_t h0, l0, h1, l1;
+                        split_tf32(x0[j], h0, l0);
+                        split_tf32(x1[j], h1, l1);
+                        mma8(pv[j], pl[kt], h0, h1);
+                        mma8(pv[j], ph[kt], l0, l1);
+                        mma8(pv[j], ph[kt], h0, h1);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        o[4 * nn + j][e] = fmaf(o[4 * nn + j][e], alpha[e >> 1], pv[j][e]);
+            }
+        } else {
+            uint32_t ph[NT][4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint32_t tt[NT];
+                split_terms<KV, NT>(sc[j >> 1][2 * (j & 1)], sc[j >> 1][2 * (j & 1) + 1], tt);
+#pragma unroll
+                for (int x = 0; x < NT; x++) ph[x][j] = tt[x];
+            }
+            const int r = lane & 15, cc = lane >> 4;
+#pragma unroll
+            for (int n = 0; n < D / 8; n += 2) {
+                uint32_t vx[4];
+                ldsm4_t(vb + r * C::kRowBytes + (((n + cc) ^ swz(r)) << 4), vx);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if constexpr (kExact) {
+                        float pv[4] = {};
+#pragma unroll
+                        for (int x = NT - 1; x >= 0; x--) mma16<KV>(pv, ph[x], vx[2 * h], vx[2 * h + 1]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[n + h][e] = fmaf(o[n + h][e], alpha[e >> 1], pv[e]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[n + h][e] *= alpha[e >> 1];
+                        mma16<KV>(o[n + h], ph[0], vx[2 * h], vx[2 * h + 1]);
+                    }
+                }
+            }
+        }
+    }
+    cp_async_wait<0>();
+    // join the warps: every warp's sums to shared memory, then all threads over (row, dims)
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        if (t4 == 0) ml[warp][g + 8 * i] = make_float2(m[i], l[i]);
+    }
+    __syncthreads();  // the rings are free
+    float* sums = reinterpret_cast<float*>(smem);
+    constexpr int LD = D + 4;
+#pragma unroll
+    for (int n = 0; n < D / 8; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            // f32: n-tile 4 nn + j column c is dim 32 nn + 4 c + j; 16 bits: 8 n + c
+            const int c = 2 * t4 + (e & 1);
+            const int d = kF32 ? 32 * (n >> 2) + 4 * c + (n & 3) : 8 * n + c;
+            sums[(warp * 16 + g + 8 * (e >> 1)) * LD + d] = o[n][e];
+        }
+    __syncthreads();
+    constexpr int TR = kFewWarps * 32 / 16;  // threads of a row
+    const int row = threadIdx.x / TR, r = r0 + row;
+    if (r >= rows) return;
+    float M = -INFINITY, L = 0.f, w[kFewWarps];
+#pragma unroll
+    for (int x = 0; x < kFewWarps; x++) M = fmaxf(M, ml[x][row].x);
+#pragma unroll
+    for (int x = 0; x < kFewWarps; x++) {
+        w[x] = ex2_approx(ml[x][row].x - (M == -INFINITY ? 0.f : M));
+        L += ml[x][row].y * w[x];
+    }
+    const int token = s.start + r / a.group, head = kvh * a.group + r % a.group;
+    const int64_t th = (int64_t)token * a.heads + head;
+    const bool last = a.splits == 1;
+    const float inv = last ? (L > 0.f ? 1.f / L : 0.f) : 1.f;
+#pragma unroll
+    for (int c = 0; c < D / 8 / TR; c++) {
+        const int d = (c * TR + threadIdx.x % TR) * 8;
+        float y[8] = {};
+#pragma unroll
+        for (int x = 0; x < kFewWarps; x++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] = fmaf(w[x], sums[(x * 16 + row) * LD + d + e], y[e]);
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] *= inv;
+        if (last)
+            Eight<IO>::store(a.out + token * a.o_row + head * a.o_head + d * sizeof(IO), y);
+        else
+            Eight<float>::store(a.part + ((int64_t)split * a.p.tokens * a.heads + th) * D + d, y);
+    }
+    if (threadIdx.x % TR == 0) {
+        if (!last)
+            a.part_ml[(int64_t)split * a.p.tokens * a.heads + th] = make_float2(M, L);
+        else if (a.lse)
+            a.lse[th] = L > 0.f ? (M + log2f(L)) * 0.693147180559945309f : -INFINITY;
+    }
+}
+
+// Joins the splits of a row: a warp per (token, head), grid over them.
+template <typename IO, int D>
+__global__ void __launch_bounds__(128) paged_attn_merge_kernel(const __grid_constant__ AttnView a, int tile_rows) {
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31;
+    const int64_t th = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (th >= (int64_t)a.p.tokens * a.heads) return;
+    const int token = (int)(th / a.heads), head = (int)(th % a.heads);
+    const int b = paged_find_seq(a.p.q_start, a.p.batch, token, lane);
+    const PagedSeq s = paged_seq(a.p, b);
+    if (!s.ok || token < s.start || token >= s.start + s.n) return;
+    const int r = (token - s.start) * a.group + head % a.group;
+    const int used = splits_used(a, key_range(a, s, r / tile_rows * tile_rows, tile_rows));
+    constexpr int E = D / 32;
+    float y[E] = {}, M = -INFINITY, L = 0.f;
+    const int64_t step = (int64_t)a.p.tokens * a.heads;
+    for (int x = lane; x < used; x += 32) M = fmaxf(M, a.part_ml[x * step + th].x);
+    M = warp_max(M);
+    const float mb = M == -INFINITY ? 0.f : M;
+    for (int x = 0; x < used; x++) {
+        const float2 p = a.part_ml[x * step + th];
+        const float w = ex2_approx(p.x - mb);
+        L = fmaf(p.y, w, L);
+        const float* src = a.part + (x * step + th) * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; e++) y[e] = fmaf(w, src[e], y[e]);
+    }
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    IO* dst = reinterpret_cast<IO*>(a.out + token * a.o_row + head * a.o_head) + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; e++) dst[e] = (IO)(y[e] * inv);
+    if (a.lse && lane == 0) a.lse[th] = L > 0.f ? (M + log2f(L)) * 0.693147180559945309f : -INFINITY;
+}
+
+// How the work is cut up: from the host's bounds alone, so that a captured
+// launch holds for any lengths within them.  A tile's keys are split where the
+// tiles alone do not fill the card: about four CTAs for each SM (two run at a
+// time), of at least 64 keys, one block of 16 a warp.
+struct Plan {
+    int row_tiles, splits, split_len;
+    int max_splits;  // for any window
+};
+Plan make_plan(const PagedView& p, int heads, int window) {
+    Plan pl{};
+    const int G = heads / p.kv_heads;
+    pl.row_tiles = (int)(((int64_t)p.max_new * G + 15) / 16);
+    const int64_t all = std::max(p.max_len, 1);
+    int64_t span = all;  // keys from a tile's base (lo rounded down to 16) to its last row's
+    if (window > 0) span = std::min<int64_t>(span, (int64_t)window + 30);
+    // tiles that can hold rows
+    const int64_t tiles =
+        std::max<int64_t>(1, std::min<int64_t>((int64_t)p.batch * pl.row_tiles,
+                                               (int64_t)p.tokens * G / 16 + p.batch)) * p.kv_heads;
+    const int64_t want = std::max<int64_t>(1, 148 * 4 / tiles);
+    pl.max_splits = (int)std::min<int64_t>(want, (all + 63) / 64);
+    const int64_t n = std::min<int64_t>(want, (span + 63) / 64);
+    pl.split_len = (int)(((span + n - 1) / n + 63) / 64 * 64);
+    pl.splits = (int)((span + pl.split_len - 1) / pl.split_len);
+    return pl;
+}
+size_t plan_bytes(const Plan& pl, const PagedView& p, int heads, int D) {
+    return pl.max_splits > 1 ? (size_t)pl.max_splits * p.tokens * heads * (D + 2) * 4 : 0;
+}
+
+template <typename IO, typename KV, int D>
+vb_status launch_few(const AttnView& a, cudaStream_t s) {
+    using C = FewCfg<KV, D>;
+    static std::atomic<unsigned long long> done{0};
+    cudaError_t e = smem_attr_once(paged_attn_few_kernel<IO, KV, D>, C::kSmem, done);
+    if (e != cudaSuccess) return cuda_fail(e, "paged attention: shared memory attribute");
+    const int64_t grid = (int64_t)a.splits * a.p.kv_heads * a.row_tiles * a.p.batch;
+    if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
+    e = launch_pdl(paged_attn_few_kernel<IO, KV, D>, dim3((unsigned)grid), dim3(kFewWarps * 32), C::kSmem, s, a);
+    if (e != cudaSuccess) return cuda_fail(e, "paged_attn_few_kernel");
+    if (a.splits > 1) {
+        const int64_t g2 = ((int64_t)a.p.tokens * a.heads + 3) / 4;
+        if (g2 > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
+        e = launch_pdl(paged_attn_merge_kernel<IO, D>, dim3((unsigned)g2), dim3(128), 0, s, a, 16);
+        if (e != cudaSuccess) return cuda_fail(e, "paged_attn_merge_kernel");
+    }
+    VB_LAUNCH_CHECK("paged attention");
+    return VB_OK;
+}
+
+template <int D>
+vb_status launch_attn(const AttnView& a, int io, int cache, cudaStream_t s) {
+    if (io == VB_F32 && cache == VB_F32) return launch_few<float, float, D>(a, s);
+    if (io == VB_F32) return launch_few<float, __nv_bfloat16, D>(a, s);
+    if (io == VB_F16) return launch_few<__half, __half, D>(a, s);
+    return launch_few<__nv_bfloat16, __nv_bfloat16, D>(a, s);
+}
+
+}  // namespace
+}  // namespace vb
+
+using namespace vb;
+
+extern "C" size_t vb_paged_attn_workspace_bytes(const vb_paged_cache* cache, const vb_paged_batch* batch, int heads) {
+    PagedView p{};
+    if (!cache || paged_view(cache, batch, cache->dtype, heads, "paged_attn", &p) || !p.batch || !p.tokens) return 0;
+    return plan_bytes(make_plan(p, heads, 0), p, heads, cache->head_dim);
+}
+
+extern "C" vb_status vb_paged_attn(const vb_paged_cache* cache, const vb_paged_batch* batch, int io, int heads,
+                                   const void* q, int64_t q_row, int64_t q_head, void* out, int64_t o_row,
+                                   int64_t o_head, float* lse, float scale, int window, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+    AttnView a{};
+    const vb_status st = paged_view(cache, batch, io, heads, "paged_attn", &a.p);
+    if (st) return st;
+    if (window < 0) return fail(VB_ERR_ARG, "paged_attn: negative window");
+    if (!batch->batch || !batch->tokens || !batch->max_new) return VB_OK;
+    if (!q || !out) return fail(VB_ERR_ARG, "paged_attn: null pointer");
+    const int es = paged_elem_bytes(io), D = cache->head_dim;
+    if (!paged_aligned(q, q_row, q_head, es) || !paged_aligned(out, o_row, o_head, es) || !paged_aligned(workspace, 0, 0, 1))
+        return fail(VB_ERR_UNSUPPORTED, "paged_attn: 16-byte alignment required");
+    const Plan pl = make_plan(a.p, heads, window);
+    const size_t need = plan_bytes(pl, a.p, heads, D);
+    if (need > workspace_bytes || (need && !workspace))
+        return fail(VB_ERR_ARG, "paged_attn: the workspace is too small");
+    a.q = static_cast<const char*>(q);
+    a.out = static_cast<char*>(out);
+    a.q_row = q_row * es, a.q_head = q_head * es, a.o_row = o_row * es, a.o_head = o_head * es;
+    a.lse = lse;
+    a.heads = heads;
+    a.group = heads / cache->kv_heads;
+    a.scale_log2 = scale * 1.44269504088896341f;
+    a.window = window;
+    a.row_tiles = pl.row_tiles;
+    a.splits = pl.splits;
+    a.split_len = pl.split_len;
+    a.part = static_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)pl.splits * a.p.tokens * heads * D);
+    return D == 128 ? launch_attn<128>(a, io, cache->dtype, as_stream(stream))
+                    : launch_attn<64>(a, io, cache->dtype, as_stream(stream));
+}
