@@ -7,6 +7,7 @@
 // are read once for all G heads.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "vb_kernels.cuh"
 #include "vb_paged.cuh"
@@ -62,6 +63,11 @@ vb_status paged_view(const vb_paged_cache* c, const vb_paged_batch* b, int io, i
 
 namespace {
 
+// How a kernel cuts its work: rows of a tile, and the split of a tile's keys.
+struct Cut {
+    int rows, splits, len;
+};
+
 struct AttnView {
     PagedView p;
     const char* q;
@@ -71,8 +77,9 @@ struct AttnView {
     int heads, group;   // group: query heads per KV head
     float scale_log2;   // scale * log2(e): the softmax runs in base 2
     int window;
-    int row_tiles;      // tiles of a KV head's rows in a sequence of max_new tokens
-    int splits, split_len;
+    int few_rows;       // sequences with at most this many rows a KV head run in the few-rows kernel
+    int row_tiles;      // its row tiles of a sequence
+    Cut few, many;
     float* part;        // [split][token][head][D] sums of a split, relative to its maximum
     float2* part_ml;    // [split][token][head] (maximum in base 2, sum of weights)
 };
@@ -92,8 +99,8 @@ __device__ __forceinline__ KeyRange key_range(const AttnView& a, const PagedSeq&
     k.base = k.lo & ~15;
     return k;
 }
-__device__ __forceinline__ int splits_used(const AttnView& a, const KeyRange& k) {
-    return max(1, (k.hi - k.base + a.split_len - 1) / a.split_len);
+__device__ __forceinline__ int splits_used(const Cut& c, const KeyRange& k) {
+    return max(1, (k.hi - k.base + c.len - 1) / c.len);
 }
 
 __device__ __forceinline__ void cp_async16(unsigned dst, const void* src, bool real) {
@@ -222,17 +229,17 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     int64_t idx = blockIdx.x;
-    const int split = (int)(idx % a.splits);
-    idx /= a.splits;
+    const int split = (int)(idx % a.few.splits);
+    idx /= a.few.splits;
     const int kvh = (int)(idx % a.p.kv_heads);
     idx /= a.p.kv_heads;
     const int r0 = (int)(idx % a.row_tiles) * 16, b = (int)(idx / a.row_tiles);
     const PagedSeq s = paged_seq(a.p, b);
     const int rows = s.n * a.group;
-    if (r0 >= rows) return;
+    if (r0 >= rows || rows > a.few_rows) return;
     const KeyRange kr = key_range(a, s, r0, 16);
-    if (split >= splits_used(a, kr)) return;
-    const int k_begin = kr.base + split * a.split_len, k_end = min(k_begin + a.split_len, kr.hi);
+    if (split >= splits_used(a.few, kr)) return;
+    const int k_begin = kr.base + split * a.few.len, k_end = min(k_begin + a.few.len, kr.hi);
     const int blocks = max(0, (k_end - k_begin + kBK - 1) / kBK);
     const int mine = blocks > warp ? (blocks - warp + kFewWarps - 1) / kFewWarps : 0;  // blocks warp, warp + 4, ...
 
@@ -492,7 +499,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
     }
     const int token = s.start + r / a.group, head = kvh * a.group + r % a.group;
     const int64_t th = (int64_t)token * a.heads + head;
-    const bool last = a.splits == 1;
+    const bool last = a.few.splits == 1;
     const float inv = last ? (L > 0.f ? 1.f / L : 0.f) : 1.f;
 #pragma unroll
     for (int c = 0; c < D / 8 / TR; c++) {
@@ -517,9 +524,420 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
     }
 }
 
+// ------------------------------------------------------------ many rows
+// Attention of 256 rows of a KV head on the 5th-generation tensor cores: two
+// tiles of 128 rows, so that one tile's softmax runs while the other's products
+// do.  Keys come 128 at a time.
+//   warps 0-3, 4-7   softmax of tile 0 / 1: a thread owns a row.  It reads its
+//                    scores from tensor memory, and writes its weights (16 bits)
+//                    back over them as the A operand of P.V.
+//   warps 8-11       producers: gather the tiles' rows from their pages with
+//                    16-byte cp.async (any page size and any strides; places
+//                    outside the range become zeros) into the 128-byte-swizzled
+//                    layout the products read; K and V take turns in a ring of
+//                    four stages.
+//   warp 12          one thread issues the products: for each key tile and row
+//                    tile P.V, then the next key tile's Q.K.  They run in order, so
+//                    a finished Q.K says that the P.V before it is finished too,
+//                    and a row's thread may rescale its sums then.
+// The running maximum is raised, and the sums rescaled, only when a score
+// exceeds it by more than 2^8: weights stay below 256, which changes no
+// rounding (they are relative), and rescaling is rare.
+// Bound by the exponentials (16 a clock on an SM: 2048 clocks for the two tiles
+// of 128 x 128) as much as by the products (2048 clocks at D = 128).
+constexpr int kTcThreads = 512;
+constexpr int kTcRows = 256;
+constexpr int kTcStages = 4;
+
+template <int D>
+struct TcCfg {
+    static constexpr int kHalf = 128 * 128;             // 128 rows of 64 elements
+    static constexpr int kTile = kHalf * (D / 64);      // Q, K or V of 128 rows
+    static constexpr int kOffKV = 2 * kTile;
+    static constexpr int kSmem = kOffKV + kTcStages * kTile + 1024;  // + alignment
+    static constexpr int kO = 256;                      // tensor-memory columns: S0, S1, O0, O1
+};
+
+// Descriptor of an operand whose rows are the summed dimension (V: rows are keys, a row's
+// 64 elements lie along N): 8 rows x 128 bytes swizzled, 1024 bytes from 8 rows to the next
+// and 16 KB from 64 elements of N to the next.
+__device__ __forceinline__ uint64_t sw128_desc_mn(unsigned saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((128 * 128) >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// D[tmem] (+)= A[tmem] B[smem]
+__device__ __forceinline__ void mma_f16_ta(unsigned tmem, unsigned atmem, uint64_t bdesc, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{ .reg .pred p; setp.ne.u32 p, %4, 0; "
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(tmem),
+        "r"(atmem), "l"(bdesc), "r"(idesc), "r"((unsigned)acc)
+        : "memory");
+}
+// 32 columns of this warp's 32 lanes
+__device__ __forceinline__ void tmem_st32(unsigned taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+// Bounded wait for a phase of an mbarrier: gives up after 2 s, or when another
+// wait of this CTA did (failed; NULL: waits on regardless).  Inline: a call
+// would hold the softmax threads to the registers of the launch.
+__device__ __forceinline__ bool tc_wait(unsigned bar, unsigned parity, volatile int* failed) {
+    if (mbar_try(bar, parity)) return true;
+    const unsigned long long t0 = now_ns();
+    for (unsigned it = 1;; it++) {
+        if (mbar_try(bar, parity)) return true;
+        if ((it & 63u) == 0 && ((failed && *failed) || now_ns() - t0 > kWaitNs)) {
+            if (failed) *failed = 1;
+            return false;
+        }
+    }
+}
+
+// Sequence and tile of the idx-th of all tiles of `rows` rows (sequences with more than
+// a.few_rows rows only), the last ones -- which see most keys -- first; b = -1: none.
+__device__ __forceinline__ void find_tile(const AttnView& a, int64_t idx, int rows, int lane, int& b, int& tile) {
+    // from the last sequence to the first
+    b = -1;
+    tile = 0;
+    for (int hi = a.p.batch; hi > 0; hi -= 32) {
+        const int i = hi - 1 - lane;
+        int n = 0;
+        if (i >= 0) {
+            const int64_t d = (int64_t)a.p.q_start[i + 1] - a.p.q_start[i];
+            n = d > 0 && d <= a.p.max_new && d * a.group > a.few_rows ? (int)((d * a.group + rows - 1) / rows) : 0;
+        }
+        int sum = n;  // tiles of lanes 0..lane
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += x;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, sum > idx);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            const int before = __shfl_sync(0xffffffffu, sum - n, l), count = __shfl_sync(0xffffffffu, n, l);
+            b = hi - 1 - l;
+            tile = count - 1 - (int)(idx - before);
+            return;
+        }
+        idx -= __shfl_sync(0xffffffffu, sum, 31);
+    }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __grid_constant__ AttnView a) {
+    using C = TcCfg<D>;
+    constexpr int NH = D / 64;
+    constexpr uint32_t kFmt = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0u : 1u;
+    // kind::f16: f32 accumulator, A and B of type kFmt; B's rows along the sum for P.V
+    constexpr uint32_t kIdS = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+    constexpr uint32_t kIdPV =
+        (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
+    extern __shared__ char smem_raw[];
+    __shared__ __align__(8) unsigned long long q_full, kv_full[kTcStages], kv_empty[kTcStages], s_full[2], p_full[2],
+        o_full[2];
+    __shared__ unsigned tmem_slot;
+    __shared__ int failed;
+    __shared__ int64_t place[2][128];
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31, wg = t >> 7;
+    pdl_wait();
+    pdl_trigger();
+    int64_t idx = blockIdx.x;
+    const int split = (int)(idx % a.many.splits);
+    idx /= a.many.splits;
+    const int kvh = (int)(idx % a.p.kv_heads);
+    idx /= a.p.kv_heads;
+    int b, tile;
+    find_tile(a, idx, kTcRows, lane, b, tile);
+    if (b < 0) return;
+    const PagedSeq s = paged_seq(a.p, b);
+    const int rows = s.n * a.group, r0 = tile * kTcRows;
+    if (r0 >= rows) return;
+    const KeyRange kr = key_range(a, s, r0, kTcRows);
+    if (split >= splits_used(a.many, kr)) return;
+    const int k_begin = kr.base + split * a.many.len, k_end = min(k_begin + a.many.len, kr.hi);
+    // key tiles of each row tile
+    int nt[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int last = min(r0 + 128 * (i + 1), rows) - 1;
+        const int top = r0 + 128 * i < rows ? min(s.len - s.n + last / a.group + 1, k_end) : k_begin;
+        nt[i] = max(0, (top - k_begin + 127) / 128);
+    }
+    const int nmax = max(nt[0], nt[1]);
+
+    const unsigned sb = (smem_addr(smem_raw) + 1023u) & ~1023u;
+    if (t == 0) {
+        mbar_init(smem_addr(&q_full), 128);
+        for (int i = 0; i < kTcStages; i++) {
+            mbar_init(smem_addr(&kv_full[i]), 128);
+            mbar_init(smem_addr(&kv_empty[i]), 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(smem_addr(&s_full[i]), 1);
+            mbar_init(smem_addr(&p_full[i]), 128);
+            mbar_init(smem_addr(&o_full[i]), 1);
+        }
+        failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned tm = tmem_slot;
+
+    if (wg < 2) {
+        // ------------------------------------------------------ softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        const int r = r0 + t;  // tile wg's row t % 128
+        const bool live = r < rows;
+        const int pos = live ? s.len - s.n + r / a.group : -1;
+        const unsigned lanes = (unsigned)(32 * (warp & 3)) << 16;
+        const unsigned tS = tm + 128u * wg + lanes, tO = tm + C::kO + 128u * wg + lanes;
+        const float sc = fabsf(a.scale_log2);
+        const bool flip = a.scale_log2 < 0.f;
+        float m = -INFINITY, l = 0.f;  // m: the maximum the sums are relative to
+        const int n = nt[wg];
+        bool ok = true;
+        for (int j = 0; j < n && ok; j++) {
+            ok = tc_wait(smem_addr(&s_full[wg]), (unsigned)j & 1u, &failed);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            float x[128];
+#pragma unroll
+            for (int c = 0; c < 4; c++) tmem_ld32(tS + 32 * c, x + 32 * c);
+            if (flip) {
+#pragma unroll
+                for (int c = 0; c < 128; c++) x[c] = -x[c];
+            }
+            // columns this row sees: lo .. hi
+            const int k0 = k_begin + j * 128;
+            const int hi = min(pos, k_end - 1) - k0, lo = a.window > 0 ? pos - a.window + 1 - k0 : 0;
+            if (__any_sync(0xffffffffu, hi < 127 || lo > 0)) {
+#pragma unroll
+                for (int c = 0; c < 128; c++) x[c] = c <= hi && c >= lo ? x[c] : -INFINITY;
+            }
+            float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+            for (int c = 4; c < 128; c += 4)
+#pragma unroll
+                for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], x[c + e]);
+            const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+            const bool raise = mt > m + 8.f || (m == -INFINITY && mt > m);
+            if (__any_sync(0xffffffffu, raise)) {
+                const float mn = raise ? mt : m;
+                const float f = m == -INFINITY ? 0.f : ex2_approx(m - mn);
+                l *= f;
+                m = mn;
+                if (j > 0) {
+#pragma unroll
+                    for (int c = 0; c < D; c += 32) {
+                        float o[32];
+                        tmem_ld32(tO + c, o);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] *= f;
+                        tmem_st32(tO + c, reinterpret_cast<const uint32_t*>(o));
+                    }
+                }
+            }
+            const float mb = m == -INFINITY ? 0.f : m;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                uint32_t w[32];
+#pragma unroll
+                for (int c = 0; c < 64; c += 2) {
+                    const int i = 64 * h + c;
+                    const float p0 = ex2_approx(fmaf(x[i], sc, -mb));
+                    const float p1 = ex2_approx(fmaf(x[i + 1], sc, -mb));
+                    sum[c & 2] += p0;
+                    sum[(c & 2) + 1] += p1;
+                    w[c / 2] = pack2<T>(p0, p1);
+                }
+                tmem_st32(tS + 32 * h, w);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            mbar_arrive(smem_addr(&p_full[wg]), 1);
+        }
+        if (n > 0) ok = tc_wait(smem_addr(&o_full[wg]), 0u, &failed) && ok;
+        ok = __all_sync(0xffffffffu, ok);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const bool last = a.many.splits == 1;
+        const float inv = last ? (l > 0.f ? 1.f / l : 0.f) : 1.f;
+        const int rr = min(r, rows - 1);
+        const int token = s.start + rr / a.group, head = kvh * a.group + rr % a.group;
+        const int64_t th = (int64_t)token * a.heads + head;
+        const int64_t pth = (int64_t)split * a.p.tokens * a.heads + th;
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+            float o[32];
+            if (n > 0) {
+                tmem_ld32(tO + c, o);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; e++) o[e] = 0.f;
+            }
+            if (live && ok) {
+#pragma unroll
+                for (int e = 0; e < 32; e++) o[e] = l > 0.f ? o[e] * inv : 0.f;
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    if (last)
+                        Eight<T>::store(a.out + token * a.o_row + head * a.o_head + (c + e) * sizeof(T), o + e);
+                    else
+                        Eight<float>::store(a.part + pth * D + c + e, o + e);
+                }
+            }
+        }
+        if (live && ok) {
+            if (!last)
+                a.part_ml[pth] = make_float2(l > 0.f ? m : -INFINITY, l);
+            else if (a.lse)
+                a.lse[th] = l > 0.f ? (m + log2f(l)) * 0.693147180559945309f : -INFINITY;
+        }
+    } else if (wg == 2) {
+        // ----------------------------------------------------- producers
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        const int pt = t & 127;
+        constexpr int RC = D / 8, RPP = 128 / RC;  // 16-byte chunks of a row, rows a pass of the 128 threads takes
+        const int pr = pt / RC, pc = pt % RC;
+        // chunk c of row r in a tile: half c / 8, swizzled inside its 128 bytes
+        const unsigned col = (unsigned)(pc >> 3) * C::kHalf;
+        auto at = [&](int r) { return (unsigned)(r * 128 + (((pc & 7) ^ (r & 7)) << 4)) + col; };
+        for (int i = 0; i < 2; i++) {
+            if (nt[i] == 0) continue;
+            for (int r = pr; r < 128; r += RPP) {
+                const int row = r0 + 128 * i + r;
+                const bool real = row < rows;
+                const int x = real ? row : 0;
+                cp_async16(sb + i * C::kTile + at(r),
+                           a.q + (int64_t)(s.start + x / a.group) * a.q_row +
+                               (int64_t)(kvh * a.group + x % a.group) * a.q_head + pc * 16,
+                           real);
+            }
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(smem_addr(&q_full), 1);
+        auto look_up = [&](int j) -> int64_t {
+            const int key = k_begin + j * 128 + pt;
+            return j < nmax && key >= kr.lo && key < k_end ? paged_offset(a.p, b, key) : -1;
+        };
+        auto publish = [&](int push) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(smem_addr(&kv_full[push % kTcStages]), 1);
+        };
+        const int64_t head_off = (int64_t)kvh * a.p.stride_head + pc * 16;
+        int64_t next = look_up(0);
+        bool ok = true;
+        int done = 0, push = 0;
+        for (int j = 0; j < nmax; j++) {
+            place[j & 1][pt] = next;
+            next = look_up(j + 1);
+            // (the other buffer's last readers passed this barrier's previous use)
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll 1
+            for (int kv = 0; kv < 2; kv++, push++) {
+                const int st = push % kTcStages;
+                if (push >= kTcStages)
+                    ok = tc_wait(smem_addr(&kv_empty[st]), (unsigned)(push / kTcStages - 1) & 1u, &failed) && ok;
+                const char* src = kv ? a.p.v : a.p.k;
+                const unsigned dst = sb + C::kOffKV + st * C::kTile;
+                if (ok) {
+#pragma unroll 4
+                    for (int r = pr; r < 128; r += RPP) {
+                        const int64_t o = place[j & 1][r];
+                        cp_async16(dst + at(r), src + (o < 0 ? 0 : o + head_off), o >= 0);
+                    }
+                }
+                cp_async_commit();
+                if (push >= 2) {
+                    cp_async_wait<2>();
+                    publish(done++);
+                }
+            }
+        }
+        cp_async_wait<0>();
+        while (done < push) publish(done++);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (t == 384 && nmax > 0) {
+            // ---------------------------------------------------- products
+            bool ok = tc_wait(smem_addr(&q_full), 0u, &failed);
+            auto wait_kv = [&](int push) {
+                ok = ok && tc_wait(smem_addr(&kv_full[push % kTcStages]), (unsigned)(push / kTcStages) & 1u, &failed);
+            };
+            auto qk = [&](int i, int j) {
+                if (ok) {
+                    const unsigned kb = sb + C::kOffKV + (2 * j % kTcStages) * C::kTile;
+#pragma unroll
+                    for (int h = 0; h < NH; h++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            mma_f16(tm + 128u * i, sw128_desc(sb + i * C::kTile + h * C::kHalf + 32u * k),
+                                    sw128_desc(kb + h * C::kHalf + 32u * k), kIdS, h > 0 || k > 0);
+                }
+                mma_commit(smem_addr(&s_full[i]));
+            };
+            wait_kv(0);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for (int i = 0; i < 2; i++)
+                if (nt[i] > 0) qk(i, 0);
+            mma_commit(smem_addr(&kv_empty[0]));
+            for (int j = 0; j < nmax; j++) {
+                wait_kv(2 * j + 1);
+                const unsigned vb = sb + C::kOffKV + ((2 * j + 1) % kTcStages) * C::kTile;
+                if (j + 1 < nmax) wait_kv(2 * j + 2);
+                for (int i = 0; i < 2; i++) {
+                    if (j >= nt[i]) continue;
+                    ok = ok && tc_wait(smem_addr(&p_full[i]), (unsigned)j & 1u, &failed);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (ok) {
+#pragma unroll
+                        for (int k = 0; k < 8; k++)
+                            mma_f16_ta(tm + C::kO + 128u * i, tm + 128u * i + 8u * k, sw128_desc_mn(vb + 2048u * k), kIdPV,
+                                       j > 0 || k > 0);
+                    }
+                    if (j + 1 < nt[i])
+                        qk(i, j + 1);
+                    else
+                        mma_commit(smem_addr(&o_full[i]));
+                }
+                mma_commit(smem_addr(&kv_empty[(2 * j + 1) % kTcStages]));
+                if (j + 1 < nmax) mma_commit(smem_addr(&kv_empty[(2 * j + 2) % kTcStages]));
+            }
+            // every product has landed before the tensor memory goes
+            for (int i = 0; i < 2; i++)
+                if (nt[i] > 0) tc_wait(smem_addr(&o_full[i]), 0u, nullptr);
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 12)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512) : "memory");
+    if (t == 0 && failed) paged_report(a.p, VB_PAGED_TIMEOUT);
+}
+
 // Joins the splits of a row: a warp per (token, head), grid over them.
 template <typename IO, int D>
-__global__ void __launch_bounds__(128) paged_attn_merge_kernel(const __grid_constant__ AttnView a, int tile_rows) {
+__global__ void __launch_bounds__(128) paged_attn_merge_kernel(const __grid_constant__ AttnView a) {
     pdl_wait();
     pdl_trigger();
     const int lane = threadIdx.x & 31;
@@ -530,7 +948,9 @@ __global__ void __launch_bounds__(128) paged_attn_merge_kernel(const __grid_cons
     const PagedSeq s = paged_seq(a.p, b);
     if (!s.ok || token < s.start || token >= s.start + s.n) return;
     const int r = (token - s.start) * a.group + head % a.group;
-    const int used = splits_used(a, key_range(a, s, r / tile_rows * tile_rows, tile_rows));
+    const Cut& cut = s.n * a.group > a.few_rows ? a.many : a.few;
+    if (cut.splits == 1) return;  // written by the kernel itself
+    const int used = splits_used(cut, key_range(a, s, r / cut.rows * cut.rows, cut.rows));
     constexpr int E = D / 32;
     float y[E] = {}, M = -INFINITY, L = 0.f;
     const int64_t step = (int64_t)a.p.tokens * a.heads;
@@ -554,28 +974,50 @@ __global__ void __launch_bounds__(128) paged_attn_merge_kernel(const __grid_cons
 
 // How the work is cut up: from the host's bounds alone, so that a captured
 // launch holds for any lengths within them.  A tile's keys are split where the
-// tiles alone do not fill the card: about four CTAs for each SM (two run at a
-// time), of at least 64 keys, one block of 16 a warp.
+// tiles alone do not fill the card.
 struct Plan {
-    int row_tiles, splits, split_len;
+    int few_rows, row_tiles;
+    Cut few, many;
     int max_splits;  // for any window
 };
-Plan make_plan(const PagedView& p, int heads, int window) {
+constexpr int kFewRows = 32;
+
+Cut make_cut(int rows, int64_t keys, int64_t want, int step, int least) {
+    Cut c;
+    c.rows = rows;
+    const int64_t n = std::max<int64_t>(1, std::min<int64_t>(want, (keys + least - 1) / least));
+    c.len = (int)(((keys + n - 1) / n + step - 1) / step * step);
+    c.splits = (int)((keys + c.len - 1) / c.len);
+    return c;
+}
+
+Plan make_plan(const PagedView& p, int io, int cache, int heads, int window) {
     Plan pl{};
     const int G = heads / p.kv_heads;
-    pl.row_tiles = (int)(((int64_t)p.max_new * G + 15) / 16);
+    const int64_t most = (int64_t)p.max_new * G, total = (int64_t)p.tokens * G;  // rows of a KV head
+    // 16-bit rows on the tensor cores' 256-row tiles from 33 rows a sequence on; one
+    // sequence alone takes one kernel for all it may hold
+    const bool tc = io != VB_F32 && most > kFewRows;
+    pl.few_rows = !tc ? 0x7fffffff : p.batch == 1 ? 0 : kFewRows;
+    const int64_t few_most = std::min<int64_t>(most, pl.few_rows);
+    pl.row_tiles = (int)((few_most + 15) / 16);
     const int64_t all = std::max(p.max_len, 1);
-    int64_t span = all;  // keys from a tile's base (lo rounded down to 16) to its last row's
-    if (window > 0) span = std::min<int64_t>(span, (int64_t)window + 30);
-    // tiles that can hold rows
-    const int64_t tiles =
-        std::max<int64_t>(1, std::min<int64_t>((int64_t)p.batch * pl.row_tiles,
-                                               (int64_t)p.tokens * G / 16 + p.batch)) * p.kv_heads;
-    const int64_t want = std::max<int64_t>(1, 148 * 4 / tiles);
-    pl.max_splits = (int)std::min<int64_t>(want, (all + 63) / 64);
-    const int64_t n = std::min<int64_t>(want, (span + 63) / 64);
-    pl.split_len = (int)(((span + n - 1) / n + 63) / 64 * 64);
-    pl.splits = (int)((span + pl.split_len - 1) / pl.split_len);
+    // keys from a tile's base (its first row's lowest, rounded down to 16) to its last row's
+    auto span = [&](int rows) {
+        return window > 0 ? std::min<int64_t>(all, (int64_t)window + (rows + G - 1) / G + 15) : all;
+    };
+    // few rows: about four CTAs for each SM (two run at a time) of at least 64 keys, one block of
+    // 16 a warp; many: one CTA for each SM of at least 512 keys
+    const int64_t tiles = std::max<int64_t>(1, std::min<int64_t>((int64_t)p.batch * pl.row_tiles, total / 16 + p.batch));
+    const int64_t want = std::max<int64_t>(1, 148 * 4 / (tiles * p.kv_heads));
+    pl.few = make_cut(16, span(16), want, 64, 64);
+    const int64_t tiles2 = std::max<int64_t>(1, (total + kTcRows - 1) / kTcRows);
+    const int64_t want2 = std::max<int64_t>(1, 148 / (tiles2 * p.kv_heads));
+    pl.many = make_cut(kTcRows, span(kTcRows), want2, 128, 512);
+    pl.max_splits = (int)std::max<int64_t>(pl.few_rows ? std::min<int64_t>(want, (all + 63) / 64) : 1,
+                                           tc ? std::min<int64_t>(want2, (all + 511) / 512) : 1);
+    if (!tc) pl.many.splits = 1;
+    if (!pl.few_rows) pl.few.splits = 1;
     return pl;
 }
 size_t plan_bytes(const Plan& pl, const PagedView& p, int heads, int D) {
@@ -583,19 +1025,36 @@ size_t plan_bytes(const Plan& pl, const PagedView& p, int heads, int D) {
 }
 
 template <typename IO, typename KV, int D>
-vb_status launch_few(const AttnView& a, cudaStream_t s) {
-    using C = FewCfg<KV, D>;
-    static std::atomic<unsigned long long> done{0};
-    cudaError_t e = smem_attr_once(paged_attn_few_kernel<IO, KV, D>, C::kSmem, done);
-    if (e != cudaSuccess) return cuda_fail(e, "paged attention: shared memory attribute");
-    const int64_t grid = (int64_t)a.splits * a.p.kv_heads * a.row_tiles * a.p.batch;
-    if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
-    e = launch_pdl(paged_attn_few_kernel<IO, KV, D>, dim3((unsigned)grid), dim3(kFewWarps * 32), C::kSmem, s, a);
-    if (e != cudaSuccess) return cuda_fail(e, "paged_attn_few_kernel");
-    if (a.splits > 1) {
-        const int64_t g2 = ((int64_t)a.p.tokens * a.heads + 3) / 4;
-        if (g2 > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
-        e = launch_pdl(paged_attn_merge_kernel<IO, D>, dim3((unsigned)g2), dim3(128), 0, s, a, 16);
+vb_status launch_attn(const AttnView& a, cudaStream_t s) {
+    cudaError_t e;
+    if constexpr (sizeof(IO) == 2) {
+        if (a.few_rows != 0x7fffffff) {
+            static std::atomic<unsigned long long> done{0};
+            e = smem_attr_once(paged_attn_tc_kernel<IO, D>, TcCfg<D>::kSmem, done);
+            if (e != cudaSuccess) return cuda_fail(e, "paged attention: shared memory attribute");
+            const int64_t tiles = std::min<int64_t>(
+                (int64_t)a.p.batch * (((int64_t)a.p.max_new * a.group + kTcRows - 1) / kTcRows),
+                (int64_t)a.p.tokens * a.group / kTcRows + a.p.batch);
+            const int64_t grid = tiles * a.many.splits * a.p.kv_heads;
+            if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
+            e = launch_pdl(paged_attn_tc_kernel<IO, D>, dim3((unsigned)grid), dim3(kTcThreads), TcCfg<D>::kSmem, s, a);
+            if (e != cudaSuccess) return cuda_fail(e, "paged_attn_tc_kernel");
+        }
+    }
+    if (a.few_rows) {
+        using C = FewCfg<KV, D>;
+        static std::atomic<unsigned long long> done{0};
+        e = smem_attr_once(paged_attn_few_kernel<IO, KV, D>, C::kSmem, done);
+        if (e != cudaSuccess) return cuda_fail(e, "paged attention: shared memory attribute");
+        const int64_t grid = (int64_t)a.few.splits * a.p.kv_heads * a.row_tiles * a.p.batch;
+        if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
+        e = launch_pdl(paged_attn_few_kernel<IO, KV, D>, dim3((unsigned)grid), dim3(kFewWarps * 32), C::kSmem, s, a);
+        if (e != cudaSuccess) return cuda_fail(e, "paged_attn_few_kernel");
+    }
+    if (a.few.splits > 1 || a.many.splits > 1) {
+        const int64_t grid = ((int64_t)a.p.tokens * a.heads + 3) / 4;
+        if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
+        e = launch_pdl(paged_attn_merge_kernel<IO, D>, dim3((unsigned)grid), dim3(128), 0, s, a);
         if (e != cudaSuccess) return cuda_fail(e, "paged_attn_merge_kernel");
     }
     VB_LAUNCH_CHECK("paged attention");
@@ -604,10 +1063,10 @@ vb_status launch_few(const AttnView& a, cudaStream_t s) {
 
 template <int D>
 vb_status launch_attn(const AttnView& a, int io, int cache, cudaStream_t s) {
-    if (io == VB_F32 && cache == VB_F32) return launch_few<float, float, D>(a, s);
-    if (io == VB_F32) return launch_few<float, __nv_bfloat16, D>(a, s);
-    if (io == VB_F16) return launch_few<__half, __half, D>(a, s);
-    return launch_few<__nv_bfloat16, __nv_bfloat16, D>(a, s);
+    if (io == VB_F32 && cache == VB_F32) return launch_attn<float, float, D>(a, s);
+    if (io == VB_F32) return launch_attn<float, __nv_bfloat16, D>(a, s);
+    if (io == VB_F16) return launch_attn<__half, __half, D>(a, s);
+    return launch_attn<__nv_bfloat16, __nv_bfloat16, D>(a, s);
 }
 
 }  // namespace
@@ -618,7 +1077,11 @@ using namespace vb;
 extern "C" size_t vb_paged_attn_workspace_bytes(const vb_paged_cache* cache, const vb_paged_batch* batch, int heads) {
     PagedView p{};
     if (!cache || paged_view(cache, batch, cache->dtype, heads, "paged_attn", &p) || !p.batch || !p.tokens) return 0;
-    return plan_bytes(make_plan(p, heads, 0), p, heads, cache->head_dim);
+    size_t most = 0;  // rows of the cache's type or, over a bf16 cache, f32
+    for (const int io : {cache->dtype, (int)VB_F32})
+        if (io == cache->dtype || cache->dtype == VB_BF16)
+            most = std::max(most, plan_bytes(make_plan(p, io, cache->dtype, heads, 0), p, heads, cache->head_dim));
+    return most;
 }
 
 extern "C" vb_status vb_paged_attn(const vb_paged_cache* cache, const vb_paged_batch* batch, int io, int heads,
@@ -634,7 +1097,7 @@ extern "C" vb_status vb_paged_attn(const vb_paged_cache* cache, const vb_paged_b
     const int es = paged_elem_bytes(io), D = cache->head_dim;
     if (!paged_aligned(q, q_row, q_head, es) || !paged_aligned(out, o_row, o_head, es) || !paged_aligned(workspace, 0, 0, 1))
         return fail(VB_ERR_UNSUPPORTED, "paged_attn: 16-byte alignment required");
-    const Plan pl = make_plan(a.p, heads, window);
+    const Plan pl = make_plan(a.p, io, cache->dtype, heads, window);
     const size_t need = plan_bytes(pl, a.p, heads, D);
     if (need > workspace_bytes || (need && !workspace))
         return fail(VB_ERR_ARG, "paged_attn: the workspace is too small");
@@ -644,13 +1107,15 @@ extern "C" vb_status vb_paged_attn(const vb_paged_cache* cache, const vb_paged_b
     a.lse = lse;
     a.heads = heads;
     a.group = heads / cache->kv_heads;
-    a.scale_log2 = scale * 1.44269504088896341f;
+    // a scale of 0 as one that no score outgrows: a masked score stays -inf under it
+    a.scale_log2 = (scale == 0.f ? 1.17549435e-38f : scale) * 1.44269504088896341f;
     a.window = window;
+    a.few_rows = pl.few_rows;
     a.row_tiles = pl.row_tiles;
-    a.splits = pl.splits;
-    a.split_len = pl.split_len;
+    a.few = pl.few;
+    a.many = pl.many;
     a.part = static_cast<float*>(workspace);
-    a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)pl.splits * a.p.tokens * heads * D);
+    a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)pl.max_splits * a.p.tokens * heads * D);
     return D == 128 ? launch_attn<128>(a, io, cache->dtype, as_stream(stream))
                     : launch_attn<64>(a, io, cache->dtype, as_stream(stream));
 }

@@ -576,8 +576,17 @@ def argmax_rows(logits, out_idx, stream=None):
 
 # -- paged serving and logits rules on torch CUDA tensors ----------------------
 
-PAGED_BAD_ROWS, PAGED_BAD_LEN, PAGED_BAD_PAGE = 1, 2, 4  # bits of a PagedBatch's status word
-_DTYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}  # VB_F32, VB_F16, VB_BF16
+PAGED_BAD_ROWS, PAGED_BAD_LEN, PAGED_BAD_PAGE, PAGED_TIMEOUT = 1, 2, 4, 8  # bits of a PagedBatch's status word
+# torch dtype -> VB_F32, VB_F16, VB_BF16 (_I32 for int32); filled when torch is there
+_TYPE = {}
+_I32 = 100
+
+
+def _types():
+    if not _TYPE:
+        import torch
+        _TYPE.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int32: _I32})
+    return _TYPE
 
 
 def _refuse(msg):
@@ -585,33 +594,33 @@ def _refuse(msg):
 
 
 def _dtype(t, what):
-    d = _DTYPES.get(str(t.dtype))
-    if d is None:
+    d = _types().get(t.dtype, _I32)
+    if d == _I32:
         _refuse(f"{what}: float32, float16 or bfloat16, not {t.dtype}")
     return d
 
 
-def _here(device):
-    """Memory of a paged call lies on the current device: its kernels run there."""
+def _here(index):
+    """Memory of these calls lies on the current device: their kernels run there."""
     import torch
-    if device.type != "cuda" or device.index != torch.cuda.current_device():
-        _refuse(f"tensors on {device}: the current CUDA device's are needed")
+    if index < 0 or index != torch.cuda.current_device():
+        _refuse("tensors of the current CUDA device are needed")
 
 
-def _array(t, dtype, device, what, ndim=1):
-    """An optional contiguous device array; its address or None."""
+def _array(t, dtype, index, what, ndim=1):
+    """A contiguous array of type `dtype` on device `index`, or None; its address or None."""
     if t is None:
         return None
-    if str(t.dtype) != dtype or t.device != device or t.dim() != ndim or not t.is_contiguous():
-        _refuse(f"{what}: a contiguous {ndim}-d {dtype} tensor on {device} is needed")
+    if _types().get(t.dtype) != dtype or t.get_device() != index or t.dim() != ndim or not t.is_contiguous():
+        _refuse(f"{what}: a contiguous {ndim}-d {'int32' if dtype == _I32 else 'float32'} tensor on the same device is needed")
     return t.data_ptr()
 
 
-def _raw_stream(stream, device):
+def _raw_stream(stream, index):
     if stream is not None:
         return int(stream)
     import torch
-    return torch._C._cuda_getCurrentRawStream(device.index)
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 class PagedCache:
@@ -623,8 +632,9 @@ class PagedCache:
             _refuse("paged cache: k and v are 4-d and alike in shape, strides, type and device")
         if k.stride(3) != 1:
             _refuse("paged cache: the head dim is contiguous")
-        _here(k.device)
-        self.k, self.v, self.device, self.dtype = k, v, k.device, _dtype(k, "paged cache")
+        self.index = k.get_device()
+        _here(self.index)
+        self.k, self.v, self.dtype = k, v, _dtype(k, "paged cache")
         self.pages, self.page_size, self.kv_heads, self.head_dim = k.shape
         self.s = VBPagedCache(k.data_ptr(), v.data_ptr(), self.dtype, self.pages, self.page_size, self.kv_heads,
                               self.head_dim, k.stride(0), k.stride(1), k.stride(2))
@@ -637,43 +647,41 @@ class PagedBatch:
     optional int32 status word.  The tensors may change between calls; the bounds hold."""
 
     def __init__(self, q_start, lens, table, *, max_new, max_len, tokens, status=None):
-        dev = lens.device
+        dev = self.index = lens.get_device()
         _here(dev)
         B = lens.shape[0] if lens.dim() == 1 else -1
         if q_start.shape != (B + 1,) or table.dim() != 2 or table.shape[0] != B or (B and table.stride(1) != 1):
             _refuse("paged batch: q_start [B + 1], lens [B] and table [B, pages] (contiguous rows)")
-        if str(table.dtype) != "torch.int32" or table.device != dev or (status is not None and status.numel() != 1):
+        if _types().get(table.dtype) != _I32 or table.get_device() != dev or (status is not None and status.numel() != 1):
             _refuse("paged batch: table is int32 beside lens, status one int32")
-        ps = None if status is None else _array(status.reshape(1), "torch.int32", dev, "status")
+        ps = None if status is None else _array(status.reshape(1), _I32, dev, "status")
         self.q_start, self.lens, self.table, self.status = q_start, lens, table, status
-        self.device, self.tokens = dev, int(tokens)
-        # a row of the table reaches at most to the next one's start
-        width = table.shape[1] if B <= 1 else min(table.shape[1], table.stride(0))
+        self.tokens, self.max_len, self.width = int(tokens), int(max_len), table.shape[1]
         if B > 1 and table.stride(0) < table.shape[1]:
             _refuse("paged batch: rows of the table overlap")
-        self.width = width
         self.s = VBPagedBatch(B, self.tokens, int(max_new), int(max_len),
-                              _array(q_start, "torch.int32", dev, "q_start"),
-                              _array(lens, "torch.int32", dev, "lens"), table.data_ptr(),
+                              _array(q_start, _I32, dev, "q_start"),
+                              _array(lens, _I32, dev, "lens"), table.data_ptr(),
                               table.stride(0) if B > 1 else table.shape[1], ps)
         self.ref = C.addressof(self.s)
 
 
 def _paged_pair(cache, batch):
-    if batch.device != cache.device:
+    if batch.index != cache.index:
         _refuse("the batch and the cache are on different devices")
-    if batch.s.max_len > batch.width * cache.page_size:
+    if batch.max_len > batch.width * cache.page_size:
         _refuse("paged batch: max_len is more than the table's pages hold")
-    _here(cache.device)
+    _here(cache.index)
 
 
 def _paged_rows(t, cache, batch, heads, dtype, what):
-    if (t.dim() != 3 or t.shape[0] != batch.tokens or t.shape[2] != cache.head_dim or t.stride(2) != 1
-            or (heads is not None and t.shape[1] != heads) or t.device != cache.device
-            or (dtype is not None and t.dtype != dtype)):
+    """Rows [tokens, heads, head_dim] of type `dtype`: their address, row and head stride."""
+    st = t.stride()
+    if (len(st) != 3 or st[2] != 1 or t.shape != (batch.tokens, heads, cache.head_dim) or t.dtype != dtype
+            or t.get_device() != cache.index):
         _refuse(f"{what}: [tokens, heads, head_dim] rows of the batch are needed, "
                 "the head dim contiguous, all of one type, on the cache's device")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+    return t.data_ptr(), st[0], st[1]
 
 
 def paged_append(cache, batch, k, v, q=None, q_out=None, cos=None, sin=None, interleaved=False, q_norm=None,
@@ -681,35 +689,29 @@ def paged_append(cache, batch, k, v, q=None, q_out=None, cos=None, sin=None, int
     """Appends the batch's new keys (normed by k_norm and rotated by cos / sin [positions, rot] on
     the way) and values to their pages; q normed and rotated the same way goes to q_out."""
     _paged_pair(cache, batch)
-    dev = cache.device
-    kp = _paged_rows(k, cache, batch, cache.kv_heads, None, "k")
-    vp = _paged_rows(v, cache, batch, cache.kv_heads, k.dtype, "v")
+    dev, kvh, dt = cache.index, cache.kv_heads, k.dtype
+    kp = _paged_rows(k, cache, batch, kvh, dt, "k")
+    vp = _paged_rows(v, cache, batch, kvh, dt, "v")
     qp = op = (None, 0, 0)
     heads = 0
     if (q is None) != (q_out is None):
         _refuse("q and q_out come together")
     if q is not None:
-        heads = q.shape[1]
-        qp = _paged_rows(q, cache, batch, None, k.dtype, "q")
-        op = _paged_rows(q_out, cache, batch, heads, k.dtype, "q_out")
-    rope = VBPagedRope()
+        heads = q.shape[1] if q.dim() == 3 else 0
+        qp = _paged_rows(q, cache, batch, heads, dt, "q")
+        op = _paged_rows(q_out, cache, batch, heads, dt, "q_out")
     if (cos is None) != (sin is None):
         _refuse("cos and sin come together")
+    positions = rot = 0
     if cos is not None:
-        if cos.shape != sin.shape:
-            _refuse("cos and sin are alike in shape")
-        rope.cos_tab = _array(cos, "torch.float32", dev, "cos", 2)
-        rope.sin_tab = _array(sin, "torch.float32", dev, "sin", 2)
-        rope.rope_positions, rope.rot = cos.shape
-        rope.interleaved = int(bool(interleaved))
+        if cos.shape != sin.shape or cos.dim() != 2:
+            _refuse("cos and sin are alike: [positions, rot]")
+        positions, rot = cos.shape
     for n in (q_norm, k_norm):
-        if n is not None and n.shape != (cache.head_dim,):
+        if n is not None and n.numel() != cache.head_dim:
             _refuse("q_norm / k_norm: [head_dim]")
-    if q_norm is not None:
-        rope.q_norm = _array(q_norm, "torch.float32", dev, "q_norm")
-    if k_norm is not None:
-        rope.k_norm = _array(k_norm, "torch.float32", dev, "k_norm")
-    rope.eps = eps
+    rope = VBPagedRope(_array(cos, 0, dev, "cos", 2), _array(sin, 0, dev, "sin", 2), positions, rot,
+                       1 if interleaved else 0, _array(q_norm, 0, dev, "q_norm"), _array(k_norm, 0, dev, "k_norm"), eps)
     check(lib().vb_paged_append(cache.ref, batch.ref, C.addressof(rope), _dtype(k, "k"), heads, *qp, *op, *kp, *vp,
                                 _raw_stream(stream, dev)))
 
@@ -723,7 +725,8 @@ def paged_attn_workspace_bytes(cache, batch, heads):
 def paged_attn_workspace(cache, batch, heads):
     """A workspace for paged_attn, on the cache's device."""
     import torch
-    return torch.empty(paged_attn_workspace_bytes(cache, batch, heads), dtype=torch.uint8, device=cache.device)
+    return torch.empty(paged_attn_workspace_bytes(cache, batch, heads), dtype=torch.uint8,
+                       device=cache.k.device)
 
 
 def paged_attn(cache, batch, q, out, lse=None, scale=None, window=0, workspace=None, stream=None):
@@ -731,19 +734,19 @@ def paged_attn(cache, batch, q, out, lse=None, scale=None, window=0, workspace=N
     each sees its last `window` positions only; lse: f32 [tokens, heads].  workspace: from
     paged_attn_workspace (one is made for the call when None)."""
     _paged_pair(cache, batch)
-    heads = q.shape[1] if q.dim() == 3 else 0
-    qp = _paged_rows(q, cache, batch, None, None, "q")
+    dev, heads = cache.index, q.shape[1] if q.dim() == 3 else 0
+    qp = _paged_rows(q, cache, batch, heads, q.dtype, "q")
     op = _paged_rows(out, cache, batch, heads, q.dtype, "out")
     if lse is not None and lse.shape != (batch.tokens, heads):
         _refuse("lse: f32 [tokens, heads]")
     if workspace is None:
         workspace = paged_attn_workspace(cache, batch, heads)
-    elif workspace.device != cache.device or not workspace.is_contiguous():
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
         _refuse("workspace: contiguous memory on the cache's device")
     check(lib().vb_paged_attn(cache.ref, batch.ref, _dtype(q, "q"), heads, *qp, *op,
-                              _array(lse, "torch.float32", cache.device, "lse", 2),
+                              _array(lse, 0, dev, "lse", 2),
                               cache.head_dim ** -0.5 if scale is None else scale, window, workspace.data_ptr(),
-                              workspace.numel() * workspace.element_size(), _raw_stream(stream, cache.device)))
+                              workspace.numel() * workspace.element_size(), _raw_stream(stream, dev)))
 
 
 class LogitsRules:
@@ -759,40 +762,41 @@ class LogitsRules:
             _refuse("hist_start and hist_ids come together")
         if len({bias_start is None, bias_ids is None, bias_vals is None}) > 1:
             _refuse("bias_start, bias_ids and bias_vals come together")
-        self.device = given[0].device if given else None
+        self.index = given[0].get_device() if given else None
         if given:
-            _here(self.device)
+            _here(self.index)
         rows = {t.shape[0] - (t is hist_start or t is bias_start) for t in given if t.dim()}
         if len(rows) > 1:
             _refuse("the rules are not all for the same number of rows")
         self.rows = rows.pop() if rows else None
         if bias_ids is not None and bias_ids.shape != bias_vals.shape:
             _refuse("bias_ids and bias_vals are alike in shape")
-        d = self.device
+        d = self.index
         self.keep = (hist_start, hist_ids, prompt_len, repetition, frequency, presence, bias_start, bias_ids,
                      bias_vals, mask)
         self.words = None if mask is None else mask.shape[1]
         self.s = VBLogitsRules(
-            _array(hist_start, "torch.int32", d, "hist_start"), _array(hist_ids, "torch.int32", d, "hist_ids"),
-            0 if hist_ids is None else hist_ids.numel(), _array(prompt_len, "torch.int32", d, "prompt_len"),
-            _array(repetition, "torch.float32", d, "repetition"), _array(frequency, "torch.float32", d, "frequency"),
-            _array(presence, "torch.float32", d, "presence"), _array(bias_start, "torch.int32", d, "bias_start"),
-            _array(bias_ids, "torch.int32", d, "bias_ids"), _array(bias_vals, "torch.float32", d, "bias_vals"),
-            0 if bias_ids is None else bias_ids.numel(), _array(mask, "torch.int32", d, "mask", 2), self.words or 0)
+            _array(hist_start, _I32, d, "hist_start"), _array(hist_ids, _I32, d, "hist_ids"),
+            0 if hist_ids is None else hist_ids.numel(), _array(prompt_len, _I32, d, "prompt_len"),
+            _array(repetition, 0, d, "repetition"), _array(frequency, 0, d, "frequency"),
+            _array(presence, 0, d, "presence"), _array(bias_start, _I32, d, "bias_start"),
+            _array(bias_ids, _I32, d, "bias_ids"), _array(bias_vals, 0, d, "bias_vals"),
+            0 if bias_ids is None else bias_ids.numel(), _array(mask, _I32, d, "mask", 2), self.words or 0)
         self.ref = C.addressof(self.s)
 
 
 def logits_process(logits, out, rules, stream=None):
     """out = the rules applied to logits [R, V] (f32, f16 or bf16; contiguous rows; out may be logits)."""
-    if logits.dim() != 2 or out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+    st, so, dev = logits.stride(), out.stride(), logits.get_device()
+    if len(st) != 2 or out.shape != logits.shape or out.dtype != logits.dtype or out.get_device() != dev:
         _refuse("logits_process: logits and out are [rows, vocab] and alike")
     R, V = logits.shape
-    if V > 1 and (logits.stride(1) != 1 or out.stride(1) != 1):
+    if V > 1 and (st[1] != 1 or so[1] != 1):
         _refuse("logits_process: rows are contiguous")
-    _here(logits.device)
-    if rules.rows not in (None, R) or rules.device not in (None, logits.device):
+    _here(dev)
+    if rules.rows not in (None, R) or rules.index not in (None, dev):
         _refuse("logits_process: the rules are for other rows, or on another device")
     if rules.words is not None and rules.words < (V + 31) // 32:
         _refuse("logits_process: the mask has too few words")
-    check(lib().vb_logits_process(logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0),
-                                  _dtype(logits, "logits"), R, V, rules.ref, _raw_stream(stream, logits.device)))
+    check(lib().vb_logits_process(logits.data_ptr(), st[0], out.data_ptr(), so[0], _dtype(logits, "logits"), R, V,
+                                  rules.ref, _raw_stream(stream, dev)))
