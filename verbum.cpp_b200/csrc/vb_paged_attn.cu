@@ -565,12 +565,49 @@ __device__ __forceinline__ uint64_t sw128_desc_mn(unsigned saddr) {
     return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((128 * 128) >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
+// Arrives at an mbarrier once this thread's cp.asyncs so far have landed.  The
+// thread that waits for it puts the proxy fence between them and its products.
+__device__ __forceinline__ void cp_async_arrive(unsigned bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
 // D[tmem] (+)= A[tmem] B[smem]
 __device__ __forceinline__ void mma_f16_ta(unsigned tmem, unsigned atmem, uint64_t bdesc, uint32_t idesc, bool acc) {
     asm volatile(
         "{ .reg .pred p; setp.ne.u32 p, %4, 0; "
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(tmem),
         "r"(atmem), "l"(bdesc), "r"(idesc), "r"((unsigned)acc)
+        : "memory");
+}
+// 128 columns of this warp's 32 lanes
+__device__ __forceinline__ void tmem_ld128(unsigned taddr, float* v) {
+    unsigned* r = reinterpret_cast<unsigned*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,  "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31,  "
+        "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47,  "
+        "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%128]; "
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79,  "
+        "%80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95,  "
+        "%96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111,  "
+        "%112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127}, [%129]; "
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
+          "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
+          "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
+          "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
+          "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
+          "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
+          "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
+          "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
+          "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+        : "r"(taddr), "r"(taddr + 64)
         : "memory");
 }
 // 32 columns of this warp's 32 lanes
@@ -718,8 +755,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             if (!__all_sync(0xffffffffu, ok)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             float x[128];
-#pragma unroll
-            for (int c = 0; c < 4; c++) tmem_ld32(tS + 32 * c, x + 32 * c);
+            tmem_ld128(tS, x);
             if (flip) {
 #pragma unroll
                 for (int c = 0; c < 128; c++) x[c] = -x[c];
@@ -832,22 +868,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
                            real);
             }
         }
-        cp_async_commit();
-        cp_async_wait<0>();
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(smem_addr(&q_full), 1);
+        cp_async_arrive(smem_addr(&q_full));
         auto look_up = [&](int j) -> int64_t {
             const int key = k_begin + j * 128 + pt;
             return j < nmax && key >= kr.lo && key < k_end ? paged_offset(a.p, b, key) : -1;
         };
-        auto publish = [&](int push) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(smem_addr(&kv_full[push % kTcStages]), 1);
-        };
         const int64_t head_off = (int64_t)kvh * a.p.stride_head + pc * 16;
         int64_t next = look_up(0);
         bool ok = true;
-        int done = 0, push = 0;
+        int push = 0;
         for (int j = 0; j < nmax; j++) {
             place[j & 1][pt] = next;
             next = look_up(j + 1);
@@ -867,15 +896,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
                         cp_async16(dst + at(r), src + (o < 0 ? 0 : o + head_off), o >= 0);
                     }
                 }
-                cp_async_commit();
-                if (push >= 2) {
-                    cp_async_wait<2>();
-                    publish(done++);
-                }
+                cp_async_arrive(smem_addr(&kv_full[st]));
             }
         }
-        cp_async_wait<0>();
-        while (done < push) publish(done++);
+        cp_async_commit();
+        cp_async_wait<0>();  // nothing in flight when the block ends
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (t == 384 && nmax > 0) {
@@ -883,6 +908,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             bool ok = tc_wait(smem_addr(&q_full), 0u, &failed);
             auto wait_kv = [&](int push) {
                 ok = ok && tc_wait(smem_addr(&kv_full[push % kTcStages]), (unsigned)(push / kTcStages) & 1u, &failed);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             };
             auto qk = [&](int i, int j) {
                 if (ok) {
