@@ -63,9 +63,10 @@ vb_status paged_view(const vb_paged_cache* c, const vb_paged_batch* b, int io, i
 
 namespace {
 
-// How a kernel cuts its work: rows of a tile, and the split of a tile's keys.
+// How a kernel cuts its work: rows of a tile, and the splits of a tile's keys, which
+// start at a multiple of `align`.
 struct Cut {
-    int rows, splits, len;
+    int rows, splits, len, align;
 };
 
 struct AttnView {
@@ -80,23 +81,24 @@ struct AttnView {
     int few_rows;       // sequences with at most this many rows a KV head run in the few-rows kernel
     int row_tiles;      // its row tiles of a sequence
     Cut few, many;
+    int box;            // rows of a page that one TMA copy brings (many rows); 0: no tensor maps
     float* part;        // [split][token][head][D] sums of a split, relative to its maximum
     float2* part_ml;    // [split][token][head] (maximum in base 2, sum of weights)
 };
 
-// The keys that rows r0 .. r0 + count - 1 (of n * G) of a sequence see.
+// The keys that the tile's rows r0 .. r0 + cut.rows - 1 (of n * G) of a sequence see.
 struct KeyRange {
     int lo, hi;  // positions lo .. hi - 1
     int base;    // lo rounded down: where the first split starts
 };
-__device__ __forceinline__ KeyRange key_range(const AttnView& a, const PagedSeq& s, int r0, int count) {
-    const int r1 = min(r0 + count, s.n * a.group) - 1;
+__device__ __forceinline__ KeyRange key_range(const AttnView& a, const PagedSeq& s, int r0, const Cut& cut) {
+    const int r1 = min(r0 + cut.rows, s.n * a.group) - 1;
     const int p0 = s.len - s.n + r0 / a.group, p1 = s.len - s.n + r1 / a.group;
     KeyRange k;
     k.hi = max(p1 + 1, 0);
     k.lo = a.window > 0 ? max(p0 - a.window + 1, 0) : 0;
     k.lo = min(k.lo, k.hi);
-    k.base = k.lo & ~15;
+    k.base = k.lo & -cut.align;
     return k;
 }
 __device__ __forceinline__ int splits_used(const Cut& c, const KeyRange& k) {
@@ -237,7 +239,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
     const PagedSeq s = paged_seq(a.p, b);
     const int rows = s.n * a.group;
     if (r0 >= rows || rows > a.few_rows) return;
-    const KeyRange kr = key_range(a, s, r0, 16);
+    const KeyRange kr = key_range(a, s, r0, a.few);
     if (split >= splits_used(a.few, kr)) return;
     const int k_begin = kr.base + split * a.few.len, k_end = min(k_begin + a.few.len, kr.hi);
     const int blocks = max(0, (k_end - k_begin + kBK - 1) / kBK);
@@ -531,23 +533,23 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
 //   warps 0-3, 4-7   softmax of tile 0 / 1: a thread owns a row.  It reads its
 //                    scores from tensor memory, and writes its weights (16 bits)
 //                    back over them as the A operand of P.V.
-//   warps 8-11       producers: gather the tiles' rows from their pages with
-//                    16-byte cp.async (any page size and any strides; places
-//                    outside the range become zeros) into the 128-byte-swizzled
-//                    layout the products read; K and V take turns in a ring of
-//                    four stages.
-//   warp 12          one thread issues the products: for each key tile and row
+//   warp 8           one thread issues the products: for each key tile and row
 //                    tile P.V, then the next key tile's Q.K.  They run in order, so
 //                    a finished Q.K says that the P.V before it is finished too,
 //                    and a row's thread may rescale its sums then.
+//   warps 9-11       producers: the tiles' rows from their pages into the
+//                    128-byte-swizzled layout the products read, by TMA or
+//                    16-byte cp.async; K and V take turns in a ring of four stages.
 // The running maximum is raised, and the sums rescaled, only when a score
 // exceeds it by more than 2^8: weights stay below 256, which changes no
 // rounding (they are relative), and rescaling is rare.
 // Bound by the exponentials (16 a clock on an SM: 2048 clocks for the two tiles
 // of 128 x 128) as much as by the products (2048 clocks at D = 128).
-constexpr int kTcThreads = 512;
+constexpr int kTcThreads = 384;
+constexpr int kTcProducers = 96;
 constexpr int kTcRows = 256;
 constexpr int kTcStages = 4;
+constexpr bool kPoly = true;
 
 template <int D>
 struct TcCfg {
@@ -558,25 +560,84 @@ struct TcCfg {
     static constexpr int kO = 256;                      // tensor-memory columns: S0, S1, O0, O1
 };
 
-// Descriptor of an operand whose rows are the summed dimension (V: rows are keys, a row's
-// 64 elements lie along N): 8 rows x 128 bytes swizzled, 1024 bytes from 8 rows to the next
-// and 16 KB from 64 elements of N to the next.
-__device__ __forceinline__ uint64_t sw128_desc_mn(unsigned saddr) {
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((128 * 128) >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// Shared-memory descriptors, 128-byte swizzle, 1024 bytes from 8 rows to the next.  The
+// low word holds the address / 16 and, for V, the 16 KB from 64 elements of N to the next
+// (V's rows are keys, the summed dimension: its operand is N-major).
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+constexpr uint32_t kDescK = 1u << 16, kDescV = ((128u * 128u) >> 4) << 16;
+
+__device__ __forceinline__ unsigned elect_one() {
+    unsigned r;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(r));
+    return r;
+}
+// The lane with `leader` set issues; addr: a descriptor's address / 16.
+// D[tmem] (+)= A[smem] B[smem]
+__device__ __forceinline__ void mma_ss(unsigned leader, unsigned tmem, unsigned a, unsigned b, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{ .reg .pred p, q; .reg .b64 da, db; setp.ne.u32 p, %4, 0; setp.ne.u32 q, %5, 0;"
+        " mov.b64 da, {%1, %6}; mov.b64 db, {%2, %6};"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p; }" ::"r"(tmem),
+        "r"(a | kDescK), "r"(b | kDescK), "r"(idesc), "r"((unsigned)acc), "r"(leader), "r"(kDescHi)
+        : "memory");
+}
+// D[tmem] (+)= A[tmem] B[smem], B N-major
+__device__ __forceinline__ void mma_ts(unsigned leader, unsigned tmem, unsigned a, unsigned b, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{ .reg .pred p, q; .reg .b64 db; setp.ne.u32 p, %4, 0; setp.ne.u32 q, %5, 0; mov.b64 db, {%2, %6};"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p; }" ::"r"(tmem),
+        "r"(a), "r"(b | kDescV), "r"(idesc), "r"((unsigned)acc), "r"(leader), "r"(kDescHi)
+        : "memory");
+}
+__device__ __forceinline__ void commit_one(unsigned leader, unsigned mbar) {
+    asm volatile(
+        "{ .reg .pred q; setp.ne.u32 q, %1, 0;"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0]; }" ::"r"(mbar),
+        "r"(leader)
+        : "memory");
+}
+// 128 columns of this warp's 32 lanes
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ f2 f2add(f2 a, f2 b) {
+    f2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// 2^y of a pair on the FMA pipe, for y <= 8: y = n + f with n whole and |f| <= 1/2 (n
+// falls out of the mantissa of 1.5 * 2^23 + y), 2^f by a polynomial of degree 4 fitted to
+// the least relative error on [-1/2, 1/2] (2.6e-6, of both signs: the weights' sum, which
+// lse shows, stays good to f32's last bits), n added to the exponent.
+__device__ __forceinline__ void exp2_poly(f2 y, float& p0, float& p1) {
+    float y0, y1;
+    f2unpack(y, y0, y1);
+    y = f2pack(fmaxf(y0, -126.f), fmaxf(y1, -126.f));  // the exponent stays a number's
+    const f2 magic = f2pack(12582912.f, 12582912.f);
+    const f2 n = f2add(y, magic), f = f2sub(y, f2sub(n, magic));
+    f2 p = f2fma(f, f2pack(0.0095701f, 0.0095701f), f2pack(0.05591786f, 0.05591786f));
+    p = f2fma(f, p, f2pack(0.24024745f, 0.24024745f));
+    p = f2fma(f, p, f2pack(0.69312181f, 0.69312181f));
+    p = f2fma(f, p, f2pack(0.99999926f, 0.99999926f));
+    float n0, n1;
+    f2unpack(p, p0, p1);
+    f2unpack(n, n0, n1);
+    p0 = __int_as_float(__float_as_int(p0) + (__float_as_int(n0) << 23));
+    p1 = __int_as_float(__float_as_int(p1) + (__float_as_int(n1) << 23));
+}
+__device__ __forceinline__ void tma_load_4d(unsigned dst, const CUtensorMap* map, int x, int y, int z, int w, unsigned mbar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(mbar)
+        : "memory");
 }
 // Arrives at an mbarrier once this thread's cp.asyncs so far have landed.  The
 // thread that waits for it puts the proxy fence between them and its products.
 __device__ __forceinline__ void cp_async_arrive(unsigned bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
-// D[tmem] (+)= A[tmem] B[smem]
-__device__ __forceinline__ void mma_f16_ta(unsigned tmem, unsigned atmem, uint64_t bdesc, uint32_t idesc, bool acc) {
-    asm volatile(
-        "{ .reg .pred p; setp.ne.u32 p, %4, 0; "
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(tmem),
-        "r"(atmem), "l"(bdesc), "r"(idesc), "r"((unsigned)acc)
-        : "memory");
 }
 // 128 columns of this warp's 32 lanes
 __device__ __forceinline__ void tmem_ld128(unsigned taddr, float* v) {
@@ -670,7 +731,9 @@ __device__ __forceinline__ void find_tile(const AttnView& a, int64_t idx, int ro
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __grid_constant__ AttnView a) {
+__global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __grid_constant__ AttnView a,
+                                                                      const __grid_constant__ CUtensorMap mk,
+                                                                      const __grid_constant__ CUtensorMap mv) {
     using C = TcCfg<D>;
     constexpr int NH = D / 64;
     constexpr uint32_t kFmt = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0u : 1u;
@@ -679,11 +742,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     constexpr uint32_t kIdPV =
         (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
     extern __shared__ char smem_raw[];
-    __shared__ __align__(8) unsigned long long q_full, kv_full[kTcStages], kv_empty[kTcStages], s_full[2], p_full[2],
-        o_full[2];
+    __shared__ __align__(8) unsigned long long q_full, kv_full[kTcStages], kv_empty[kTcStages], s_full[2],
+        p_full[2][2], o_full[2], turn[2];
     __shared__ unsigned tmem_slot;
     __shared__ int failed;
-    __shared__ int64_t place[2][128];
+    __shared__ int64_t place[128];
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31, wg = t >> 7;
     pdl_wait();
     pdl_trigger();
@@ -698,7 +761,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     const PagedSeq s = paged_seq(a.p, b);
     const int rows = s.n * a.group, r0 = tile * kTcRows;
     if (r0 >= rows) return;
-    const KeyRange kr = key_range(a, s, r0, kTcRows);
+    const KeyRange kr = key_range(a, s, r0, a.many);
     if (split >= splits_used(a.many, kr)) return;
     const int k_begin = kr.base + split * a.many.len, k_end = min(k_begin + a.many.len, kr.hi);
     // key tiles of each row tile
@@ -713,20 +776,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
 
     const unsigned sb = (smem_addr(smem_raw) + 1023u) & ~1023u;
     if (t == 0) {
-        mbar_init(smem_addr(&q_full), 128);
+        mbar_init(smem_addr(&q_full), kTcProducers);
         for (int i = 0; i < kTcStages; i++) {
-            mbar_init(smem_addr(&kv_full[i]), 128);
+            mbar_init(smem_addr(&kv_full[i]), kTcProducers);
             mbar_init(smem_addr(&kv_empty[i]), 1);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(smem_addr(&s_full[i]), 1);
-            mbar_init(smem_addr(&p_full[i]), 128);
+            mbar_init(smem_addr(&p_full[i][0]), 4);
+            mbar_init(smem_addr(&p_full[i][1]), 4);
+            mbar_init(smem_addr(&turn[i]), 4);
             mbar_init(smem_addr(&o_full[i]), 1);
         }
         failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 12) {
+    if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)),
                      "r"(512)
                      : "memory");
@@ -739,7 +804,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
 
     if (wg < 2) {
         // ------------------------------------------------------ softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int r = r0 + t;  // tile wg's row t % 128
         const bool live = r < rows;
         const int pos = live ? s.len - s.n + r / a.group : -1;
@@ -748,7 +813,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         const float sc = fabsf(a.scale_log2);
         const bool flip = a.scale_log2 < 0.f;
         float m = -INFINITY, l = 0.f;  // m: the maximum the sums are relative to
-        const int n = nt[wg];
+        const int n = nt[wg], both = min(nt[0], nt[1]);
         bool ok = true;
         for (int j = 0; j < n && ok; j++) {
             ok = tc_wait(smem_addr(&s_full[wg]), (unsigned)j & 1u, &failed);
@@ -763,15 +828,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             // columns this row sees: lo .. hi
             const int k0 = k_begin + j * 128;
             const int hi = min(pos, k_end - 1) - k0, lo = a.window > 0 ? pos - a.window + 1 - k0 : 0;
-            if (__any_sync(0xffffffffu, hi < 127 || lo > 0)) {
+            const bool edge = __any_sync(0xffffffffu, hi < 127 || lo > 0);
+            if (edge) {
 #pragma unroll
                 for (int c = 0; c < 128; c++) x[c] = c <= hi && c >= lo ? x[c] : -INFINITY;
             }
-            float mx[4] = {x[0], x[1], x[2], x[3]};
+            float mx[4] = {fmaxf(x[0], x[1]), fmaxf(x[2], x[3]), fmaxf(x[4], x[5]), fmaxf(x[6], x[7])};
 #pragma unroll
-            for (int c = 4; c < 128; c += 4)
+            for (int c = 8; c < 128; c += 8)
 #pragma unroll
-                for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], x[c + e]);
+                for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], x[c + 2 * e], x[c + 2 * e + 1]);
             const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
             const bool raise = mt > m + 8.f || (m == -INFINITY && mt > m);
             if (__any_sync(0xffffffffu, raise)) {
@@ -791,25 +857,47 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
                 }
             }
             const float mb = m == -INFINITY ? 0.f : m;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                uint32_t w[32];
-#pragma unroll
-                for (int c = 0; c < 64; c += 2) {
-                    const int i = 64 * h + c;
-                    const float p0 = ex2_approx(fmaf(x[i], sc, -mb));
-                    const float p1 = ex2_approx(fmaf(x[i + 1], sc, -mb));
-                    sum[c & 2] += p0;
-                    sum[(c & 2) + 1] += p1;
-                    w[c / 2] = pack2<T>(p0, p1);
-                }
-                tmem_st32(tS + 32 * h, w);
+            // The tiles take turns at the exponentials: side by side both would be slow, and
+            // then both wait for the products.  0, 1, 0, 1, ... while both have key tiles.
+            if (wg == 0 ? j > 0 && j < both : j < both) {
+                ok = tc_wait(smem_addr(&turn[wg]), (unsigned)(wg == 0 ? j - 1 : j) & 1u, &failed);
+                if (!__all_sync(0xffffffffu, ok)) break;
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            mbar_arrive(smem_addr(&p_full[wg]), 1);
+            f2 sum[2] = {0ull, 0ull};
+            const f2 sc2 = f2pack(sc, sc), mb2 = f2pack(-mb, -mb);
+            auto weights = [&](auto inner) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int c = 0; c < 64; c += 2) {
+                        const f2 y = f2fma(f2pack(x[64 * h + c], x[64 * h + c + 1]), sc2, mb2);
+                        float p0, p1;
+                        // one pair in four on the FMA pipe, where no score is masked
+                        if (decltype(inner)::value && (c & 6) == 6) {
+                            exp2_poly(y, p0, p1);
+                        } else {
+                            f2unpack(y, p0, p1);
+                            p0 = ex2_approx(p0);
+                            p1 = ex2_approx(p1);
+                        }
+                        sum[(c >> 1) & 1] = f2add(sum[(c >> 1) & 1], f2pack(p0, p1));
+                        w[c / 2] = pack2<T>(p0, p1);
+                    }
+                    tmem_st32(tS + 32 * h, w);
+                    // this half's products may start while the other's weights are made
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_addr(&p_full[wg][h]), 1);
+                }
+            };
+            if (edge)
+                weights(std::false_type{});
+            else
+                weights(std::integral_constant<bool, kPoly>{});
+            if (lane == 0 && j + wg < both) mbar_arrive(smem_addr(&turn[1 - wg]), 1);
+            l += f2sum(sum[0]) + f2sum(sum[1]);
         }
         if (n > 0) ok = tc_wait(smem_addr(&o_full[wg]), 0u, &failed) && ok;
         ok = __all_sync(0xffffffffu, ok);
@@ -847,116 +935,176 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             else if (a.lse)
                 a.lse[th] = l > 0.f ? (m + log2f(l)) * 0.693147180559945309f : -INFINITY;
         }
-    } else if (wg == 2) {
-        // ----------------------------------------------------- producers
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-        const int pt = t & 127;
-        constexpr int RC = D / 8, RPP = 128 / RC;  // 16-byte chunks of a row, rows a pass of the 128 threads takes
-        const int pr = pt / RC, pc = pt % RC;
-        // chunk c of row r in a tile: half c / 8, swizzled inside its 128 bytes
-        const unsigned col = (unsigned)(pc >> 3) * C::kHalf;
-        auto at = [&](int r) { return (unsigned)(r * 128 + (((pc & 7) ^ (r & 7)) << 4)) + col; };
-        for (int i = 0; i < 2; i++) {
-            if (nt[i] == 0) continue;
-            for (int r = pr; r < 128; r += RPP) {
-                const int row = r0 + 128 * i + r;
-                const bool real = row < rows;
-                const int x = real ? row : 0;
-                cp_async16(sb + i * C::kTile + at(r),
-                           a.q + (int64_t)(s.start + x / a.group) * a.q_row +
-                               (int64_t)(kvh * a.group + x % a.group) * a.q_head + pc * 16,
-                           real);
-            }
-        }
-        cp_async_arrive(smem_addr(&q_full));
-        auto look_up = [&](int j) -> int64_t {
-            const int key = k_begin + j * 128 + pt;
-            return j < nmax && key >= kr.lo && key < k_end ? paged_offset(a.p, b, key) : -1;
-        };
-        const int64_t head_off = (int64_t)kvh * a.p.stride_head + pc * 16;
-        int64_t next = look_up(0);
-        bool ok = true;
-        int push = 0;
-        for (int j = 0; j < nmax; j++) {
-            place[j & 1][pt] = next;
-            next = look_up(j + 1);
-            // (the other buffer's last readers passed this barrier's previous use)
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-#pragma unroll 1
-            for (int kv = 0; kv < 2; kv++, push++) {
-                const int st = push % kTcStages;
-                if (push >= kTcStages)
-                    ok = tc_wait(smem_addr(&kv_empty[st]), (unsigned)(push / kTcStages - 1) & 1u, &failed) && ok;
-                const char* src = kv ? a.p.v : a.p.k;
-                const unsigned dst = sb + C::kOffKV + st * C::kTile;
-                if (ok) {
-#pragma unroll 4
-                    for (int r = pr; r < 128; r += RPP) {
-                        const int64_t o = place[j & 1][r];
-                        cp_async16(dst + at(r), src + (o < 0 ? 0 : o + head_off), o >= 0);
-                    }
-                }
-                cp_async_arrive(smem_addr(&kv_full[st]));
-            }
-        }
-        cp_async_commit();
-        cp_async_wait<0>();  // nothing in flight when the block ends
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-        if (t == 384 && nmax > 0) {
-            // ---------------------------------------------------- products
-            bool ok = tc_wait(smem_addr(&q_full), 0u, &failed);
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 8) {
+            // ------------------------------------------------- products
+            // The whole warp runs this, one lane's instructions count: what the products take
+            // (descriptors, addresses) then stays in uniform registers.  A single lane's branch
+            // moved every operand there first and issued at half the tensor cores' pace.
+            const unsigned leader = elect_one();
+            const unsigned utm = __shfl_sync(0xffffffffu, tm, 0);
+            const int n0 = __shfl_sync(0xffffffffu, nt[0], 0), n1 = __shfl_sync(0xffffffffu, nt[1], 0);
+            const int nm = max(n0, n1);
+            const int k_lo = __shfl_sync(0xffffffffu, kr.lo - k_begin, 0), k_hi = __shfl_sync(0xffffffffu, k_end - k_begin, 0);
+            const unsigned q_d = (sb & 0x3FFFFu) >> 4, kv_d = q_d + (C::kOffKV >> 4);
+            bool ok = nm > 0 && tc_wait(smem_addr(&q_full), 0u, &failed);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             auto wait_kv = [&](int push) {
                 ok = ok && tc_wait(smem_addr(&kv_full[push % kTcStages]), (unsigned)(push / kTcStages) & 1u, &failed);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                // rows that came by cp.async, not TMA
+                const int k0 = (push >> 1) * 128;
+                if (!a.box || k0 < k_lo || k0 + 128 > k_hi) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                ok = __all_sync(0xffffffffu, ok);
             };
             auto qk = [&](int i, int j) {
                 if (ok) {
-                    const unsigned kb = sb + C::kOffKV + (2 * j % kTcStages) * C::kTile;
+                    const unsigned qd = q_d + i * (C::kTile >> 4), kd = kv_d + (2 * j % kTcStages) * (C::kTile >> 4);
 #pragma unroll
                     for (int h = 0; h < NH; h++)
 #pragma unroll
                         for (int k = 0; k < 4; k++)
-                            mma_f16(tm + 128u * i, sw128_desc(sb + i * C::kTile + h * C::kHalf + 32u * k),
-                                    sw128_desc(kb + h * C::kHalf + 32u * k), kIdS, h > 0 || k > 0);
+                            mma_ss(leader, utm + 128u * i, qd + h * (C::kHalf >> 4) + 2 * k, kd + h * (C::kHalf >> 4) + 2 * k,
+                                   kIdS, h > 0 || k > 0);
                 }
-                mma_commit(smem_addr(&s_full[i]));
+                commit_one(leader, smem_addr(&s_full[i]));
             };
-            wait_kv(0);
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            for (int i = 0; i < 2; i++)
-                if (nt[i] > 0) qk(i, 0);
-            mma_commit(smem_addr(&kv_empty[0]));
-            for (int j = 0; j < nmax; j++) {
+            if (nm > 0) {
+                wait_kv(0);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (n0 > 0) qk(0, 0);
+                if (n1 > 0) qk(1, 0);
+                commit_one(leader, smem_addr(&kv_empty[0]));
+            }
+            for (int j = 0; j < nm; j++) {
                 wait_kv(2 * j + 1);
-                const unsigned vb = sb + C::kOffKV + ((2 * j + 1) % kTcStages) * C::kTile;
-                if (j + 1 < nmax) wait_kv(2 * j + 2);
-                for (int i = 0; i < 2; i++) {
-                    if (j >= nt[i]) continue;
-                    ok = ok && tc_wait(smem_addr(&p_full[i]), (unsigned)j & 1u, &failed);
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (ok) {
+                const unsigned vd = kv_d + ((2 * j + 1) % kTcStages) * (C::kTile >> 4);
+                if (j + 1 < nm) wait_kv(2 * j + 2);
 #pragma unroll
-                        for (int k = 0; k < 8; k++)
-                            mma_f16_ta(tm + C::kO + 128u * i, tm + 128u * i + 8u * k, sw128_desc_mn(vb + 2048u * k), kIdPV,
-                                       j > 0 || k > 0);
+                for (int i = 0; i < 2; i++) {
+                    const int ni = i ? n1 : n0;
+                    if (j >= ni) continue;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        ok = ok && tc_wait(smem_addr(&p_full[i][h]), (unsigned)j & 1u, &failed);
+                        ok = __all_sync(0xffffffffu, ok);
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        if (!ok) continue;
+#pragma unroll
+                        for (int k = 4 * h; k < 4 * h + 4; k++)
+                            mma_ts(leader, utm + C::kO + 128u * i, utm + 128u * i + 8u * k, vd + 128 * k, kIdPV, j > 0 || k > 0);
                     }
-                    if (j + 1 < nt[i])
+                    if (j + 1 < ni)
                         qk(i, j + 1);
                     else
-                        mma_commit(smem_addr(&o_full[i]));
+                        commit_one(leader, smem_addr(&o_full[i]));
                 }
-                mma_commit(smem_addr(&kv_empty[(2 * j + 1) % kTcStages]));
-                if (j + 1 < nmax) mma_commit(smem_addr(&kv_empty[(2 * j + 2) % kTcStages]));
+                commit_one(leader, smem_addr(&kv_empty[(2 * j + 1) % kTcStages]));
+                if (j + 1 < nm) commit_one(leader, smem_addr(&kv_empty[(2 * j + 2) % kTcStages]));
             }
             // every product has landed before the tensor memory goes
-            for (int i = 0; i < 2; i++)
-                if (nt[i] > 0) tc_wait(smem_addr(&o_full[i]), 0u, nullptr);
+            if (n0 > 0) tc_wait(smem_addr(&o_full[0]), 0u, nullptr);
+            if (n1 > 0) tc_wait(smem_addr(&o_full[1]), 0u, nullptr);
+        } else {
+            // ------------------------------------------------- producers
+            const int pt = t - (kTcThreads - kTcProducers);
+            constexpr int RC = D / 8, RPP = kTcProducers / RC;  // 16-byte chunks of a row, rows a pass takes
+            const int pr = pt / RC, pc = pt % RC;
+            // chunk c of row r in a tile: half c / 8, swizzled inside its 128 bytes
+            const unsigned col = (unsigned)(pc >> 3) * C::kHalf;
+            auto at = [&](int r) { return (unsigned)(r * 128 + (((pc & 7) ^ (r & 7)) << 4)) + col; };
+            for (int i = 0; i < 2; i++) {
+                if (nt[i] == 0) continue;
+                for (int r = pr; r < 128; r += RPP) {
+                    const int row = r0 + 128 * i + r;
+                    const bool real = row < rows;
+                    const int x = real ? row : 0;
+                    cp_async16(sb + i * C::kTile + at(r),
+                               a.q + (int64_t)(s.start + x / a.group) * a.q_row +
+                                   (int64_t)(kvh * a.group + x % a.group) * a.q_head + pc * 16,
+                               real);
+                }
+            }
+            cp_async_arrive(smem_addr(&q_full));
+            // Key tiles that lie wholly inside the range come by TMA, a box of rows of one page
+            // by one thread; at its edges, where places outside must read as zeros (weights of
+            // 0 do not silence a NaN), and where pages do not tile 128 keys, by cp.async.
+            const int boxes = a.box ? 128 / a.box : 0;
+            auto by_tma = [&](int j) {
+                const int k0 = k_begin + j * 128;
+                return boxes > 0 && k0 >= kr.lo && k0 + 128 <= k_end;
+            };
+            // page and position of box pt of a tile that comes by TMA
+            int page = 0, row = 0;
+            auto look_up = [&](int j) {
+                if (j >= nmax || pt >= boxes || !by_tma(j)) return;
+                const int key = k_begin + j * 128 + pt * a.box, pg = key >> a.p.page_shift;
+                page = a.p.table[(size_t)b * a.p.table_stride + pg];
+                row = key - (pg << a.p.page_shift);
+                if ((unsigned)page >= (unsigned)a.p.num_pages) {
+                    paged_report(a.p, VB_PAGED_BAD_PAGE);
+                    page = a.p.num_pages;  // beyond the map: zeros
+                }
+            };
+            const int64_t head_off = (int64_t)kvh * a.p.stride_head + pc * 16;
+            look_up(0);
+            bool ok = true;
+            int push = 0;
+            for (int j = 0; j < nmax; j++) {
+                const int pg = page, py = row;
+                const bool tma = by_tma(j);
+                look_up(j + 1);
+                if (!tma) {
+                    // byte offset of every key's row, -1: zeros
+                    asm volatile("bar.sync 1, %0;" ::"n"(kTcProducers) : "memory");  // the last such tile's readers are done
+                    for (int r = pt; r < 128; r += kTcProducers) {
+                        const int key = k_begin + j * 128 + r;
+                        place[r] = key >= kr.lo && key < k_end ? paged_offset(a.p, b, key) : -1;
+                    }
+                    asm volatile("bar.sync 1, %0;" ::"n"(kTcProducers) : "memory");
+                }
+#pragma unroll 1
+                for (int kv = 0; kv < 2; kv++, push++) {
+                    const int st = push % kTcStages;
+                    const unsigned full = smem_addr(&kv_full[st]);
+                    if (push >= kTcStages)
+                        ok = tc_wait(smem_addr(&kv_empty[st]), (unsigned)(push / kTcStages - 1) & 1u, &failed) && ok;
+                    const unsigned dst = sb + C::kOffKV + st * C::kTile;
+                    if (tma) {
+                        // all arrivals by one thread, with the bytes that are on their way
+                        if (pt == 0) {
+                            if (ok) mbar_expect_tx(full, C::kTile);
+                            mbar_arrive(full, ok ? kTcProducers - 1 : kTcProducers);
+                        }
+                        if (pt < boxes && ok) {
+#pragma unroll
+                            for (int h = 0; h < NH; h++)
+                                tma_load_4d(dst + h * C::kHalf + pt * a.box * 128, kv ? &mv : &mk, 64 * h, py, kvh, pg, full);
+                        }
+                    } else {
+                        const char* src = kv ? a.p.v : a.p.k;
+                        if (ok) {
+#pragma unroll 4
+                            for (int r = pr; r < 128; r += RPP) {
+                                const int64_t o = place[r];
+                                cp_async16(dst + at(r), src + (o < 0 ? 0 : o + head_off), o >= 0);
+                            }
+                        }
+                        cp_async_arrive(full);
+                    }
+                }
+            }
+            // nothing in flight when the block ends: the products waited for every TMA copy, unless a wait gave up
+            if (*(volatile int*)&failed)
+                for (int i = max(0, push - kTcStages); i < push; i++)
+                    tc_wait(smem_addr(&kv_full[i % kTcStages]), (unsigned)(i / kTcStages) & 1u, nullptr);
+            cp_async_commit();
+            cp_async_wait<0>();
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 12)
+    if (warp == 8)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512) : "memory");
     if (t == 0 && failed) paged_report(a.p, VB_PAGED_TIMEOUT);
 }
@@ -976,7 +1124,7 @@ __global__ void __launch_bounds__(128) paged_attn_merge_kernel(const __grid_cons
     const int r = (token - s.start) * a.group + head % a.group;
     const Cut& cut = s.n * a.group > a.few_rows ? a.many : a.few;
     if (cut.splits == 1) return;  // written by the kernel itself
-    const int used = splits_used(cut, key_range(a, s, r / cut.rows * cut.rows, cut.rows));
+    const int used = splits_used(cut, key_range(a, s, r / cut.rows * cut.rows, cut));
     constexpr int E = D / 32;
     float y[E] = {}, M = -INFINITY, L = 0.f;
     const int64_t step = (int64_t)a.p.tokens * a.heads;
@@ -1008,9 +1156,10 @@ struct Plan {
 };
 constexpr int kFewRows = 32;
 
-Cut make_cut(int rows, int64_t keys, int64_t want, int step, int least) {
+Cut make_cut(int rows, int align, int64_t keys, int64_t want, int step, int least) {
     Cut c;
     c.rows = rows;
+    c.align = align;
     const int64_t n = std::max<int64_t>(1, std::min<int64_t>(want, (keys + least - 1) / least));
     c.len = (int)(((keys + n - 1) / n + step - 1) / step * step);
     c.splits = (int)((keys + c.len - 1) / c.len);
@@ -1028,18 +1177,18 @@ Plan make_plan(const PagedView& p, int io, int cache, int heads, int window) {
     const int64_t few_most = std::min<int64_t>(most, pl.few_rows);
     pl.row_tiles = (int)((few_most + 15) / 16);
     const int64_t all = std::max(p.max_len, 1);
-    // keys from a tile's base (its first row's lowest, rounded down to 16) to its last row's
-    auto span = [&](int rows) {
-        return window > 0 ? std::min<int64_t>(all, (int64_t)window + (rows + G - 1) / G + 15) : all;
+    // keys from a tile's base (its first row's lowest, rounded down) to its last row's
+    auto span = [&](int rows, int align) {
+        return window > 0 ? std::min<int64_t>(all, (int64_t)window + (rows + G - 1) / G + align - 1) : all;
     };
     // few rows: about four CTAs for each SM (two run at a time) of at least 64 keys, one block of
     // 16 a warp; many: one CTA for each SM of at least 512 keys
     const int64_t tiles = std::max<int64_t>(1, std::min<int64_t>((int64_t)p.batch * pl.row_tiles, total / 16 + p.batch));
     const int64_t want = std::max<int64_t>(1, 148 * 4 / (tiles * p.kv_heads));
-    pl.few = make_cut(16, span(16), want, 64, 64);
+    pl.few = make_cut(16, 16, span(16, 16), want, 64, 64);
     const int64_t tiles2 = std::max<int64_t>(1, (total + kTcRows - 1) / kTcRows);
     const int64_t want2 = std::max<int64_t>(1, 148 / (tiles2 * p.kv_heads));
-    pl.many = make_cut(kTcRows, span(kTcRows), want2, 128, 512);
+    pl.many = make_cut(kTcRows, 128, span(kTcRows, 128), want2, 128, 512);
     pl.max_splits = (int)std::max<int64_t>(pl.few_rows ? std::min<int64_t>(want, (all + 63) / 64) : 1,
                                            tc ? std::min<int64_t>(want2, (all + 511) / 512) : 1);
     if (!tc) pl.many.splits = 1;
@@ -1048,6 +1197,25 @@ Plan make_plan(const PagedView& p, int io, int cache, int heads, int window) {
 }
 size_t plan_bytes(const Plan& pl, const PagedView& p, int heads, int D) {
     return pl.max_splits > 1 ? (size_t)pl.max_splits * p.tokens * heads * (D + 2) * 4 : 0;
+}
+
+// Tensor map of a pool as [page][kv head][position][dim], boxes of one page's rows (128 at
+// most) x 64 dims, 128-byte swizzle.  Returns the rows of a box; 0 where pages are not
+// whole groups of 8 rows that tile 128, or the map is refused: the rows are then gathered
+// by cp.async.
+int page_map(const PagedView& p, const char* base, int D, bool half, CUtensorMap* map) {
+    if (p.page_shift < 3) return 0;
+    auto fn = tc_encode_fn();
+    if (!fn) return 0;
+    const int box = std::min(p.page_size, 128);
+    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)p.page_size, (cuuint64_t)p.kv_heads, (cuuint64_t)p.num_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)p.stride_pos, (cuuint64_t)p.stride_head, (cuuint64_t)p.stride_page};
+    const cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1}, es[4] = {1, 1, 1, 1};
+    const CUresult r =
+        fn(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<char*>(base),
+           dims, strides, boxes, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? box : 0;
 }
 
 template <typename IO, typename KV, int D>
@@ -1063,7 +1231,12 @@ vb_status launch_attn(const AttnView& a, cudaStream_t s) {
                 (int64_t)a.p.tokens * a.group / kTcRows + a.p.batch);
             const int64_t grid = tiles * a.many.splits * a.p.kv_heads;
             if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
-            e = launch_pdl(paged_attn_tc_kernel<IO, D>, dim3((unsigned)grid), dim3(kTcThreads), TcCfg<D>::kSmem, s, a);
+            AttnView b = a;
+            CUtensorMap mk{}, mv{};
+            b.box = page_map(a.p, a.p.k, D, std::is_same<IO, __half>::value, &mk);
+            if (b.box && !page_map(a.p, a.p.v, D, std::is_same<IO, __half>::value, &mv)) b.box = 0;
+            e = launch_pdl(paged_attn_tc_kernel<IO, D>, dim3((unsigned)grid), dim3(kTcThreads), TcCfg<D>::kSmem, s, b, mk,
+                           mv);
             if (e != cudaSuccess) return cuda_fail(e, "paged_attn_tc_kernel");
         }
     }

@@ -89,6 +89,9 @@ __device__ __forceinline__ void tmem_ld32(unsigned taddr, float* v) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// The driver's cuTensorMapEncodeTiled; null if it has none (vb_tcgemm.cu).
+PFN_cuTensorMapEncodeTiled_v12000 tc_encode_fn();
+
 // 2-D bf16 tensor map over [rows][cols], boxes of 64 columns x box_rows rows,
 // 128-byte swizzle (vb_tcgemm.cu).
 vb_status tc_make_map(CUtensorMap* map, const void* base, int rows, int cols, int box_rows);

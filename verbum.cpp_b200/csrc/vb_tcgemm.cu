@@ -820,7 +820,9 @@ __global__ void weights_bf16_kernel(const void* W, bool q8, size_t total, __nv_b
     }
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+}  // namespace
+
+PFN_cuTensorMapEncodeTiled_v12000 tc_encode_fn() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
     static std::once_flag once;
     std::call_once(once, [] {
@@ -834,6 +836,8 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
+namespace {
+
 vb_status make_map(CUtensorMap* map, const void* base, int rows, int K, int box_rows) {
     return tc_make_map(map, base, rows, K, box_rows);
 }
@@ -842,7 +846,7 @@ vb_status make_map(CUtensorMap* map, const void* base, int rows, int K, int box_
 
 // 2-D bf16 tensor map over [rows][K], boxes of 64 (K) x box_rows, 128-byte swizzle.
 vb_status tc_make_map(CUtensorMap* map, const void* base, int rows, int K, int box_rows) {
-    auto fn = encode_fn();
+    auto fn = tc_encode_fn();
     if (!fn) return fail(VB_ERR_UNSUPPORTED, "tensor-core gemm: cuTensorMapEncodeTiled unavailable");
     const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
     const cuuint64_t strides[1] = {(cuuint64_t)K * 2};
