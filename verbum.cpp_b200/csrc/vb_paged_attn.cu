@@ -530,14 +530,17 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
 // Attention of 256 rows of a KV head on the 5th-generation tensor cores: two
 // tiles of 128 rows, so that one tile's softmax runs while the other's products
 // do.  Keys come 128 at a time.
-//   warps 0-3, 4-7   softmax of tile 0 / 1: a thread owns a row.  It reads its
-//                    scores from tensor memory, and writes its weights (16 bits)
-//                    back over them as the A operand of P.V.
-//   warp 8           one thread issues the products: for each key tile and row
+//   warps 0-7, 8-15  softmax of tile 0 / 1: two threads share a row, 64 keys each.
+//                    They read their scores from tensor memory, agree on the
+//                    maximum through shared memory, and write their weights (16
+//                    bits) back over the scores as the A operand of P.V.  (With
+//                    one thread a row its chain of load, maximum, exponentials and
+//                    store was longer than the products of the other tile.)
+//   warp 16          one thread issues the products: for each key tile and row
 //                    tile P.V, then the next key tile's Q.K.  They run in order, so
 //                    a finished Q.K says that the P.V before it is finished too,
 //                    and a row's thread may rescale its sums then.
-//   warps 9-11       producers: the tiles' rows from their pages into the
+//   warps 17-19      producers: the tiles' rows from their pages into the
 //                    128-byte-swizzled layout the products read, by TMA or
 //                    16-byte cp.async; K and V take turns in a ring of four stages.
 // The running maximum is raised, and the sums rescaled, only when a score
@@ -545,11 +548,11 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
 // rounding (they are relative), and rescaling is rare.
 // Bound by the exponentials (16 a clock on an SM: 2048 clocks for the two tiles
 // of 128 x 128) as much as by the products (2048 clocks at D = 128).
-constexpr int kTcThreads = 384;
+constexpr int kTcThreads = 640;
 constexpr int kTcProducers = 96;
 constexpr int kTcRows = 256;
 constexpr int kTcStages = 4;
-constexpr bool kPoly = true;
+constexpr int kPoly = 4;  // one pair of exponentials in so many on the FMA pipe
 
 template <int D>
 struct TcCfg {
@@ -596,7 +599,6 @@ __device__ __forceinline__ void commit_one(unsigned leader, unsigned mbar) {
         "r"(leader)
         : "memory");
 }
-// 128 columns of this warp's 32 lanes
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -639,48 +641,24 @@ __device__ __forceinline__ void tma_load_4d(unsigned dst, const CUtensorMap* map
 __device__ __forceinline__ void cp_async_arrive(unsigned bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
-// 128 columns of this warp's 32 lanes
-__device__ __forceinline__ void tmem_ld128(unsigned taddr, float* v) {
+// 16 columns of this warp's 32 lanes
+__device__ __forceinline__ void tmem_ld16(unsigned taddr, float* v) {
     unsigned* r = reinterpret_cast<unsigned*>(v);
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,  "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31,  "
-        "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47,  "
-        "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%128]; "
-        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79,  "
-        "%80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95,  "
-        "%96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111,  "
-        "%112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127}, [%129]; "
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16]; "
         "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
-          "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
-          "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
-          "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
-          "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
-          "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
-          "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
-          "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
-          "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
-        : "r"(taddr), "r"(taddr + 64)
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
         : "memory");
 }
-// 32 columns of this warp's 32 lanes
-__device__ __forceinline__ void tmem_st32(unsigned taddr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_st16(unsigned taddr, const uint32_t* r) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
 
@@ -743,10 +721,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
     extern __shared__ char smem_raw[];
     __shared__ __align__(8) unsigned long long q_full, kv_full[kTcStages], kv_empty[kTcStages], s_full[2],
-        p_full[2][2], o_full[2], turn[2];
+        p_full[2], o_full[2];
     __shared__ unsigned tmem_slot;
     __shared__ int failed;
     __shared__ int64_t place[128];
+    __shared__ float xch[2][2][128];
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31, wg = t >> 7;
     pdl_wait();
     pdl_trigger();
@@ -783,15 +762,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(smem_addr(&s_full[i]), 1);
-            mbar_init(smem_addr(&p_full[i][0]), 4);
-            mbar_init(smem_addr(&p_full[i][1]), 4);
-            mbar_init(smem_addr(&turn[i]), 4);
+            mbar_init(smem_addr(&p_full[i]), 8);
             mbar_init(smem_addr(&o_full[i]), 1);
         }
         failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)),
                      "r"(512)
                      : "memory");
@@ -802,79 +779,82 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tm = tmem_slot;
 
-    if (wg < 2) {
+    if (wg < 4) {
         // ------------------------------------------------------ softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        const int r = r0 + t;  // tile wg's row t % 128
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        const int i = wg >> 1, hf = wg & 1;  // row tile; half of the keys (scores, weights) and of the dims (sums)
+        const int row = t & 127, r = r0 + 128 * i + row;
         const bool live = r < rows;
         const int pos = live ? s.len - s.n + r / a.group : -1;
         const unsigned lanes = (unsigned)(32 * (warp & 3)) << 16;
-        const unsigned tS = tm + 128u * wg + lanes, tO = tm + C::kO + 128u * wg + lanes;
+        const unsigned tS = tm + 128u * i + lanes, tO = tm + C::kO + 128u * i + (D / 2) * hf + lanes;
         const float sc = fabsf(a.scale_log2);
         const bool flip = a.scale_log2 < 0.f;
-        float m = -INFINITY, l = 0.f;  // m: the maximum the sums are relative to
-        const int n = nt[wg], both = min(nt[0], nt[1]);
+        float m = -INFINITY, l = 0.f;  // m: the maximum the sums are relative to; l: this half's sum
+        const int n = nt[i], pair = 2 + 4 * i + (warp & 3);
+        // what the row's other thread says of it (the two warps of 32 rows meet)
+        auto other = [&](float v) {
+            xch[i][hf][row] = v;
+            asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+            return xch[i][hf ^ 1][row];
+        };
         bool ok = true;
-        for (int j = 0; j < n && ok; j++) {
-            ok = tc_wait(smem_addr(&s_full[wg]), (unsigned)j & 1u, &failed);
-            if (!__all_sync(0xffffffffu, ok)) break;
+        // (no way out of the loop when a wait fails: the other warp of the pair counts on this one)
+        for (int j = 0; j < n; j++) {
+            ok = tc_wait(smem_addr(&s_full[i]), (unsigned)j & 1u, &failed) && ok;
+            __syncwarp();
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            float x[128];
-            tmem_ld128(tS, x);
+            float x[64];
+            tmem_ld64(tS + 64 * hf, x);
             if (flip) {
 #pragma unroll
-                for (int c = 0; c < 128; c++) x[c] = -x[c];
+                for (int c = 0; c < 64; c++) x[c] = -x[c];
             }
             // columns this row sees: lo .. hi
-            const int k0 = k_begin + j * 128;
+            const int k0 = k_begin + j * 128 + 64 * hf;
             const int hi = min(pos, k_end - 1) - k0, lo = a.window > 0 ? pos - a.window + 1 - k0 : 0;
-            const bool edge = __any_sync(0xffffffffu, hi < 127 || lo > 0);
+            const bool edge = __any_sync(0xffffffffu, hi < 63 || lo > 0);
             if (edge) {
 #pragma unroll
-                for (int c = 0; c < 128; c++) x[c] = c <= hi && c >= lo ? x[c] : -INFINITY;
+                for (int c = 0; c < 64; c++) x[c] = c <= hi && c >= lo ? x[c] : -INFINITY;
             }
             float mx[4] = {fmaxf(x[0], x[1]), fmaxf(x[2], x[3]), fmaxf(x[4], x[5]), fmaxf(x[6], x[7])};
 #pragma unroll
-            for (int c = 8; c < 128; c += 8)
+            for (int c = 8; c < 64; c += 8)
 #pragma unroll
                 for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], x[c + 2 * e], x[c + 2 * e + 1]);
-            const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
-            const bool raise = mt > m + 8.f || (m == -INFINITY && mt > m);
-            if (__any_sync(0xffffffffu, raise)) {
-                const float mn = raise ? mt : m;
+            float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+            top = fmaxf(top, other(top));
+            const bool raise = top > m + 8.f || (m == -INFINITY && top > m);
+            if (__any_sync(0xffffffffu, raise)) {  // in both warps of the pair alike
+                const float mn = raise ? top : m;
                 const float f = m == -INFINITY ? 0.f : ex2_approx(m - mn);
                 l *= f;
                 m = mn;
                 if (j > 0) {
 #pragma unroll
-                    for (int c = 0; c < D; c += 32) {
-                        float o[32];
-                        tmem_ld32(tO + c, o);
+                    for (int c = 0; c < D / 2; c += 16) {
+                        float o[16];
+                        tmem_ld16(tO + c, o);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] *= f;
-                        tmem_st32(tO + c, reinterpret_cast<const uint32_t*>(o));
+                        for (int e = 0; e < 16; e++) o[e] *= f;
+                        tmem_st16(tO + c, reinterpret_cast<const uint32_t*>(o));
                     }
                 }
             }
             const float mb = m == -INFINITY ? 0.f : m;
-            // The tiles take turns at the exponentials: side by side both would be slow, and
-            // then both wait for the products.  0, 1, 0, 1, ... while both have key tiles.
-            if (wg == 0 ? j > 0 && j < both : j < both) {
-                ok = tc_wait(smem_addr(&turn[wg]), (unsigned)(wg == 0 ? j - 1 : j) & 1u, &failed);
-                if (!__all_sync(0xffffffffu, ok)) break;
-            }
             f2 sum[2] = {0ull, 0ull};
             const f2 sc2 = f2pack(sc, sc), mb2 = f2pack(-mb, -mb);
             auto weights = [&](auto inner) {
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    uint32_t w[32];
+                    uint32_t w[16];
 #pragma unroll
-                    for (int c = 0; c < 64; c += 2) {
-                        const f2 y = f2fma(f2pack(x[64 * h + c], x[64 * h + c + 1]), sc2, mb2);
+                    for (int c = 0; c < 32; c += 2) {
+                        const f2 y = f2fma(f2pack(x[32 * h + c], x[32 * h + c + 1]), sc2, mb2);
                         float p0, p1;
-                        // one pair in four on the FMA pipe, where no score is masked
-                        if (decltype(inner)::value && (c & 6) == 6) {
+                        // some pairs on the FMA pipe, where no score is masked
+                        if (decltype(inner)::value && (c / 2) % kPoly == kPoly - 1) {
                             exp2_poly(y, p0, p1);
                         } else {
                             f2unpack(y, p0, p1);
@@ -884,24 +864,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
                         sum[(c >> 1) & 1] = f2add(sum[(c >> 1) & 1], f2pack(p0, p1));
                         w[c / 2] = pack2<T>(p0, p1);
                     }
-                    tmem_st32(tS + 32 * h, w);
-                    // this half's products may start while the other's weights are made
-                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_addr(&p_full[wg][h]), 1);
+                    tmem_st16(tS + 32 * hf + 16 * h, w);
                 }
             };
+            // the scores of both halves have been read (other() above): the weights may go over them
             if (edge)
                 weights(std::false_type{});
             else
-                weights(std::integral_constant<bool, kPoly>{});
-            if (lane == 0 && j + wg < both) mbar_arrive(smem_addr(&turn[1 - wg]), 1);
+                weights(std::true_type{});
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_addr(&p_full[i]), 1);
             l += f2sum(sum[0]) + f2sum(sum[1]);
         }
-        if (n > 0) ok = tc_wait(smem_addr(&o_full[wg]), 0u, &failed) && ok;
+        if (n > 0) ok = tc_wait(smem_addr(&o_full[i]), 0u, &failed) && ok;
         ok = __all_sync(0xffffffffu, ok);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");  // the last maximum has been read
+        l += other(l);
         const bool last = a.many.splits == 1;
         const float inv = last ? (l > 0.f ? 1.f / l : 0.f) : 1.f;
         const int rr = min(r, rows - 1);
@@ -909,7 +890,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         const int64_t th = (int64_t)token * a.heads + head;
         const int64_t pth = (int64_t)split * a.p.tokens * a.heads + th;
 #pragma unroll
-        for (int c = 0; c < D; c += 32) {
+        for (int c = 0; c < D / 2; c += 32) {
             float o[32];
             if (n > 0) {
                 tmem_ld32(tO + c, o);
@@ -918,26 +899,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
                 for (int e = 0; e < 32; e++) o[e] = 0.f;
             }
             if (live && ok) {
+                const int d = (D / 2) * hf + c;
 #pragma unroll
                 for (int e = 0; e < 32; e++) o[e] = l > 0.f ? o[e] * inv : 0.f;
 #pragma unroll
                 for (int e = 0; e < 32; e += 8) {
                     if (last)
-                        Eight<T>::store(a.out + token * a.o_row + head * a.o_head + (c + e) * sizeof(T), o + e);
+                        Eight<T>::store(a.out + token * a.o_row + head * a.o_head + (d + e) * sizeof(T), o + e);
                     else
-                        Eight<float>::store(a.part + pth * D + c + e, o + e);
+                        Eight<float>::store(a.part + pth * D + d + e, o + e);
                 }
             }
         }
-        if (live && ok) {
+        if (live && ok && hf == 0) {
             if (!last)
                 a.part_ml[pth] = make_float2(l > 0.f ? m : -INFINITY, l);
             else if (a.lse)
                 a.lse[th] = l > 0.f ? (m + log2f(l)) * 0.693147180559945309f : -INFINITY;
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (warp == 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == 16) {
             // ------------------------------------------------- products
             // The whole warp runs this, one lane's instructions count: what the products take
             // (descriptors, addresses) then stays in uniform registers.  A single lane's branch
@@ -976,22 +958,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
                 if (n1 > 0) qk(1, 0);
                 commit_one(leader, smem_addr(&kv_empty[0]));
             }
+            if (nm > 0) wait_kv(1);
+            if (nm > 1) wait_kv(2);
             for (int j = 0; j < nm; j++) {
-                wait_kv(2 * j + 1);
                 const unsigned vd = kv_d + ((2 * j + 1) % kTcStages) * (C::kTile >> 4);
-                if (j + 1 < nm) wait_kv(2 * j + 2);
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     const int ni = i ? n1 : n0;
                     if (j >= ni) continue;
+                    ok = ok && tc_wait(smem_addr(&p_full[i]), (unsigned)j & 1u, &failed);
+                    ok = __all_sync(0xffffffffu, ok);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (ok) {
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        ok = ok && tc_wait(smem_addr(&p_full[i][h]), (unsigned)j & 1u, &failed);
-                        ok = __all_sync(0xffffffffu, ok);
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        if (!ok) continue;
-#pragma unroll
-                        for (int k = 4 * h; k < 4 * h + 4; k++)
+                        for (int k = 0; k < 8; k++)
                             mma_ts(leader, utm + C::kO + 128u * i, utm + 128u * i + 8u * k, vd + 128 * k, kIdPV, j > 0 || k > 0);
                     }
                     if (j + 1 < ni)
@@ -1000,7 +980,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
                         commit_one(leader, smem_addr(&o_full[i]));
                 }
                 commit_one(leader, smem_addr(&kv_empty[(2 * j + 1) % kTcStages]));
-                if (j + 1 < nm) commit_one(leader, smem_addr(&kv_empty[(2 * j + 2) % kTcStages]));
+                if (j + 1 < nm) {
+                    commit_one(leader, smem_addr(&kv_empty[(2 * j + 2) % kTcStages]));
+                    // the next round's V and K, asked after while this round's products run
+                    wait_kv(2 * j + 3);
+                    if (j + 2 < nm) wait_kv(2 * j + 4);
+                }
             }
             // every product has landed before the tensor memory goes
             if (n0 > 0) tc_wait(smem_addr(&o_full[0]), 0u, nullptr);
@@ -1104,7 +1089,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 8)
+    if (warp == 16)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512) : "memory");
     if (t == 0 && failed) paged_report(a.p, VB_PAGED_TIMEOUT);
 }
