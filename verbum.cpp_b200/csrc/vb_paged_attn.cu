@@ -193,40 +193,54 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
     lo = __float_as_uint(x - __uint_as_float(hi));
 }
 
+// The transpose of a matrix of 8 x 8 16-bit values spread over the warp
+__device__ __forceinline__ uint32_t mat_t(uint32_t a) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+
+// ------------------------------------------------------------- few rows
 constexpr int kFewWarps = 4;
 constexpr int kBK = 16;  // keys a warp takes at a time
 
-template <typename KV, int D>
+template <typename KV, int D, int NR>
 struct FewCfg {
+    static constexpr int kRows = 8 * NR;
     static constexpr int kRowBytes = D * (int)sizeof(KV);
     static constexpr int kBlockBytes = kBK * kRowBytes;  // K or V of a block
-    // three stages of 8 KB (D = 128, 16 bits) a warp: 96 KB in flight per CTA, two CTAs on an SM
-    static constexpr int kStages = sizeof(KV) == 4 && D == 128 ? 3 : kRowBytes == 128 ? 6 : 3;
+    // 96 KB in flight per CTA and two CTAs on an SM, or (f32, D = 128) 192 KB and one
+    static constexpr int kStages = kRowBytes == 128 ? 6 : 3;
     static constexpr int kWarpBytes = kStages * 2 * kBlockBytes;
-    static constexpr int kMerge = kFewWarps * 16 * (D + 4) * 4;  // the warps' sums, rows padded by 16 bytes
+    static constexpr int kLd = D + 4;  // row of the warps' sums, floats
+    static constexpr int kMerge = kFewWarps * kRows * kLd * 4;
     static constexpr int kSmem = kFewWarps * kWarpBytes > kMerge ? kFewWarps * kWarpBytes : kMerge;
 };
 
-// Attention of 16 rows of a KV head: grid (split, KV head, row tile, sequence)
+// Attention of 8 NR rows of a KV head: grid (split, KV head, row tile, sequence)
 // in one axis, 4 warps.  The warps share the rows and take turns at blocks of
 // 16 keys, each with a ring of its own in shared memory (no barrier in the
 // loop); at the end they join their (m, l, sum).
 //
-// Bound by memory when a tile holds all rows of its KV head (decoding).  16-bit
-// caches: one m16n8k16 product per 16 keys x 8 dims.  f32 rows over a bf16
-// cache: q and the weights as three bf16 terms.  f32 cache: hi/lo tf32 pairs,
-// three products.  Where the result is f32 a block's P.V is summed apart and
-// added to the running sum by an FMA: the tensor core's own accumulation
-// truncates, which over thousands of keys would show.
-template <typename IO, typename KV, int D>
+// Bound by memory when a tile holds all rows of its KV head (decoding), so the
+// products are turned round: the 16 keys (then the 16 dims of V) are the M of
+// m16n8k16 and the query rows its N, of which eight are enough -- with the rows
+// as M, half of every product of a head group of 8 or fewer was padding.
+//   S^T (16 keys x 8 rows) = K Q^T,  O^T (D x 8 rows) += V^T P^T.
+// A thread holds the scores, maxima and sums of rows 2 t4 and 2 t4 + 1.
+// f32 rows over a bf16 cache: q and the weights as three bf16 terms.  f32 cache:
+// hi/lo tf32 pairs, three products.  Where the result is f32 a block's V^T P^T is
+// summed apart and added to the running sum by an FMA: the tensor core's own
+// accumulation truncates, which over thousands of keys would show.
+template <typename IO, typename KV, int D, int NR>
 __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __grid_constant__ AttnView a) {
-    using C = FewCfg<KV, D>;
+    using C = FewCfg<KV, D, NR>;
     constexpr bool kF32 = sizeof(KV) == 4;
     constexpr bool kExact = sizeof(IO) == 4;
     constexpr int NT = !kF32 && kExact ? 3 : 1;  // bf16 terms of an f32 operand
     constexpr int NK = D / 16;
     extern __shared__ __align__(1024) char smem[];
-    __shared__ float2 ml[kFewWarps][16];
+    __shared__ float2 ml[kFewWarps][C::kRows];
     pdl_wait();
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
@@ -235,7 +249,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
     idx /= a.few.splits;
     const int kvh = (int)(idx % a.p.kv_heads);
     idx /= a.p.kv_heads;
-    const int r0 = (int)(idx % a.row_tiles) * 16, b = (int)(idx / a.row_tiles);
+    const int r0 = (int)(idx % a.row_tiles) * C::kRows, b = (int)(idx / a.row_tiles);
     const PagedSeq s = paged_seq(a.p, b);
     const int rows = s.n * a.group;
     if (r0 >= rows || rows > a.few_rows) return;
@@ -252,8 +266,9 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
         const int key = k_begin + (warp + i * kFewWarps) * kBK + (lane & 15);
         return i < mine && key >= kr.lo && key < k_end ? paged_offset(a.p, b, key) : -1;
     };
-    // 16-byte chunk c of row r sits at chunk c ^ swz(r): the loads below touch 8 rows (or 2 and 4) at once
-    auto swz = [](int r) { return kF32 ? (((r >> 1) & 3) ^ ((r & 1) << 1)) << 1 : r & 7; };
+    // 16-byte chunk c of row r sits at chunk c ^ swz(r): no load below meets a bank twice, be it
+    // 8 rows at one chunk (16 bits), 2 rows x 4 chunks (K) or 4 rows x 2 chunks (V)
+    auto swz = [](int r) { return kF32 ? (((r & 1) << 1) | ((r >> 1) & 1)) << 1 : r & 7; };
     auto fetch = [&](int i, int64_t off) {
         if (i < mine) {
             constexpr int RC = C::kRowBytes / 16, RPI = 32 / RC;
@@ -274,53 +289,55 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
     for (int i = 0; i < C::kStages - 1; i++) fetch(i, look_up(i));
     int64_t next = look_up(C::kStages - 1);
 
-    // rows g and g + 8 of the tile: token, query head, position
-    int pos[2];
-    const char* qp[2];
+    // q, the N operand: row 8 n + g of the tile.  f32 cache: dims 16 kk + 4 t4 .. + 3 (the order
+    // of the dims inside a product is free as long as K's is the same); 16 bits: dims
+    // 16 kk + 2 t4, + 1, + 8, + 9.
+    float qf[kF32 ? NR : 1][NK][4];
+    uint32_t qh[kF32 ? 1 : NR][NK][NT][2];
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int r = r0 + g + 8 * i;
-        pos[i] = r < rows ? s.len - s.n + r / a.group : -1;
-        const int rr = min(r, rows - 1);
-        qp[i] = a.q + (int64_t)(s.start + rr / a.group) * a.q_row + (int64_t)(kvh * a.group + rr % a.group) * a.q_head;
-    }
-    // q fragments.  f32 cache: dims 16 kk + 4 t4 .. + 3 of both rows (the order of
-    // the dims inside a product is free as long as K's is the same).  16 bits: the
-    // m16n8k16 layout, dims 16 kk + 2 t4, + 1, + 8, + 9.
-    float qf[kF32 ? NK : 1][8];
-    uint32_t qh[kF32 ? 1 : NK][NT][4];
-    if constexpr (kF32) {
+    for (int n = 0; n < NR; n++) {
+        const int r = min(r0 + 8 * n + g, rows - 1);
+        const char* qp = a.q + (int64_t)(s.start + r / a.group) * a.q_row + (int64_t)(kvh * a.group + r % a.group) * a.q_head;
 #pragma unroll
-        for (int kk = 0; kk < NK; kk++)
+        for (int kk = 0; kk < NK; kk++) {
+            if constexpr (kF32) {
+                const float4 x = *reinterpret_cast<const float4*>(qp + (16 * kk + 4 * t4) * 4);
+                qf[n][kk][0] = x.x, qf[n][kk][1] = x.y, qf[n][kk][2] = x.z, qf[n][kk][3] = x.w;
+            } else {
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const float4 x = *reinterpret_cast<const float4*>(qp[i] + (16 * kk + 4 * t4) * 4);
-                qf[kk][4 * i] = x.x, qf[kk][4 * i + 1] = x.y, qf[kk][4 * i + 2] = x.z, qf[kk][4 * i + 3] = x.w;
-            }
-    } else {
+                for (int e = 0; e < 2; e++) {
+                    const char* x = qp + (16 * kk + 2 * t4 + 8 * e) * sizeof(IO);
+                    if constexpr (kExact) {
+                        const float2 f = *reinterpret_cast<const float2*>(x);
+                        uint32_t tt[NT];
+                        split_terms<KV, NT>(f.x, f.y, tt);
 #pragma unroll
-        for (int kk = 0; kk < NK; kk++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {  // a0 (g, lo), a1 (g + 8, lo), a2 (g, hi), a3 (g + 8, hi)
-                const char* x = qp[j & 1] + (16 * kk + 2 * t4 + 8 * (j >> 1)) * sizeof(IO);
-                if constexpr (kExact) {
-                    const float2 f = *reinterpret_cast<const float2*>(x);
-                    uint32_t tt[NT];
-                    split_terms<KV, NT>(f.x, f.y, tt);
-#pragma unroll
-                    for (int n = 0; n < NT; n++) qh[kk][n][j] = tt[n];
-                } else {
-                    qh[kk][0][j] = *reinterpret_cast<const uint32_t*>(x);
+                        for (int i = 0; i < NT; i++) qh[n][kk][i][e] = tt[i];
+                    } else {
+                        qh[n][kk][0][e] = *reinterpret_cast<const uint32_t*>(x);
+                    }
                 }
             }
+        }
     }
-
-    float o[D / 8][4];
+    // rows 8 n + 2 t4 + e: position, running maximum and sum
+    int pos[NR][2];
+    float m[NR][2], l[NR][2];
+    float o[NR][D / 16][4];
 #pragma unroll
-    for (int n = 0; n < D / 8; n++)
+    for (int n = 0; n < NR; n++) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[n][e] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        for (int e = 0; e < 2; e++) {
+            const int r = r0 + 8 * n + 2 * t4 + e;
+            pos[n][e] = r < rows ? s.len - s.n + r / a.group : -1;
+            m[n][e] = -INFINITY;
+            l[n][e] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < D / 16; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[n][i][e] = 0.f;
+    }
 
     for (int i = 0; i < mine; i++) {
         cp_async_wait<C::kStages - 2>();
@@ -329,139 +346,158 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
         next = look_up(i + C::kStages);
         const unsigned kb = ring + (unsigned)(i % C::kStages) * 2 * C::kBlockBytes, vb = kb + C::kBlockBytes;
         const int key0 = k_begin + (warp + i * kFewWarps) * kBK;
-        // S: 16 rows x 16 keys as two n-tiles; the small terms in an accumulator of their own
-        float sc[2][4] = {}, sl[2][4] = {};
+        // scores: keys g (e 0, 1) and g + 8 (e 2, 3), rows 2 t4 + (e & 1); the small terms apart
+        float sc[NR][4] = {}, sl[NR][4] = {}, sm[kF32 ? NR : 1][4] = {};
         if constexpr (kF32) {
 #pragma unroll
             for (int kk = 0; kk < NK; kk++) {
-                uint32_t qhi[8], qlo[8];
+                uint32_t kh[2][4], kl[2][4];
 #pragma unroll
-                for (int e = 0; e < 8; e++) split_tf32(qf[kk][e], qhi[e], qlo[e]);
+                for (int h = 0; h < 2; h++) {
+                    const int r = 8 * h + g;
+                    const float4 x = lds128(kb + r * C::kRowBytes + (((4 * kk + t4) ^ swz(r)) << 4));
+                    split_tf32(x.x, kh[h][0], kl[h][0]);
+                    split_tf32(x.y, kh[h][1], kl[h][1]);
+                    split_tf32(x.z, kh[h][2], kl[h][2]);
+                    split_tf32(x.w, kh[h][3], kl[h][3]);
+                }
 #pragma unroll
-                for (int n = 0; n < 2; n++) {
-                    const int r = 8 * n + g;
-                    const float4 kx = lds128(kb + r * C::kRowBytes + (((4 * kk + t4) ^ swz(r)) << 4));
-                    const float kv[4] = {kx.x, kx.y, kx.z, kx.w};
-                    uint32_t khi[4], klo[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) split_tf32(kv[e], khi[e], klo[e]);
+                for (int n = 0; n < NR; n++)
 #pragma unroll
                     for (int h = 0; h < 4; h += 2) {
-                        const uint32_t ah[4] = {qhi[h], qhi[4 + h], qhi[h + 1], qhi[5 + h]};
-                        const uint32_t al[4] = {qlo[h], qlo[4 + h], qlo[h + 1], qlo[5 + h]};
-                        mma8(sc[n], ah, khi[h], khi[h + 1]);
-                        mma8(sl[n], ah, klo[h], klo[h + 1]);
-                        mma8(sl[n], al, khi[h], khi[h + 1]);
+                        uint32_t qhi[2], qlo[2];
+                        split_tf32(qf[n][kk][h], qhi[0], qlo[0]);
+                        split_tf32(qf[n][kk][h + 1], qhi[1], qlo[1]);
+                        const uint32_t ah[4] = {kh[0][h], kh[1][h], kh[0][h + 1], kh[1][h + 1]};
+                        const uint32_t al[4] = {kl[0][h], kl[1][h], kl[0][h + 1], kl[1][h + 1]};
+                        mma8(sc[n], ah, qhi[0], qhi[1]);
+                        mma8(sl[n], al, qhi[0], qhi[1]);
+                        mma8(sm[n], ah, qlo[0], qlo[1]);
                     }
-                }
             }
+#pragma unroll
+            for (int n = 0; n < NR; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) sl[n][e] += sm[n][e];
         } else {
-            const int r = (lane & 7) + ((lane >> 4) << 3), cc = (lane >> 3) & 1;
+            const int r = lane & 15, cc = lane >> 4;
 #pragma unroll
             for (int kk = 0; kk < NK; kk++) {
                 uint32_t kx[4];
                 ldsm4(kb + r * C::kRowBytes + (((2 * kk + cc) ^ swz(r)) << 4), kx);
 #pragma unroll
-                for (int n = 0; n < 2; n++) {
-                    mma16<KV>(sc[n], qh[kk][0], kx[2 * n], kx[2 * n + 1]);
+                for (int n = 0; n < NR; n++) {
+                    mma16<KV>(sc[n], kx, qh[n][kk][0][0], qh[n][kk][0][1]);
 #pragma unroll
-                    for (int x = 1; x < NT; x++) mma16<KV>(sl[n], qh[kk][x], kx[2 * n], kx[2 * n + 1]);
+                    for (int x = 1; x < NT; x++) mma16<KV>(sl[n], kx, qh[n][kk][x][0], qh[n][kk][x][1]);
                 }
             }
         }
-        // weights: rows g (e 0, 1) and g + 8 (e 2, 3), keys key0 + 8 n + 2 t4 + (e & 1)
-        float mx[2] = {m[0], m[1]};
+        float alpha[NR][2];
 #pragma unroll
-        for (int n = 0; n < 2; n++)
+        for (int n = 0; n < NR; n++) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const int key = key0 + 8 * n + 2 * t4 + (e & 1), p = pos[e >> 1];
-                float x = (sc[n][e] + sl[n][e]) * a.scale_log2;
-                if (key > p || key >= k_end || (a.window > 0 && key <= p - a.window)) x = -INFINITY;
-                sc[n][e] = x;
-                mx[e >> 1] = fmaxf(mx[e >> 1], x);
+                const int key = key0 + g + 8 * (e >> 1), p = pos[n][e & 1];
+                const float x = (sc[n][e] + sl[n][e]) * a.scale_log2;
+                sc[n][e] = key > p || key >= k_end || (a.window > 0 && key <= p - a.window) ? -INFINITY : x;
             }
-        float alpha[2];
 #pragma unroll
-        for (int i2 = 0; i2 < 2; i2++) {
-            mx[i2] = fmaxf(mx[i2], __shfl_xor_sync(0xffffffffu, mx[i2], 1));
-            mx[i2] = fmaxf(mx[i2], __shfl_xor_sync(0xffffffffu, mx[i2], 2));
-            const float mb = mx[i2] == -INFINITY ? 0.f : mx[i2];
-            alpha[i2] = ex2_approx(m[i2] - mb);
-            m[i2] = mx[i2];
-            mx[i2] = mb;
-            l[i2] *= alpha[i2];
+            for (int e = 0; e < 2; e++) {
+                float mx = fmaxf(sc[n][e], sc[n][e + 2]);
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                mx = fmaxf(mx, m[n][e]);
+                const float mb = mx == -INFINITY ? 0.f : mx;
+                alpha[n][e] = ex2_approx(m[n][e] - mb);
+                m[n][e] = mx;
+                sc[n][e] = ex2_approx(sc[n][e] - mb);
+                sc[n][e + 2] = ex2_approx(sc[n][e + 2] - mb);
+                l[n][e] = fmaf(l[n][e], alpha[n][e], sc[n][e] + sc[n][e + 2]);
+            }
         }
-#pragma unroll
-        for (int n = 0; n < 2; n++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                sc[n][e] = ex2_approx(sc[n][e] - mx[e >> 1]);
-                l[e >> 1] += sc[n][e];
-            }
-        // P.V
         if constexpr (kF32) {
-            // keys 8 kt + 2 t4 and + 1 of the block are the product's k = t4 and t4 + 4, dims
-            // 32 nn + 4 g + j its column g for j = 0..3: the same order in P and V
-            uint32_t ph[2][4], pl[2][4];
+            // product kt sums keys 8 kt + t4 (k = t4) and + 4 (k = t4 + 4): a row's weights come from
+            // the lanes that hold those keys.  The M rows g and g + 8 of product (np, j) are dims
+            // 64 np + 4 g + j and + 32.
+            uint32_t ph[NR][2][2], pl[NR][2][2];
 #pragma unroll
-            for (int kt = 0; kt < 2; kt++) {
-                split_tf32(sc[kt][0], ph[kt][0], pl[kt][0]);
-                split_tf32(sc[kt][2], ph[kt][1], pl[kt][1]);
-                split_tf32(sc[kt][1], ph[kt][2], pl[kt][2]);
-                split_tf32(sc[kt][3], ph[kt][3], pl[kt][3]);
-            }
+            for (int n = 0; n < NR; n++)
 #pragma unroll
-            for (int nn = 0; nn < D / 32; nn++) {
-                float pv[4][4] = {};
+                for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int src = 4 * (t4 + 4 * h) + (g >> 1);
+                        const float x0 = __shfl_sync(0xffffffffu, sc[n][2 * kt], src);
+                        const float x1 = __shfl_sync(0xffffffffu, sc[n][2 * kt + 1], src);
+                        split_tf32(g & 1 ? x1 : x0, ph[n][kt][h], pl[n][kt][h]);
+                    }
+#pragma unroll
+            for (int np = 0; np < D / 64; np++) {
+                float pv[NR][4][4] = {};
 #pragma unroll
                 for (int kt = 0; kt < 2; kt++) {
-                    const int ra = 8 * kt + 2 * t4;
-                    const float4 va = lds128(vb + ra * C::kRowBytes + (((8 * nn + g) ^ swz(ra)) << 4));
-                    const float4 vc = lds128(vb + (ra + 1) * C::kRowBytes + (((8 * nn + g) ^ swz(ra + 1)) << 4));
-                    const float x0[4] = {va.x, va.y, va.z, va.w}, x1[4] = {vc.x, vc.y, vc.z, vc.w};
+                    // v[2 h + x]: key 8 kt + t4 + 4 h, dims 64 np + 32 x + 4 g ..
+                    uint32_t vh[4][4], vl[4][4];
+#pragma unroll
+                    for (int y = 0; y < 4; y++) {
+                        const int r = 8 * kt + t4 + 4 * (y >> 1);
+                        const float4 x = lds128(vb + r * C::kRowBytes + (((16 * np + 8 * (y & 1) + g) ^ swz(r)) << 4));
+                        split_tf32(x.x, vh[y][0], vl[y][0]);
+                        split_tf32(x.y, vh[y][1], vl[y][1]);
+                        split_tf32(x.z, vh[y][2], vl[y][2]);
+                        split_tf32(x.w, vh[y][3], vl[y][3]);
+                    }
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        uint32_t h0, l0, h1, l1;
-                        split_tf32(x0[j], h0, l0);
-                        split_tf32(x1[j], h1, l1);
-                        mma8(pv[j], pl[kt], h0, h1);
-                        mma8(pv[j], ph[kt], l0, l1);
-                        mma8(pv[j], ph[kt], h0, h1);
+                        const uint32_t ah[4] = {vh[0][j], vh[1][j], vh[2][j], vh[3][j]};
+                        const uint32_t al[4] = {vl[0][j], vl[1][j], vl[2][j], vl[3][j]};
+#pragma unroll
+                        for (int n = 0; n < NR; n++) {
+                            mma8(pv[n][j], al, ph[n][kt][0], ph[n][kt][1]);
+                            mma8(pv[n][j], ah, pl[n][kt][0], pl[n][kt][1]);
+                            mma8(pv[n][j], ah, ph[n][kt][0], ph[n][kt][1]);
+                        }
                     }
                 }
 #pragma unroll
-                for (int j = 0; j < 4; j++)
+                for (int n = 0; n < NR; n++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        o[4 * nn + j][e] = fmaf(o[4 * nn + j][e], alpha[e >> 1], pv[j][e]);
+                    for (int j = 0; j < 4; j++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            o[n][4 * np + j][e] = fmaf(o[n][4 * np + j][e], alpha[n][e & 1], pv[n][j][e]);
             }
         } else {
-            uint32_t ph[NT][4];
+            // weights to the N operand's layout: keys 2 t4, + 1 (+ 8) of row g
+            uint32_t ph[NR][NT][2];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                uint32_t tt[NT];
-                split_terms<KV, NT>(sc[j >> 1][2 * (j & 1)], sc[j >> 1][2 * (j & 1) + 1], tt);
-#pragma unroll
-                for (int x = 0; x < NT; x++) ph[x][j] = tt[x];
-            }
-            const int r = lane & 15, cc = lane >> 4;
-#pragma unroll
-            for (int n = 0; n < D / 8; n += 2) {
-                uint32_t vx[4];
-                ldsm4_t(vb + r * C::kRowBytes + (((n + cc) ^ swz(r)) << 4), vx);
+            for (int n = 0; n < NR; n++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
+                    uint32_t tt[NT];
+                    split_terms<KV, NT>(sc[n][2 * h], sc[n][2 * h + 1], tt);
+#pragma unroll
+                    for (int x = 0; x < NT; x++) ph[n][x][h] = mat_t(tt[x]);
+                }
+            const int r = (lane & 7) + ((lane >> 4) << 3), cc = (lane >> 3) & 1;
+#pragma unroll
+            for (int i2 = 0; i2 < D / 16; i2++) {
+                uint32_t vx[4];
+                ldsm4_t(vb + r * C::kRowBytes + (((2 * i2 + cc) ^ swz(r)) << 4), vx);
+#pragma unroll
+                for (int n = 0; n < NR; n++) {
                     if constexpr (kExact) {
                         float pv[4] = {};
 #pragma unroll
-                        for (int x = NT - 1; x >= 0; x--) mma16<KV>(pv, ph[x], vx[2 * h], vx[2 * h + 1]);
+                        for (int x = NT - 1; x >= 0; x--) mma16<KV>(pv, vx, ph[n][x][0], ph[n][x][1]);
 #pragma unroll
-                        for (int e = 0; e < 4; e++) o[n + h][e] = fmaf(o[n + h][e], alpha[e >> 1], pv[e]);
+                        for (int e = 0; e < 4; e++) o[n][i2][e] = fmaf(o[n][i2][e], alpha[n][e & 1], pv[e]);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) o[n + h][e] *= alpha[e >> 1];
-                        mma16<KV>(o[n + h], ph[0], vx[2 * h], vx[2 * h + 1]);
+                        for (int e = 0; e < 4; e++) o[n][i2][e] *= alpha[n][e & 1];
+                        mma16<KV>(o[n][i2], vx, ph[n][0][0], ph[n][0][1]);
                     }
                 }
             }
@@ -470,59 +506,56 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
     cp_async_wait<0>();
     // join the warps: every warp's sums to shared memory, then all threads over (row, dims)
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        if (t4 == 0) ml[warp][g + 8 * i] = make_float2(m[i], l[i]);
-    }
+    for (int n = 0; n < NR; n++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 4);
+            l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 8);
+            l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
+            if (g == 0) ml[warp][8 * n + 2 * t4 + e] = make_float2(m[n][e], l[n][e]);
+        }
     __syncthreads();  // the rings are free
     float* sums = reinterpret_cast<float*>(smem);
-    constexpr int LD = D + 4;
 #pragma unroll
-    for (int n = 0; n < D / 8; n++)
+    for (int n = 0; n < NR; n++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            // f32: n-tile 4 nn + j column c is dim 32 nn + 4 c + j; 16 bits: 8 n + c
-            const int c = 2 * t4 + (e & 1);
-            const int d = kF32 ? 32 * (n >> 2) + 4 * c + (n & 3) : 8 * n + c;
-            sums[(warp * 16 + g + 8 * (e >> 1)) * LD + d] = o[n][e];
-        }
+        for (int i = 0; i < D / 16; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int d = kF32 ? 64 * (i >> 2) + 32 * (e >> 1) + 4 * g + (i & 3) : 16 * i + 8 * (e >> 1) + g;
+                sums[(warp * C::kRows + 8 * n + 2 * t4 + (e & 1)) * C::kLd + d] = o[n][i][e];
+            }
     __syncthreads();
-    constexpr int TR = kFewWarps * 32 / 16;  // threads of a row
-    const int row = threadIdx.x / TR, r = r0 + row;
-    if (r >= rows) return;
-    float M = -INFINITY, L = 0.f, w[kFewWarps];
-#pragma unroll
-    for (int x = 0; x < kFewWarps; x++) M = fmaxf(M, ml[x][row].x);
-#pragma unroll
-    for (int x = 0; x < kFewWarps; x++) {
-        w[x] = ex2_approx(ml[x][row].x - (M == -INFINITY ? 0.f : M));
-        L += ml[x][row].y * w[x];
-    }
-    const int token = s.start + r / a.group, head = kvh * a.group + r % a.group;
-    const int64_t th = (int64_t)token * a.heads + head;
     const bool last = a.few.splits == 1;
-    const float inv = last ? (L > 0.f ? 1.f / L : 0.f) : 1.f;
-#pragma unroll
-    for (int c = 0; c < D / 8 / TR; c++) {
-        const int d = (c * TR + threadIdx.x % TR) * 8;
+    for (int it = threadIdx.x; it < C::kRows * (D / 8); it += kFewWarps * 32) {
+        const int row = it / (D / 8), r = r0 + row, d = it % (D / 8) * 8;
+        if (r >= rows) break;
+        float M = -INFINITY, L = 0.f;
         float y[8] = {};
 #pragma unroll
-        for (int x = 0; x < kFewWarps; x++)
+        for (int x = 0; x < kFewWarps; x++) M = fmaxf(M, ml[x][row].x);
 #pragma unroll
-            for (int e = 0; e < 8; e++) y[e] = fmaf(w[x], sums[(x * 16 + row) * LD + d + e], y[e]);
+        for (int x = 0; x < kFewWarps; x++) {
+            const float w = ex2_approx(ml[x][row].x - (M == -INFINITY ? 0.f : M));
+            L = fmaf(ml[x][row].y, w, L);
+            float z[8];
+            Eight<float>::load(sums + (x * C::kRows + row) * C::kLd + d, z);
 #pragma unroll
-        for (int e = 0; e < 8; e++) y[e] *= inv;
-        if (last)
+            for (int e = 0; e < 8; e++) y[e] = fmaf(w, z[e], y[e]);
+        }
+        const int token = s.start + r / a.group, head = kvh * a.group + r % a.group;
+        const int64_t th = (int64_t)token * a.heads + head;
+        const int64_t pth = (int64_t)split * a.p.tokens * a.heads + th;
+        if (last) {
+            const float inv = L > 0.f ? 1.f / L : 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] *= inv;
             Eight<IO>::store(a.out + token * a.o_row + head * a.o_head + d * sizeof(IO), y);
-        else
-            Eight<float>::store(a.part + ((int64_t)split * a.p.tokens * a.heads + th) * D + d, y);
-    }
-    if (threadIdx.x % TR == 0) {
-        if (!last)
-            a.part_ml[(int64_t)split * a.p.tokens * a.heads + th] = make_float2(M, L);
-        else if (a.lse)
-            a.lse[th] = L > 0.f ? (M + log2f(L)) * 0.693147180559945309f : -INFINITY;
+            if (d == 0 && a.lse) a.lse[th] = L > 0.f ? (M + log2f(L)) * 0.693147180559945309f : -INFINITY;
+        } else {
+            Eight<float>::store(a.part + pth * D + d, y);
+            if (d == 0) a.part_ml[pth] = make_float2(M, L);
+        }
     }
 }
 
@@ -1160,7 +1193,10 @@ Plan make_plan(const PagedView& p, int io, int cache, int heads, int window) {
     const bool tc = io != VB_F32 && most > kFewRows;
     pl.few_rows = !tc ? 0x7fffffff : p.batch == 1 ? 0 : kFewRows;
     const int64_t few_most = std::min<int64_t>(most, pl.few_rows);
-    pl.row_tiles = (int)((few_most + 15) / 16);
+    // rows of a tile: all of a sequence's where that is at most 32 (16 where q takes three terms or
+    // 32 bits: more do not fit the registers)
+    const int tile = few_most <= 8 ? 8 : few_most <= 16 || io == VB_F32 ? 16 : 32;
+    pl.row_tiles = (int)((few_most + tile - 1) / tile);
     const int64_t all = std::max(p.max_len, 1);
     // keys from a tile's base (its first row's lowest, rounded down) to its last row's
     auto span = [&](int rows, int align) {
@@ -1168,9 +1204,9 @@ Plan make_plan(const PagedView& p, int io, int cache, int heads, int window) {
     };
     // few rows: about four CTAs for each SM (two run at a time) of at least 64 keys, one block of
     // 16 a warp; many: one CTA for each SM of at least 512 keys
-    const int64_t tiles = std::max<int64_t>(1, std::min<int64_t>((int64_t)p.batch * pl.row_tiles, total / 16 + p.batch));
+    const int64_t tiles = std::max<int64_t>(1, std::min<int64_t>((int64_t)p.batch * pl.row_tiles, total / tile + p.batch));
     const int64_t want = std::max<int64_t>(1, 148 * 4 / (tiles * p.kv_heads));
-    pl.few = make_cut(16, 16, span(16, 16), want, 64, 64);
+    pl.few = make_cut(tile, 16, span(tile, 16), want, 64, 64);
     const int64_t tiles2 = std::max<int64_t>(1, (total + kTcRows - 1) / kTcRows);
     const int64_t want2 = std::max<int64_t>(1, 148 / (tiles2 * p.kv_heads));
     pl.many = make_cut(kTcRows, 128, span(kTcRows, 128), want2, 128, 512);
@@ -1203,6 +1239,18 @@ int page_map(const PagedView& p, const char* base, int D, bool half, CUtensorMap
     return r == CUDA_SUCCESS ? box : 0;
 }
 
+template <typename IO, typename KV, int D, int NR>
+vb_status launch_few(const AttnView& a, cudaStream_t s) {
+    using C = FewCfg<KV, D, NR>;
+    static std::atomic<unsigned long long> done{0};
+    cudaError_t e = smem_attr_once(paged_attn_few_kernel<IO, KV, D, NR>, C::kSmem, done);
+    if (e != cudaSuccess) return cuda_fail(e, "paged attention: shared memory attribute");
+    const int64_t grid = (int64_t)a.few.splits * a.p.kv_heads * a.row_tiles * a.p.batch;
+    if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
+    e = launch_pdl(paged_attn_few_kernel<IO, KV, D, NR>, dim3((unsigned)grid), dim3(kFewWarps * 32), C::kSmem, s, a);
+    return e == cudaSuccess ? VB_OK : cuda_fail(e, "paged_attn_few_kernel");
+}
+
 template <typename IO, typename KV, int D>
 vb_status launch_attn(const AttnView& a, cudaStream_t s) {
     cudaError_t e;
@@ -1226,14 +1274,15 @@ vb_status launch_attn(const AttnView& a, cudaStream_t s) {
         }
     }
     if (a.few_rows) {
-        using C = FewCfg<KV, D>;
-        static std::atomic<unsigned long long> done{0};
-        e = smem_attr_once(paged_attn_few_kernel<IO, KV, D>, C::kSmem, done);
-        if (e != cudaSuccess) return cuda_fail(e, "paged attention: shared memory attribute");
-        const int64_t grid = (int64_t)a.few.splits * a.p.kv_heads * a.row_tiles * a.p.batch;
-        if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
-        e = launch_pdl(paged_attn_few_kernel<IO, KV, D>, dim3((unsigned)grid), dim3(kFewWarps * 32), C::kSmem, s, a);
-        if (e != cudaSuccess) return cuda_fail(e, "paged_attn_few_kernel");
+        vb_status st = VB_OK;
+        if (a.few.rows == 8) {
+            st = launch_few<IO, KV, D, 1>(a, s);
+        } else if (sizeof(IO) == 4 || a.few.rows == 16) {
+            st = launch_few<IO, KV, D, 2>(a, s);
+        } else {
+            if constexpr (sizeof(IO) == 2) st = launch_few<IO, KV, D, 4>(a, s);
+        }
+        if (st) return st;
     }
     if (a.few.splits > 1 || a.many.splits > 1) {
         const int64_t grid = ((int64_t)a.p.tokens * a.heads + 3) / 4;
