@@ -80,10 +80,13 @@ struct AttnView {
     int window;
     int few_rows;       // sequences with at most this many rows a KV head run in the few-rows kernel
     int row_tiles;      // its row tiles of a sequence
+    int stream;         // blocks that share all its keys evenly (one row tile a sequence); 0: a block per tile and split
     Cut few, many;
     int box;            // rows of a page that one TMA copy brings (many rows); 0: no tensor maps
     float* part;        // [split][token][head][D] sums of a split, relative to its maximum
     float2* part_ml;    // [split][token][head] (maximum in base 2, sum of weights)
+    float* strm;        // the same of the shared keys: [block][2][tile row][D]
+    float2* strm_ml;    // [block][2][tile row]
 };
 
 // The keys that the tile's rows r0 .. r0 + cut.rows - 1 (of n * G) of a sequence see.
@@ -100,6 +103,37 @@ __device__ __forceinline__ KeyRange key_range(const AttnView& a, const PagedSeq&
     k.lo = min(k.lo, k.hi);
     k.base = k.lo & -cut.align;
     return k;
+}
+// Sharing out the keys of the few-rows kernel's tiles.  A tile (sequence, KV head) is
+// units of 64 keys, one at least; the units of all sequences follow one another, KV heads
+// within a sequence, and block c of N <= W takes units [c W / N, (c + 1) W / N).
+constexpr int kUnit = 64;
+__device__ __forceinline__ int stream_units(const AttnView& a, int b) {
+    const int start = a.p.q_start[b], end = a.p.q_start[b + 1];
+    const int64_t rows = (int64_t)(end - start) * a.group;
+    if (start < 0 || end <= start || end > a.p.tokens || end - start > a.p.max_new || rows > a.few_rows) return 0;
+    PagedSeq s;
+    s.n = end - start;
+    s.len = a.p.lens[b];
+    if (s.len < 0 || s.len > a.p.max_len) s.len = 0;
+    const KeyRange k = key_range(a, s, 0, a.few);
+    return max(1, (k.hi - k.base + kUnit - 1) / kUnit);
+}
+// Units of all sequences, and of those before sequence b, of one KV head; by the whole warp.
+__device__ __forceinline__ void stream_sums(const AttnView& a, int b, int lane, int64_t& all, int64_t& before) {
+    int64_t x = 0, y = 0;
+    for (int i = lane; i < a.p.batch; i += 32) {
+        const int u = stream_units(a, i);
+        x += u;
+        if (i < b) y += u;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        x += __shfl_xor_sync(0xffffffffu, x, o);
+        y += __shfl_xor_sync(0xffffffffu, y, o);
+    }
+    all = x * a.p.kv_heads;
+    before = y * a.p.kv_heads;
 }
 __device__ __forceinline__ int splits_used(const Cut& c, const KeyRange& k) {
     return max(1, (k.hi - k.base + c.len - 1) / c.len);
@@ -201,6 +235,12 @@ __device__ __forceinline__ uint32_t mat_t(uint32_t a) {
 }
 
 // ------------------------------------------------------------- few rows
+// The same by cutting the bits off: cheaper, for the operand whose other one is rounded
+// (the product of two cut-off rests would be of one sign, and add up).
+__device__ __forceinline__ void cut_tf32(float x, uint32_t& hi, uint32_t& lo) {
+    hi = __float_as_uint(x) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
+}
 constexpr int kFewWarps = 4;
 constexpr int kBK = 16;  // keys a warp takes at a time
 
@@ -217,10 +257,9 @@ struct FewCfg {
     static constexpr int kSmem = kFewWarps * kWarpBytes > kMerge ? kFewWarps * kWarpBytes : kMerge;
 };
 
-// Attention of 8 NR rows of a KV head: grid (split, KV head, row tile, sequence)
-// in one axis, 4 warps.  The warps share the rows and take turns at blocks of
-// 16 keys, each with a ring of its own in shared memory (no barrier in the
-// loop); at the end they join their (m, l, sum).
+// Attention of 8 NR rows of a KV head by 4 warps.  The warps share the rows and
+// take turns at blocks of 16 keys, each with a ring of its own in shared memory
+// (no barrier in the loop); at the end they join their (m, l, sum).
 //
 // Bound by memory when a tile holds all rows of its KV head (decoding), so the
 // products are turned round: the 16 keys (then the 16 dims of V) are the M of
@@ -232,30 +271,27 @@ struct FewCfg {
 // hi/lo tf32 pairs, three products.  Where the result is f32 a block's V^T P^T is
 // summed apart and added to the running sum by an FMA: the tensor core's own
 // accumulation truncates, which over thousands of keys would show.
+// Where a piece of a tile's keys leaves its rows: the output, or sums to be joined.
+struct Sink {
+    bool last;       // the piece is the whole tile
+    float* part;     // row `row` of the tile at part + row_of(row) * D
+    float2* ml;
+    int64_t base;    // row_of: split * tokens * heads + token * heads + head, or (by_row) the tile's row
+    bool by_row;
+};
+
+// Rows r0 .. of KV head kvh of sequence b over keys k_begin .. k_end - 1, by the block.
 template <typename IO, typename KV, int D, int NR>
-__global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __grid_constant__ AttnView a) {
+__device__ __forceinline__ void few_piece(const AttnView& a, const PagedSeq& s, int b, int kvh, int r0, const KeyRange& kr,
+                                          int k_begin, int k_end, const Sink& sink, char* smem,
+                                          float2 (*ml)[8 * NR]) {
     using C = FewCfg<KV, D, NR>;
     constexpr bool kF32 = sizeof(KV) == 4;
     constexpr bool kExact = sizeof(IO) == 4;
     constexpr int NT = !kF32 && kExact ? 3 : 1;  // bf16 terms of an f32 operand
     constexpr int NK = D / 16;
-    extern __shared__ __align__(1024) char smem[];
-    __shared__ float2 ml[kFewWarps][C::kRows];
-    pdl_wait();
-    pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-    int64_t idx = blockIdx.x;
-    const int split = (int)(idx % a.few.splits);
-    idx /= a.few.splits;
-    const int kvh = (int)(idx % a.p.kv_heads);
-    idx /= a.p.kv_heads;
-    const int r0 = (int)(idx % a.row_tiles) * C::kRows, b = (int)(idx / a.row_tiles);
-    const PagedSeq s = paged_seq(a.p, b);
     const int rows = s.n * a.group;
-    if (r0 >= rows || rows > a.few_rows) return;
-    const KeyRange kr = key_range(a, s, r0, a.few);
-    if (split >= splits_used(a.few, kr)) return;
-    const int k_begin = kr.base + split * a.few.len, k_end = min(k_begin + a.few.len, kr.hi);
     const int blocks = max(0, (k_end - k_begin + kBK - 1) / kBK);
     const int mine = blocks > warp ? (blocks - warp + kFewWarps - 1) / kFewWarps : 0;  // blocks warp, warp + 4, ...
 
@@ -356,10 +392,10 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
                 for (int h = 0; h < 2; h++) {
                     const int r = 8 * h + g;
                     const float4 x = lds128(kb + r * C::kRowBytes + (((4 * kk + t4) ^ swz(r)) << 4));
-                    split_tf32(x.x, kh[h][0], kl[h][0]);
-                    split_tf32(x.y, kh[h][1], kl[h][1]);
-                    split_tf32(x.z, kh[h][2], kl[h][2]);
-                    split_tf32(x.w, kh[h][3], kl[h][3]);
+                    cut_tf32(x.x, kh[h][0], kl[h][0]);
+                    cut_tf32(x.y, kh[h][1], kl[h][1]);
+                    cut_tf32(x.z, kh[h][2], kl[h][2]);
+                    cut_tf32(x.w, kh[h][3], kl[h][3]);
                 }
 #pragma unroll
                 for (int n = 0; n < NR; n++)
@@ -444,10 +480,10 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
                     for (int y = 0; y < 4; y++) {
                         const int r = 8 * kt + t4 + 4 * (y >> 1);
                         const float4 x = lds128(vb + r * C::kRowBytes + (((16 * np + 8 * (y & 1) + g) ^ swz(r)) << 4));
-                        split_tf32(x.x, vh[y][0], vl[y][0]);
-                        split_tf32(x.y, vh[y][1], vl[y][1]);
-                        split_tf32(x.z, vh[y][2], vl[y][2]);
-                        split_tf32(x.w, vh[y][3], vl[y][3]);
+                        cut_tf32(x.x, vh[y][0], vl[y][0]);
+                        cut_tf32(x.y, vh[y][1], vl[y][1]);
+                        cut_tf32(x.z, vh[y][2], vl[y][2]);
+                        cut_tf32(x.w, vh[y][3], vl[y][3]);
                     }
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
@@ -526,7 +562,6 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
                 sums[(warp * C::kRows + 8 * n + 2 * t4 + (e & 1)) * C::kLd + d] = o[n][i][e];
             }
     __syncthreads();
-    const bool last = a.few.splits == 1;
     for (int it = threadIdx.x; it < C::kRows * (D / 8); it += kFewWarps * 32) {
         const int row = it / (D / 8), r = r0 + row, d = it % (D / 8) * 8;
         if (r >= rows) break;
@@ -545,16 +580,91 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
         }
         const int token = s.start + r / a.group, head = kvh * a.group + r % a.group;
         const int64_t th = (int64_t)token * a.heads + head;
-        const int64_t pth = (int64_t)split * a.p.tokens * a.heads + th;
-        if (last) {
+        if (sink.last) {
             const float inv = L > 0.f ? 1.f / L : 0.f;
 #pragma unroll
             for (int e = 0; e < 8; e++) y[e] *= inv;
             Eight<IO>::store(a.out + token * a.o_row + head * a.o_head + d * sizeof(IO), y);
             if (d == 0 && a.lse) a.lse[th] = L > 0.f ? (M + log2f(L)) * 0.693147180559945309f : -INFINITY;
         } else {
-            Eight<float>::store(a.part + pth * D + d, y);
-            if (d == 0) a.part_ml[pth] = make_float2(M, L);
+            const int64_t at = sink.base + (sink.by_row ? row : th);
+            Eight<float>::store(sink.part + at * D + d, y);
+            if (d == 0) sink.ml[at] = make_float2(M, L);
+        }
+    }
+}
+
+// STREAM: the keys of all tiles shared out evenly; else a grid of (split, KV head, row tile,
+// sequence) in one axis.
+template <typename IO, typename KV, int D, int NR, bool STREAM>
+__global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __grid_constant__ AttnView a) {
+    using C = FewCfg<KV, D, NR>;
+    extern __shared__ __align__(1024) char smem[];
+    __shared__ float2 ml[kFewWarps][C::kRows];
+    pdl_wait();
+    pdl_trigger();
+    if constexpr (!STREAM) {
+        int64_t idx = blockIdx.x;
+        const int split = (int)(idx % a.few.splits);
+        idx /= a.few.splits;
+        const int kvh = (int)(idx % a.p.kv_heads);
+        idx /= a.p.kv_heads;
+        const int r0 = (int)(idx % a.row_tiles) * C::kRows, b = (int)(idx / a.row_tiles);
+        const PagedSeq s = paged_seq(a.p, b);
+        const int rows = s.n * a.group;
+        if (r0 >= rows || rows > a.few_rows) return;
+        const KeyRange kr = key_range(a, s, r0, a.few);
+        if (split >= splits_used(a.few, kr)) return;
+        const int k_begin = kr.base + split * a.few.len;
+        const Sink sink{a.few.splits == 1, a.part, a.part_ml, (int64_t)split * a.p.tokens * a.heads, false};
+        few_piece<IO, KV, D, NR>(a, s, b, kvh, r0, kr, k_begin, min(k_begin + a.few.len, kr.hi), sink, smem, ml);
+    } else {
+        // this block's units, piece by piece: a piece is what it has of one tile
+        const int lane = threadIdx.x & 31;
+        int64_t all, dummy;
+        stream_sums(a, 0, lane, all, dummy);
+        const int64_t blocks = min((int64_t)a.stream, all);  // no block between others is empty
+        if (blockIdx.x >= blocks) return;
+        int64_t u = all * blockIdx.x / blocks;
+        const int64_t u_end = all * (blockIdx.x + 1) / blocks;
+        // the sequence of unit u: 32 sequences a step
+        int b = 0;
+        int64_t off = u;  // u's number within sequence b
+        for (int b0 = 0; b0 < a.p.batch; b0 += 32) {
+            const int64_t mine = b0 + lane < a.p.batch ? (int64_t)stream_units(a, b0 + lane) * a.p.kv_heads : 0;
+            int64_t sum = mine;
+    #pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t x = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += x;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, sum > off);
+            if (past) {
+                const int l = __ffs(past) - 1;
+                off -= __shfl_sync(0xffffffffu, sum - mine, l);
+                b = b0 + l;
+                break;
+            }
+            off -= __shfl_sync(0xffffffffu, sum, 31);
+        }
+        while (u < u_end) {
+            const int n = stream_units(a, b);  // units of a tile
+            if (n == 0 || off >= (int64_t)n * a.p.kv_heads) {
+                off -= (int64_t)n * a.p.kv_heads;
+                if (++b >= a.p.batch) return;  // (the lengths changed under the kernel)
+                continue;
+            }
+            const PagedSeq s = paged_seq(a.p, b);
+            const KeyRange kr = key_range(a, s, 0, a.few);
+            const int kvh = (int)(off / n), first = (int)(off % n);
+            const int take = (int)min((int64_t)(n - first), u_end - u);
+            const int slot = first > 0 ? 0 : 1;  // a tile begun by an earlier block; begun here
+            const Sink sink{take == n, a.strm, a.strm_ml, ((int64_t)blockIdx.x * 2 + slot) * C::kRows, true};
+            const int k_begin = kr.base + first * kUnit;
+            few_piece<IO, KV, D, NR>(a, s, b, kvh, 0, kr, k_begin, min(k_begin + take * kUnit, kr.hi), sink, smem, ml);
+            u += take;
+            off += take;
+            __syncthreads();  // the shared memory is free for the next piece
         }
     }
 }
@@ -1140,20 +1250,44 @@ __global__ void __launch_bounds__(128) paged_attn_merge_kernel(const __grid_cons
     const PagedSeq s = paged_seq(a.p, b);
     if (!s.ok || token < s.start || token >= s.start + s.n) return;
     const int r = (token - s.start) * a.group + head % a.group;
-    const Cut& cut = s.n * a.group > a.few_rows ? a.many : a.few;
-    if (cut.splits == 1) return;  // written by the kernel itself
-    const int used = splits_used(cut, key_range(a, s, r / cut.rows * cut.rows, cut));
+    // part x of the row is at at0 + x * step
+    const bool few = s.n * a.group <= a.few_rows;
+    int used;
+    int64_t at0 = th, step = (int64_t)a.p.tokens * a.heads;
+    const float* part = a.part;
+    const float2* part_ml = a.part_ml;
+    if (few && a.stream) {
+        int64_t all, u0;
+        stream_sums(a, b, lane, all, u0);
+        const int n = stream_units(a, b);
+        u0 += (int64_t)(head / a.group) * n;
+        // the block of unit u: the last c with c W / N <= u, rounded down
+        const int64_t blocks = min((int64_t)a.stream, all);
+        const int64_t c0 = ((u0 + 1) * blocks - 1) / all, c1 = ((u0 + n) * blocks - 1) / all;
+        used = (int)(c1 - c0) + 1;
+        if (used == 1) return;  // written by the kernel itself
+        // slot 1 of block c0, then slot 0 of the next ones
+        part = a.strm;
+        part_ml = a.strm_ml;
+        step = 2 * a.few.rows;
+        at0 = c0 * step + r;
+    } else {
+        const Cut& cut = few ? a.few : a.many;
+        if (cut.splits == 1) return;  // written by the kernel itself
+        used = splits_used(cut, key_range(a, s, r / cut.rows * cut.rows, cut));
+    }
+    const int64_t first = few && a.stream ? a.few.rows : 0;  // part 0 is a slot further
     constexpr int E = D / 32;
     float y[E] = {}, M = -INFINITY, L = 0.f;
-    const int64_t step = (int64_t)a.p.tokens * a.heads;
-    for (int x = lane; x < used; x += 32) M = fmaxf(M, a.part_ml[x * step + th].x);
+    for (int x = lane; x < used; x += 32) M = fmaxf(M, part_ml[at0 + x * step + (x == 0 ? first : 0)].x);
     M = warp_max(M);
     const float mb = M == -INFINITY ? 0.f : M;
     for (int x = 0; x < used; x++) {
-        const float2 p = a.part_ml[x * step + th];
+        const int64_t at = at0 + x * step + (x == 0 ? first : 0);
+        const float2 p = part_ml[at];
         const float w = ex2_approx(p.x - mb);
         L = fmaf(p.y, w, L);
-        const float* src = a.part + (x * step + th) * D + lane * E;
+        const float* src = part + at * D + lane * E;
 #pragma unroll
         for (int e = 0; e < E; e++) y[e] = fmaf(w, src[e], y[e]);
     }
@@ -1168,7 +1302,7 @@ __global__ void __launch_bounds__(128) paged_attn_merge_kernel(const __grid_cons
 // launch holds for any lengths within them.  A tile's keys are split where the
 // tiles alone do not fill the card.
 struct Plan {
-    int few_rows, row_tiles;
+    int few_rows, row_tiles, stream;
     Cut few, many;
     int max_splits;  // for any window
 };
@@ -1184,7 +1318,7 @@ Cut make_cut(int rows, int align, int64_t keys, int64_t want, int step, int leas
     return c;
 }
 
-Plan make_plan(const PagedView& p, int io, int cache, int heads, int window) {
+Plan make_plan(const PagedView& p, int io, int cache, int heads, int D, int window) {
     Plan pl{};
     const int G = heads / p.kv_heads;
     const int64_t most = (int64_t)p.max_new * G, total = (int64_t)p.tokens * G;  // rows of a KV head
@@ -1202,10 +1336,16 @@ Plan make_plan(const PagedView& p, int io, int cache, int heads, int window) {
     auto span = [&](int rows, int align) {
         return window > 0 ? std::min<int64_t>(all, (int64_t)window + (rows + G - 1) / G + align - 1) : all;
     };
-    // few rows: about four CTAs for each SM (two run at a time) of at least 64 keys, one block of
-    // 16 a warp; many: one CTA for each SM of at least 512 keys
+    // few rows: where a sequence's rows are one tile its keys are shared out evenly over as many
+    // blocks as the card runs at a time; else about four CTAs for each SM of at least 64 keys (one
+    // block of 16 a warp).  Many: one CTA for each SM of at least 512 keys.
     const int64_t tiles = std::max<int64_t>(1, std::min<int64_t>((int64_t)p.batch * pl.row_tiles, total / tile + p.batch));
-    const int64_t want = std::max<int64_t>(1, 148 * 4 / (tiles * p.kv_heads));
+    const int64_t want = pl.row_tiles == 1 ? 1 : std::max<int64_t>(1, 148 * 4 / (tiles * p.kv_heads));
+    if (pl.row_tiles == 1) {
+        const int64_t most_units = (int64_t)p.batch * p.kv_heads * ((span(tile, 16) + kUnit - 1) / kUnit);
+        const int per_sm = cache == VB_F32 && D == 128 ? 1 : 2;
+        pl.stream = (int)std::min<int64_t>(148 * per_sm, most_units);
+    }
     pl.few = make_cut(tile, 16, span(tile, 16), want, 64, 64);
     const int64_t tiles2 = std::max<int64_t>(1, (total + kTcRows - 1) / kTcRows);
     const int64_t want2 = std::max<int64_t>(1, 148 / (tiles2 * p.kv_heads));
@@ -1217,7 +1357,8 @@ Plan make_plan(const PagedView& p, int io, int cache, int heads, int window) {
     return pl;
 }
 size_t plan_bytes(const Plan& pl, const PagedView& p, int heads, int D) {
-    return pl.max_splits > 1 ? (size_t)pl.max_splits * p.tokens * heads * (D + 2) * 4 : 0;
+    return (pl.max_splits > 1 ? (size_t)pl.max_splits * p.tokens * heads * (D + 2) * 4 : 0) +
+           (pl.row_tiles == 1 ? (size_t)148 * 2 * 2 * pl.few.rows * (D + 2) * 4 : 0);
 }
 
 // Tensor map of a pool as [page][kv head][position][dim], boxes of one page's rows (128 at
@@ -1239,16 +1380,21 @@ int page_map(const PagedView& p, const char* base, int D, bool half, CUtensorMap
     return r == CUDA_SUCCESS ? box : 0;
 }
 
-template <typename IO, typename KV, int D, int NR>
+template <typename IO, typename KV, int D, int NR, bool STREAM>
 vb_status launch_few(const AttnView& a, cudaStream_t s) {
     using C = FewCfg<KV, D, NR>;
     static std::atomic<unsigned long long> done{0};
-    cudaError_t e = smem_attr_once(paged_attn_few_kernel<IO, KV, D, NR>, C::kSmem, done);
+    cudaError_t e = smem_attr_once(paged_attn_few_kernel<IO, KV, D, NR, STREAM>, C::kSmem, done);
     if (e != cudaSuccess) return cuda_fail(e, "paged attention: shared memory attribute");
-    const int64_t grid = (int64_t)a.few.splits * a.p.kv_heads * a.row_tiles * a.p.batch;
+    const int64_t grid = STREAM ? a.stream : (int64_t)a.few.splits * a.p.kv_heads * a.row_tiles * a.p.batch;
     if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
-    e = launch_pdl(paged_attn_few_kernel<IO, KV, D, NR>, dim3((unsigned)grid), dim3(kFewWarps * 32), C::kSmem, s, a);
+    e = launch_pdl(paged_attn_few_kernel<IO, KV, D, NR, STREAM>, dim3((unsigned)grid), dim3(kFewWarps * 32), C::kSmem, s, a);
     return e == cudaSuccess ? VB_OK : cuda_fail(e, "paged_attn_few_kernel");
+}
+
+template <typename IO, typename KV, int D, int NR>
+vb_status launch_few(const AttnView& a, cudaStream_t s) {
+    return a.stream ? launch_few<IO, KV, D, NR, true>(a, s) : launch_few<IO, KV, D, NR, false>(a, s);
 }
 
 template <typename IO, typename KV, int D>
@@ -1284,7 +1430,7 @@ vb_status launch_attn(const AttnView& a, cudaStream_t s) {
         }
         if (st) return st;
     }
-    if (a.few.splits > 1 || a.many.splits > 1) {
+    if (a.stream > 1 || a.few.splits > 1 || a.many.splits > 1) {
         const int64_t grid = ((int64_t)a.p.tokens * a.heads + 3) / 4;
         if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
         e = launch_pdl(paged_attn_merge_kernel<IO, D>, dim3((unsigned)grid), dim3(128), 0, s, a);
@@ -1313,7 +1459,7 @@ extern "C" size_t vb_paged_attn_workspace_bytes(const vb_paged_cache* cache, con
     size_t most = 0;  // rows of the cache's type or, over a bf16 cache, f32
     for (const int io : {cache->dtype, (int)VB_F32})
         if (io == cache->dtype || cache->dtype == VB_BF16)
-            most = std::max(most, plan_bytes(make_plan(p, io, cache->dtype, heads, 0), p, heads, cache->head_dim));
+            most = std::max(most, plan_bytes(make_plan(p, io, cache->dtype, heads, cache->head_dim, 0), p, heads, cache->head_dim));
     return most;
 }
 
@@ -1330,7 +1476,7 @@ extern "C" vb_status vb_paged_attn(const vb_paged_cache* cache, const vb_paged_b
     const int es = paged_elem_bytes(io), D = cache->head_dim;
     if (!paged_aligned(q, q_row, q_head, es) || !paged_aligned(out, o_row, o_head, es) || !paged_aligned(workspace, 0, 0, 1))
         return fail(VB_ERR_UNSUPPORTED, "paged_attn: 16-byte alignment required");
-    const Plan pl = make_plan(a.p, io, cache->dtype, heads, window);
+    const Plan pl = make_plan(a.p, io, cache->dtype, heads, D, window);
     const size_t need = plan_bytes(pl, a.p, heads, D);
     if (need > workspace_bytes || (need && !workspace))
         return fail(VB_ERR_ARG, "paged_attn: the workspace is too small");
@@ -1345,9 +1491,17 @@ extern "C" vb_status vb_paged_attn(const vb_paged_cache* cache, const vb_paged_b
     a.window = window;
     a.few_rows = pl.few_rows;
     a.row_tiles = pl.row_tiles;
+    a.stream = pl.stream;
     a.few = pl.few;
     a.many = pl.many;
-    a.part = static_cast<float*>(workspace);
+    float* w = static_cast<float*>(workspace);
+    if (pl.row_tiles == 1) {
+        const size_t parts = (size_t)148 * 2 * 2 * pl.few.rows;
+        a.strm = w;
+        a.strm_ml = reinterpret_cast<float2*>(w + parts * D);
+        w += parts * (D + 2);
+    }
+    a.part = w;
     a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)pl.max_splits * a.p.tokens * heads * D);
     return D == 128 ? launch_attn<128>(a, io, cache->dtype, as_stream(stream))
                     : launch_attn<64>(a, io, cache->dtype, as_stream(stream));
