@@ -110,18 +110,20 @@ __device__ __forceinline__ KeyRange key_range(const AttnView& a, const PagedSeq&
 constexpr int kUnit = 64;
 __device__ __forceinline__ int stream_units(const AttnView& a, int b) {
     const int start = a.p.q_start[b], end = a.p.q_start[b + 1];
-    const int64_t rows = (int64_t)(end - start) * a.group;
-    if (start < 0 || end <= start || end > a.p.tokens || end - start > a.p.max_new || rows > a.few_rows) return 0;
     PagedSeq s;
-    s.n = end - start;
     s.len = a.p.lens[b];
+    s.n = end - start;
     if (s.len < 0 || s.len > a.p.max_len) s.len = 0;
     const KeyRange k = key_range(a, s, 0, a.few);
-    return max(1, (k.hi - k.base + kUnit - 1) / kUnit);
+    const bool ok = start >= 0 && end > start && end <= a.p.tokens && s.n <= a.p.max_new &&
+                    (int64_t)s.n * a.group <= a.few_rows;
+    return ok ? max(1, (k.hi - k.base + kUnit - 1) / kUnit) : 0;
 }
-// Units of all sequences, and of those before sequence b, of one KV head; by the whole warp.
-__device__ __forceinline__ void stream_sums(const AttnView& a, int b, int lane, int64_t& all, int64_t& before) {
-    int64_t x = 0, y = 0;
+// Units of all sequences, and of those before sequence b; by the whole warp.  (The host
+// sees to it that they fit 32 bits.)
+__device__ __forceinline__ void stream_sums(const AttnView& a, int b, int lane, int& all, int& before) {
+    int x = 0, y = 0;
+#pragma unroll 2
     for (int i = lane; i < a.p.batch; i += 32) {
         const int u = stream_units(a, i);
         x += u;
@@ -249,8 +251,10 @@ struct FewCfg {
     static constexpr int kRows = 8 * NR;
     static constexpr int kRowBytes = D * (int)sizeof(KV);
     static constexpr int kBlockBytes = kBK * kRowBytes;  // K or V of a block
-    // 96 KB in flight per CTA and two CTAs on an SM, or (f32, D = 128) 192 KB and one
-    static constexpr int kStages = kRowBytes == 128 ? 6 : 3;
+    // 64 KB of ring per CTA and three CTAs on an SM, or (f32, D = 128) 128 KB and one.  (A third
+    // stage and two CTAs moved less: a piece's end and the next one's start leave a CTA without
+    // loads in flight, and more of the others' fill in.)
+    static constexpr int kStages = kRowBytes == 128 ? 4 : 2;
     static constexpr int kWarpBytes = kStages * 2 * kBlockBytes;
     static constexpr int kLd = D + 4;  // row of the warps' sums, floats
     static constexpr int kMerge = kFewWarps * kRows * kLd * 4;
@@ -621,21 +625,25 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
     } else {
         // this block's units, piece by piece: a piece is what it has of one tile
         const int lane = threadIdx.x & 31;
-        int64_t all, dummy;
-        stream_sums(a, 0, lane, all, dummy);
-        const int64_t blocks = min((int64_t)a.stream, all);  // no block between others is empty
-        if (blockIdx.x >= blocks) return;
-        int64_t u = all * blockIdx.x / blocks;
-        const int64_t u_end = all * (blockIdx.x + 1) / blocks;
+        if (a.p.status && blockIdx.x == 0)  // the sequences that get no units are reported too
+            for (int i = threadIdx.x; i < a.p.batch; i += kFewWarps * 32) paged_seq(a.p, i);
+        int all, unused;
+        stream_sums(a, 0, lane, all, unused);
+        const int blocks = min(a.stream, all);  // no block between others is empty
+        const int c = (int)blockIdx.x;
+        if (c >= blocks) return;
+        // c * all / blocks in 32 bits
+        const int per = all / blocks, more = all % blocks;
+        int u = per * c + more * c / blocks;
+        const int u_end = per * (c + 1) + more * (c + 1) / blocks;
         // the sequence of unit u: 32 sequences a step
-        int b = 0;
-        int64_t off = u;  // u's number within sequence b
+        int b = 0, off = u;  // u's number within sequence b
         for (int b0 = 0; b0 < a.p.batch; b0 += 32) {
-            const int64_t mine = b0 + lane < a.p.batch ? (int64_t)stream_units(a, b0 + lane) * a.p.kv_heads : 0;
-            int64_t sum = mine;
-    #pragma unroll
+            const int mine = b0 + lane < a.p.batch ? stream_units(a, b0 + lane) * a.p.kv_heads : 0;
+            int sum = mine;
+#pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int64_t x = __shfl_up_sync(0xffffffffu, sum, o);
+                const int x = __shfl_up_sync(0xffffffffu, sum, o);
                 if (lane >= o) sum += x;
             }
             const unsigned past = __ballot_sync(0xffffffffu, sum > off);
@@ -649,15 +657,14 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
         }
         while (u < u_end) {
             const int n = stream_units(a, b);  // units of a tile
-            if (n == 0 || off >= (int64_t)n * a.p.kv_heads) {
-                off -= (int64_t)n * a.p.kv_heads;
+            if (n == 0 || off >= n * a.p.kv_heads) {
+                off -= n * a.p.kv_heads;
                 if (++b >= a.p.batch) return;  // (the lengths changed under the kernel)
                 continue;
             }
             const PagedSeq s = paged_seq(a.p, b);
             const KeyRange kr = key_range(a, s, 0, a.few);
-            const int kvh = (int)(off / n), first = (int)(off % n);
-            const int take = (int)min((int64_t)(n - first), u_end - u);
+            const int kvh = off / n, first = off % n, take = min(n - first, u_end - u);
             const int slot = first > 0 ? 0 : 1;  // a tile begun by an earlier block; begun here
             const Sink sink{take == n, a.strm, a.strm_ml, ((int64_t)blockIdx.x * 2 + slot) * C::kRows, true};
             const int k_begin = kr.base + first * kUnit;
@@ -1250,44 +1257,20 @@ __global__ void __launch_bounds__(128) paged_attn_merge_kernel(const __grid_cons
     const PagedSeq s = paged_seq(a.p, b);
     if (!s.ok || token < s.start || token >= s.start + s.n) return;
     const int r = (token - s.start) * a.group + head % a.group;
-    // part x of the row is at at0 + x * step
-    const bool few = s.n * a.group <= a.few_rows;
-    int used;
-    int64_t at0 = th, step = (int64_t)a.p.tokens * a.heads;
-    const float* part = a.part;
-    const float2* part_ml = a.part_ml;
-    if (few && a.stream) {
-        int64_t all, u0;
-        stream_sums(a, b, lane, all, u0);
-        const int n = stream_units(a, b);
-        u0 += (int64_t)(head / a.group) * n;
-        // the block of unit u: the last c with c W / N <= u, rounded down
-        const int64_t blocks = min((int64_t)a.stream, all);
-        const int64_t c0 = ((u0 + 1) * blocks - 1) / all, c1 = ((u0 + n) * blocks - 1) / all;
-        used = (int)(c1 - c0) + 1;
-        if (used == 1) return;  // written by the kernel itself
-        // slot 1 of block c0, then slot 0 of the next ones
-        part = a.strm;
-        part_ml = a.strm_ml;
-        step = 2 * a.few.rows;
-        at0 = c0 * step + r;
-    } else {
-        const Cut& cut = few ? a.few : a.many;
-        if (cut.splits == 1) return;  // written by the kernel itself
-        used = splits_used(cut, key_range(a, s, r / cut.rows * cut.rows, cut));
-    }
-    const int64_t first = few && a.stream ? a.few.rows : 0;  // part 0 is a slot further
+    const Cut& cut = s.n * a.group > a.few_rows ? a.many : a.few;
+    if (cut.splits == 1) return;  // written by the kernel itself
+    const int used = splits_used(cut, key_range(a, s, r / cut.rows * cut.rows, cut));
+    const int64_t step = (int64_t)a.p.tokens * a.heads;
     constexpr int E = D / 32;
     float y[E] = {}, M = -INFINITY, L = 0.f;
-    for (int x = lane; x < used; x += 32) M = fmaxf(M, part_ml[at0 + x * step + (x == 0 ? first : 0)].x);
+    for (int x = lane; x < used; x += 32) M = fmaxf(M, a.part_ml[x * step + th].x);
     M = warp_max(M);
     const float mb = M == -INFINITY ? 0.f : M;
     for (int x = 0; x < used; x++) {
-        const int64_t at = at0 + x * step + (x == 0 ? first : 0);
-        const float2 p = part_ml[at];
+        const float2 p = a.part_ml[x * step + th];
         const float w = ex2_approx(p.x - mb);
         L = fmaf(p.y, w, L);
-        const float* src = part + at * D + lane * E;
+        const float* src = a.part + (x * step + th) * D + lane * E;
 #pragma unroll
         for (int e = 0; e < E; e++) y[e] = fmaf(w, src[e], y[e]);
     }
@@ -1296,6 +1279,66 @@ __global__ void __launch_bounds__(128) paged_attn_merge_kernel(const __grid_cons
 #pragma unroll
     for (int e = 0; e < E; e++) dst[e] = (IO)(y[e] * inv);
     if (a.lse && lane == 0) a.lse[th] = L > 0.f ? (M + log2f(L)) * 0.693147180559945309f : -INFINITY;
+}
+
+// Joins the pieces of one row of a shared-out tile: grid over (sequence, KV head, tile
+// row), 8 warps take turns at the pieces.
+constexpr int kJoinWarps = 8;
+template <typename IO, int D>
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const __grid_constant__ AttnView a, int tile_rows) {
+    __shared__ float sums[kJoinWarps][D];
+    // (before the wait only what the kernel before, which has waited itself, did not write)
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int r = blockIdx.x % tile_rows, kvh = blockIdx.x / tile_rows % a.p.kv_heads;
+    const int b = blockIdx.x / (tile_rows * a.p.kv_heads);
+    int all, u0;
+    stream_sums(a, b, lane, all, u0);
+    const int n = stream_units(a, b);
+    pdl_wait();
+    pdl_trigger();
+    if (n == 0) return;
+    const PagedSeq s = paged_seq(a.p, b);
+    if (r >= s.n * a.group) return;
+    u0 += kvh * n;
+    // the block of unit u: the last c with c W / N <= u, rounded down
+    const int blocks = min(a.stream, all);
+    const int c0 = (int)(((int64_t)(u0 + 1) * blocks - 1) / all), c1 = (int)(((int64_t)(u0 + n) * blocks - 1) / all);
+    const int used = c1 - c0 + 1;
+    if (used == 1) return;  // written by the kernel itself
+    // slot 1 of block c0, then slot 0 of the next ones
+    auto at = [&](int x) { return ((int64_t)(c0 + x) * 2 + (x == 0)) * a.few.rows + r; };
+    float M = -INFINITY;
+    for (int x = lane; x < used; x += 32) M = fmaxf(M, a.strm_ml[at(x)].x);
+    M = warp_max(M);
+    const float mb = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    for (int x = lane; x < used; x += 32) {
+        const float2 p = a.strm_ml[at(x)];
+        L = fmaf(p.y, ex2_approx(p.x - mb), L);
+    }
+    L = warp_sum(L);
+    constexpr int E = D / 32;
+    float y[E] = {};
+#pragma unroll 4
+    for (int x = warp; x < used; x += kJoinWarps) {
+        const float w = ex2_approx(a.strm_ml[at(x)].x - mb);
+        const float* src = a.strm + at(x) * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; e++) y[e] = fmaf(w, src[e], y[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) sums[warp][lane * E + e] = y[e];
+    __syncthreads();
+    const int token = s.start + r / a.group, head = kvh * a.group + r % a.group;
+    if (threadIdx.x < D) {
+        float z = 0.f;
+#pragma unroll
+        for (int x = 0; x < kJoinWarps; x++) z += sums[x][threadIdx.x];
+        z *= L > 0.f ? 1.f / L : 0.f;
+        reinterpret_cast<IO*>(a.out + token * a.o_row + head * a.o_head)[threadIdx.x] = (IO)z;
+    }
+    if (a.lse && threadIdx.x == 0)
+        a.lse[(int64_t)token * a.heads + head] = L > 0.f ? (M + log2f(L)) * 0.693147180559945309f : -INFINITY;
 }
 
 // How the work is cut up: from the host's bounds alone, so that a captured
@@ -1307,6 +1350,7 @@ struct Plan {
     int max_splits;  // for any window
 };
 constexpr int kFewRows = 32;
+constexpr int kStreamMost = 148 * 3;  // blocks that share out a batch's keys
 
 Cut make_cut(int rows, int align, int64_t keys, int64_t want, int step, int least) {
     Cut c;
@@ -1343,8 +1387,8 @@ Plan make_plan(const PagedView& p, int io, int cache, int heads, int D, int wind
     const int64_t want = pl.row_tiles == 1 ? 1 : std::max<int64_t>(1, 148 * 4 / (tiles * p.kv_heads));
     if (pl.row_tiles == 1) {
         const int64_t most_units = (int64_t)p.batch * p.kv_heads * ((span(tile, 16) + kUnit - 1) / kUnit);
-        const int per_sm = cache == VB_F32 && D == 128 ? 1 : 2;
-        pl.stream = (int)std::min<int64_t>(148 * per_sm, most_units);
+        if (most_units > 0x3fffffff) return pl;  // (the caller refuses)
+        pl.stream = (int)std::min<int64_t>(cache == VB_F32 && D == 128 ? 148 : kStreamMost, most_units);
     }
     pl.few = make_cut(tile, 16, span(tile, 16), want, 64, 64);
     const int64_t tiles2 = std::max<int64_t>(1, (total + kTcRows - 1) / kTcRows);
@@ -1358,7 +1402,7 @@ Plan make_plan(const PagedView& p, int io, int cache, int heads, int D, int wind
 }
 size_t plan_bytes(const Plan& pl, const PagedView& p, int heads, int D) {
     return (pl.max_splits > 1 ? (size_t)pl.max_splits * p.tokens * heads * (D + 2) * 4 : 0) +
-           (pl.row_tiles == 1 ? (size_t)148 * 2 * 2 * pl.few.rows * (D + 2) * 4 : 0);
+           (pl.row_tiles == 1 ? (size_t)kStreamMost * 2 * pl.few.rows * (D + 2) * 4 : 0);
 }
 
 // Tensor map of a pool as [page][kv head][position][dim], boxes of one page's rows (128 at
@@ -1430,7 +1474,14 @@ vb_status launch_attn(const AttnView& a, cudaStream_t s) {
         }
         if (st) return st;
     }
-    if (a.stream > 1 || a.few.splits > 1 || a.many.splits > 1) {
+    if (a.stream > 1) {
+        const int rows = (int)std::min<int64_t>(a.few.rows, (int64_t)a.p.max_new * a.group);
+        const int64_t grid = (int64_t)a.p.batch * a.p.kv_heads * rows;
+        if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
+        e = launch_pdl(paged_attn_join_kernel<IO, D>, dim3((unsigned)grid), dim3(kJoinWarps * 32), 0, s, a, rows);
+        if (e != cudaSuccess) return cuda_fail(e, "paged_attn_join_kernel");
+    }
+    if (a.few.splits > 1 || a.many.splits > 1) {
         const int64_t grid = ((int64_t)a.p.tokens * a.heads + 3) / 4;
         if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
         e = launch_pdl(paged_attn_merge_kernel<IO, D>, dim3((unsigned)grid), dim3(128), 0, s, a);
@@ -1477,6 +1528,7 @@ extern "C" vb_status vb_paged_attn(const vb_paged_cache* cache, const vb_paged_b
     if (!paged_aligned(q, q_row, q_head, es) || !paged_aligned(out, o_row, o_head, es) || !paged_aligned(workspace, 0, 0, 1))
         return fail(VB_ERR_UNSUPPORTED, "paged_attn: 16-byte alignment required");
     const Plan pl = make_plan(a.p, io, cache->dtype, heads, D, window);
+    if (pl.row_tiles == 1 && !pl.stream) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many keys");
     const size_t need = plan_bytes(pl, a.p, heads, D);
     if (need > workspace_bytes || (need && !workspace))
         return fail(VB_ERR_ARG, "paged_attn: the workspace is too small");
@@ -1496,7 +1548,7 @@ extern "C" vb_status vb_paged_attn(const vb_paged_cache* cache, const vb_paged_b
     a.many = pl.many;
     float* w = static_cast<float*>(workspace);
     if (pl.row_tiles == 1) {
-        const size_t parts = (size_t)148 * 2 * 2 * pl.few.rows;
+        const size_t parts = (size_t)kStreamMost * 2 * pl.few.rows;
         a.strm = w;
         a.strm_ml = reinterpret_cast<float2*>(w + parts * D);
         w += parts * (D + 2);
