@@ -18,24 +18,24 @@ namespace vb {
 
 vb_status paged_view(const vb_paged_cache* c, const vb_paged_batch* b, int io, int heads, const char* who,
                      PagedView* out) {
-    const std::string w = std::string(who) + ": ";
-    if (!c || !b || !c->k || !c->v) return fail(VB_ERR_ARG, w + "null pointer");
+    const auto refuse = [who](vb_status code, const char* msg) { return fail(code, std::string(who) + ": " + msg); };
+    if (!c || !b || !c->k || !c->v) return refuse(VB_ERR_ARG, "null pointer");
     const int es = paged_elem_bytes(c->dtype);
-    if (!es || !paged_elem_bytes(io)) return fail(VB_ERR_ARG, w + "unknown element type");
+    if (!es || !paged_elem_bytes(io)) return refuse(VB_ERR_ARG, "unknown element type");
     if (io != c->dtype && !(io == VB_F32 && c->dtype == VB_BF16))
-        return fail(VB_ERR_UNSUPPORTED, w + "rows have the cache's type, or f32 with a bf16 cache");
-    if (c->head_dim != 64 && c->head_dim != 128) return fail(VB_ERR_UNSUPPORTED, w + "head_dim must be 64 or 128");
-    if (c->num_pages <= 0 || c->page_size <= 0 || c->kv_heads <= 0) return fail(VB_ERR_ARG, w + "non-positive shape");
-    if (heads <= 0 || heads % c->kv_heads) return fail(VB_ERR_ARG, w + "heads must be a multiple of kv_heads");
-    if (c->stride_page < 0 || c->stride_pos < 0 || c->stride_head < 0) return fail(VB_ERR_ARG, w + "negative stride");
+        return refuse(VB_ERR_UNSUPPORTED, "rows have the cache's type, or f32 with a bf16 cache");
+    if (c->head_dim != 64 && c->head_dim != 128) return refuse(VB_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
+    if (c->num_pages <= 0 || c->page_size <= 0 || c->kv_heads <= 0) return refuse(VB_ERR_ARG, "non-positive shape");
+    if (heads <= 0 || heads % c->kv_heads) return refuse(VB_ERR_ARG, "heads must be a multiple of kv_heads");
+    if (c->stride_page < 0 || c->stride_pos < 0 || c->stride_head < 0) return refuse(VB_ERR_ARG, "negative stride");
     if (!paged_aligned(c->k, c->stride_pos, c->stride_head, es) || !paged_aligned(c->v, c->stride_page, 0, es))
-        return fail(VB_ERR_UNSUPPORTED, w + "16-byte alignment required");
+        return refuse(VB_ERR_UNSUPPORTED, "16-byte alignment required");
     if (b->batch < 0 || b->tokens < 0 || b->max_new < 0 || b->max_len < 0 || b->table_stride < 0)
-        return fail(VB_ERR_ARG, w + "negative size");
+        return refuse(VB_ERR_ARG, "negative size");
     if (b->batch && b->tokens) {
-        if (!b->q_start || !b->lens || (b->max_len && !b->table)) return fail(VB_ERR_ARG, w + "null pointer");
+        if (!b->q_start || !b->lens || (b->max_len && !b->table)) return refuse(VB_ERR_ARG, "null pointer");
         if (b->max_len > (int64_t)b->table_stride * c->page_size)
-            return fail(VB_ERR_ARG, w + "max_len is more than the table's pages hold");
+            return refuse(VB_ERR_ARG, "max_len is more than the table's pages hold");
     }
     PagedView& p = *out;
     p.k = static_cast<const char*>(c->k);
@@ -43,9 +43,7 @@ vb_status paged_view(const vb_paged_cache* c, const vb_paged_batch* b, int io, i
     p.num_pages = c->num_pages;
     p.page_size = c->page_size;
     p.kv_heads = c->kv_heads;
-    p.page_shift = -1;
-    for (int i = 0; i < 31; i++)
-        if (c->page_size == 1 << i) p.page_shift = i;
+    p.page_shift = (c->page_size & (c->page_size - 1)) == 0 ? __builtin_ctz((unsigned)c->page_size) : -1;
     p.stride_page = c->stride_page * es;
     p.stride_pos = c->stride_pos * es;
     p.stride_head = c->stride_head * es;
@@ -80,6 +78,7 @@ struct AttnView {
     int window;
     int few_rows;       // sequences with at most this many rows a KV head run in the few-rows kernel
     int row_tiles;      // its row tiles of a sequence
+    bool cluster;       // a cluster of blocks for each tile (one row tile a sequence, few and short)
     int stream;         // blocks that share all its keys evenly (one row tile a sequence); 0: a block per tile and split
     Cut few, many;
     int box;            // rows of a page that one TMA copy brings (many rows); 0: no tensor maps
@@ -282,13 +281,14 @@ struct Sink {
     float2* ml;
     int64_t base;    // row_of: split * tokens * heads + token * heads + head, or (by_row) the tile's row
     bool by_row;
+    bool keep;       // neither: the sums stay in shared memory, row `row` at row * (D + 4), its (m, l) in kept
 };
 
 // Rows r0 .. of KV head kvh of sequence b over keys k_begin .. k_end - 1, by the block.
 template <typename IO, typename KV, int D, int NR>
 __device__ __forceinline__ void few_piece(const AttnView& a, const PagedSeq& s, int b, int kvh, int r0, const KeyRange& kr,
                                           int k_begin, int k_end, const Sink& sink, char* smem,
-                                          float2 (*ml)[8 * NR]) {
+                                          float2 (*ml)[8 * NR], float2* kept = nullptr) {
     using C = FewCfg<KV, D, NR>;
     constexpr bool kF32 = sizeof(KV) == 4;
     constexpr bool kExact = sizeof(IO) == 4;
@@ -584,7 +584,10 @@ __device__ __forceinline__ void few_piece(const AttnView& a, const PagedSeq& s, 
         }
         const int token = s.start + r / a.group, head = kvh * a.group + r % a.group;
         const int64_t th = (int64_t)token * a.heads + head;
-        if (sink.last) {
+        if (sink.keep) {
+            Eight<float>::store(sums + row * C::kLd + d, y);  // (over what this thread alone has read)
+            if (d == 0) kept[row] = make_float2(M, L);
+        } else if (sink.last) {
             const float inv = L > 0.f ? 1.f / L : 0.f;
 #pragma unroll
             for (int e = 0; e < 8; e++) y[e] *= inv;
@@ -598,16 +601,69 @@ __device__ __forceinline__ void few_piece(const AttnView& a, const PagedSeq& s, 
     }
 }
 
-// STREAM: the keys of all tiles shared out evenly; else a grid of (split, KV head, row tile,
-// sequence) in one axis.
-template <typename IO, typename KV, int D, int NR, bool STREAM>
+__device__ __forceinline__ float4 cl_ld4(unsigned addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
+// How the kernel's blocks share the work: a grid of (split, KV head, row tile, sequence) in
+// one axis; the keys of all tiles shared out evenly; or a cluster of 8 blocks for a tile,
+// which join their pieces through each other's shared memory (no second launch).
+enum FewMode { kGrid, kStream, kCluster };
+constexpr int kCl = 8;
+
+template <typename IO, typename KV, int D, int NR, int MODE>
 __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __grid_constant__ AttnView a) {
     using C = FewCfg<KV, D, NR>;
     extern __shared__ __align__(1024) char smem[];
     __shared__ float2 ml[kFewWarps][C::kRows];
     pdl_wait();
     pdl_trigger();
-    if constexpr (!STREAM) {
+    if constexpr (MODE == kCluster) {
+        __shared__ float2 kept[C::kRows];
+        const int rank = (int)cl_rank(), tile = (int)blockIdx.x / kCl;
+        const int kvh = tile % a.p.kv_heads, b = tile / a.p.kv_heads;
+        const PagedSeq s = paged_seq(a.p, b);
+        const int rows = s.n * a.group;
+        if (rows == 0 || rows > a.few_rows) return;  // (the whole cluster)
+        const KeyRange kr = key_range(a, s, 0, a.few);
+        const int n = (kr.hi - kr.base + kBK - 1) / kBK;  // blocks of 16 keys
+        const int k_begin = kr.base + n * rank / kCl * kBK, k_end = min(kr.base + n * (rank + 1) / kCl * kBK, kr.hi);
+        const Sink sink{false, nullptr, nullptr, 0, false, true};
+        few_piece<IO, KV, D, NR>(a, s, b, kvh, 0, kr, k_begin, k_end, sink, smem, ml, kept);
+        cluster_sync_all();
+        for (int it = rank * kFewWarps * 32 + threadIdx.x; it < C::kRows * (D / 4); it += kCl * kFewWarps * 32) {
+            const int row = it / (D / 4), d = it % (D / 4) * 4;
+            if (row >= rows) break;
+            float2 q[kCl];
+            float M = -INFINITY, L = 0.f;
+#pragma unroll
+            for (int c = 0; c < kCl; c++) {
+                const unsigned at = cl_map(smem_addr(&kept[row]), c);
+                q[c] = make_float2(cl_ld(at), cl_ld(at + 4));
+                M = fmaxf(M, q[c].x);
+            }
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < kCl; c++) {
+                const float w = ex2_approx(q[c].x - (M == -INFINITY ? 0.f : M));
+                const float4 z = cl_ld4(cl_map(smem_addr(smem) + (row * C::kLd + d) * 4, c));
+                L = fmaf(q[c].y, w, L);
+                y.x = fmaf(w, z.x, y.x), y.y = fmaf(w, z.y, y.y), y.z = fmaf(w, z.z, y.z), y.w = fmaf(w, z.w, y.w);
+            }
+            const float inv = L > 0.f ? 1.f / L : 0.f;
+            const int token = s.start + row / a.group, head = kvh * a.group + row % a.group;
+            IO* dst = reinterpret_cast<IO*>(a.out + token * a.o_row + head * a.o_head) + d;
+            dst[0] = (IO)(y.x * inv), dst[1] = (IO)(y.y * inv), dst[2] = (IO)(y.z * inv), dst[3] = (IO)(y.w * inv);
+            if (d == 0 && a.lse)
+                a.lse[(int64_t)token * a.heads + head] = L > 0.f ? (M + log2f(L)) * 0.693147180559945309f : -INFINITY;
+        }
+        cluster_sync_all();  // no block leaves while others read its shared memory
+    } else if constexpr (MODE == kGrid) {
         int64_t idx = blockIdx.x;
         const int split = (int)(idx % a.few.splits);
         idx /= a.few.splits;
@@ -620,7 +676,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
         const KeyRange kr = key_range(a, s, r0, a.few);
         if (split >= splits_used(a.few, kr)) return;
         const int k_begin = kr.base + split * a.few.len;
-        const Sink sink{a.few.splits == 1, a.part, a.part_ml, (int64_t)split * a.p.tokens * a.heads, false};
+        const Sink sink{a.few.splits == 1, a.part, a.part_ml, (int64_t)split * a.p.tokens * a.heads, false, false};
         few_piece<IO, KV, D, NR>(a, s, b, kvh, r0, kr, k_begin, min(k_begin + a.few.len, kr.hi), sink, smem, ml);
     } else {
         // this block's units, piece by piece: a piece is what it has of one tile
@@ -666,7 +722,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
             const KeyRange kr = key_range(a, s, 0, a.few);
             const int kvh = off / n, first = off % n, take = min(n - first, u_end - u);
             const int slot = first > 0 ? 0 : 1;  // a tile begun by an earlier block; begun here
-            const Sink sink{take == n, a.strm, a.strm_ml, ((int64_t)blockIdx.x * 2 + slot) * C::kRows, true};
+            const Sink sink{take == n, a.strm, a.strm_ml, ((int64_t)blockIdx.x * 2 + slot) * C::kRows, true, false};
             const int k_begin = kr.base + first * kUnit;
             few_piece<IO, KV, D, NR>(a, s, b, kvh, 0, kr, k_begin, min(k_begin + take * kUnit, kr.hi), sink, smem, ml);
             u += take;
@@ -1346,6 +1402,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const 
 // tiles alone do not fill the card.
 struct Plan {
     int few_rows, row_tiles, stream;
+    bool cluster;
     Cut few, many;
     int max_splits;  // for any window
 };
@@ -1388,6 +1445,9 @@ Plan make_plan(const PagedView& p, int io, int cache, int heads, int D, int wind
     if (pl.row_tiles == 1) {
         const int64_t most_units = (int64_t)p.batch * p.kv_heads * ((span(tile, 16) + kUnit - 1) / kUnit);
         if (most_units > 0x3fffffff) return pl;  // (the caller refuses)
+        // Clusters where all fit the card at once and a block's share is at most 512 keys: one token
+        // of one sequence of 777 keys takes one launch and CLUSTER_US instead of two and STREAM_US.
+        pl.cluster = (int64_t)p.batch * p.kv_heads * kCl <= 148 * 2 && span(tile, 16) <= kCl * 512;
         pl.stream = (int)std::min<int64_t>(cache == VB_F32 && D == 128 ? 148 : kStreamMost, most_units);
     }
     pl.few = make_cut(tile, 16, span(tile, 16), want, 64, 64);
@@ -1424,21 +1484,28 @@ int page_map(const PagedView& p, const char* base, int D, bool half, CUtensorMap
     return r == CUDA_SUCCESS ? box : 0;
 }
 
-template <typename IO, typename KV, int D, int NR, bool STREAM>
+template <typename IO, typename KV, int D, int NR, int MODE>
 vb_status launch_few(const AttnView& a, cudaStream_t s) {
     using C = FewCfg<KV, D, NR>;
     static std::atomic<unsigned long long> done{0};
-    cudaError_t e = smem_attr_once(paged_attn_few_kernel<IO, KV, D, NR, STREAM>, C::kSmem, done);
+    cudaError_t e = smem_attr_once(paged_attn_few_kernel<IO, KV, D, NR, MODE>, C::kSmem, done);
     if (e != cudaSuccess) return cuda_fail(e, "paged attention: shared memory attribute");
-    const int64_t grid = STREAM ? a.stream : (int64_t)a.few.splits * a.p.kv_heads * a.row_tiles * a.p.batch;
+    if (MODE == kCluster) {
+        const int64_t blocks = (int64_t)a.p.batch * a.p.kv_heads * kCl;
+        e = launch_pdl_cluster(paged_attn_few_kernel<IO, KV, D, NR, MODE>, dim3((unsigned)blocks), dim3(kFewWarps * 32),
+                               C::kSmem, dim3(kCl, 1, 1), s, a);
+        return e == cudaSuccess ? VB_OK : cuda_fail(e, "paged_attn_few_kernel");
+    }
+    const int64_t grid = MODE == kStream ? a.stream : (int64_t)a.few.splits * a.p.kv_heads * a.row_tiles * a.p.batch;
     if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
-    e = launch_pdl(paged_attn_few_kernel<IO, KV, D, NR, STREAM>, dim3((unsigned)grid), dim3(kFewWarps * 32), C::kSmem, s, a);
+    e = launch_pdl(paged_attn_few_kernel<IO, KV, D, NR, MODE>, dim3((unsigned)grid), dim3(kFewWarps * 32), C::kSmem, s, a);
     return e == cudaSuccess ? VB_OK : cuda_fail(e, "paged_attn_few_kernel");
 }
 
 template <typename IO, typename KV, int D, int NR>
 vb_status launch_few(const AttnView& a, cudaStream_t s) {
-    return a.stream ? launch_few<IO, KV, D, NR, true>(a, s) : launch_few<IO, KV, D, NR, false>(a, s);
+    if (a.cluster) return launch_few<IO, KV, D, NR, kCluster>(a, s);
+    return a.stream ? launch_few<IO, KV, D, NR, kStream>(a, s) : launch_few<IO, KV, D, NR, kGrid>(a, s);
 }
 
 template <typename IO, typename KV, int D>
@@ -1543,7 +1610,8 @@ extern "C" vb_status vb_paged_attn(const vb_paged_cache* cache, const vb_paged_b
     a.window = window;
     a.few_rows = pl.few_rows;
     a.row_tiles = pl.row_tiles;
-    a.stream = pl.stream;
+    a.cluster = pl.cluster;
+    a.stream = pl.cluster ? 0 : pl.stream;
     a.few = pl.few;
     a.many = pl.many;
     float* w = static_cast<float*>(workspace);

@@ -577,16 +577,16 @@ def argmax_rows(logits, out_idx, stream=None):
 # -- paged serving and logits rules on torch CUDA tensors ----------------------
 
 PAGED_BAD_ROWS, PAGED_BAD_LEN, PAGED_BAD_PAGE, PAGED_TIMEOUT = 1, 2, 4, 8  # bits of a PagedBatch's status word
-# torch dtype -> VB_F32, VB_F16, VB_BF16 (_I32 for int32); filled when torch is there
-_TYPE = {}
-_I32 = 100
+# torch and its dtypes -> VB_F32, VB_F16, VB_BF16 (_I32 for int32), once there is a handle
+_T, _TYPE, _I32 = None, {}, 100
 
 
-def _types():
-    if not _TYPE:
+def _load_torch():
+    global _T
+    if _T is None:
         import torch
         _TYPE.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int32: _I32})
-    return _TYPE
+        _T = torch
 
 
 def _refuse(msg):
@@ -594,7 +594,7 @@ def _refuse(msg):
 
 
 def _dtype(t, what):
-    d = _types().get(t.dtype, _I32)
+    d = _TYPE.get(t.dtype, _I32)
     if d == _I32:
         _refuse(f"{what}: float32, float16 or bfloat16, not {t.dtype}")
     return d
@@ -602,8 +602,7 @@ def _dtype(t, what):
 
 def _here(index):
     """Memory of these calls lies on the current device: their kernels run there."""
-    import torch
-    if index < 0 or index != torch.cuda.current_device():
+    if index < 0 or index != _T.cuda.current_device():
         _refuse("tensors of the current CUDA device are needed")
 
 
@@ -611,16 +610,13 @@ def _array(t, dtype, index, what, ndim=1):
     """A contiguous array of type `dtype` on device `index`, or None; its address or None."""
     if t is None:
         return None
-    if _types().get(t.dtype) != dtype or t.get_device() != index or t.dim() != ndim or not t.is_contiguous():
+    if _TYPE.get(t.dtype) != dtype or t.get_device() != index or t.dim() != ndim or not t.is_contiguous():
         _refuse(f"{what}: a contiguous {ndim}-d {'int32' if dtype == _I32 else 'float32'} tensor on the same device is needed")
     return t.data_ptr()
 
 
 def _raw_stream(stream, index):
-    if stream is not None:
-        return int(stream)
-    import torch
-    return torch._C._cuda_getCurrentRawStream(index)
+    return _T._C._cuda_getCurrentRawStream(index) if stream is None else int(stream)
 
 
 class PagedCache:
@@ -628,6 +624,7 @@ class PagedCache:
     any order in memory (k.transpose(1, 2) of a [page, head, position, dim] tensor is one)."""
 
     def __init__(self, k, v):
+        _load_torch()
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or k.stride() != v.stride():
             _refuse("paged cache: k and v are 4-d and alike in shape, strides, type and device")
         if k.stride(3) != 1:
@@ -647,12 +644,13 @@ class PagedBatch:
     optional int32 status word.  The tensors may change between calls; the bounds hold."""
 
     def __init__(self, q_start, lens, table, *, max_new, max_len, tokens, status=None):
+        _load_torch()
         dev = self.index = lens.get_device()
         _here(dev)
         B = lens.shape[0] if lens.dim() == 1 else -1
         if q_start.shape != (B + 1,) or table.dim() != 2 or table.shape[0] != B or (B and table.stride(1) != 1):
             _refuse("paged batch: q_start [B + 1], lens [B] and table [B, pages] (contiguous rows)")
-        if _types().get(table.dtype) != _I32 or table.get_device() != dev or (status is not None and status.numel() != 1):
+        if _TYPE.get(table.dtype) != _I32 or table.get_device() != dev or (status is not None and status.numel() != 1):
             _refuse("paged batch: table is int32 beside lens, status one int32")
         ps = None if status is None else _array(status.reshape(1), _I32, dev, "status")
         self.q_start, self.lens, self.table, self.status = q_start, lens, table, status
@@ -674,11 +672,10 @@ def _paged_pair(cache, batch):
     _here(cache.index)
 
 
-def _paged_rows(t, cache, batch, heads, dtype, what):
+def _paged_rows(t, shape, dtype, index, what):
     """Rows [tokens, heads, head_dim] of type `dtype`: their address, row and head stride."""
     st = t.stride()
-    if (len(st) != 3 or st[2] != 1 or t.shape != (batch.tokens, heads, cache.head_dim) or t.dtype != dtype
-            or t.get_device() != cache.index):
+    if t.shape != shape or st[2] != 1 or t.dtype is not dtype or t.get_device() != index:
         _refuse(f"{what}: [tokens, heads, head_dim] rows of the batch are needed, "
                 "the head dim contiguous, all of one type, on the cache's device")
     return t.data_ptr(), st[0], st[1]
@@ -689,17 +686,19 @@ def paged_append(cache, batch, k, v, q=None, q_out=None, cos=None, sin=None, int
     """Appends the batch's new keys (normed by k_norm and rotated by cos / sin [positions, rot] on
     the way) and values to their pages; q normed and rotated the same way goes to q_out."""
     _paged_pair(cache, batch)
-    dev, kvh, dt = cache.index, cache.kv_heads, k.dtype
-    kp = _paged_rows(k, cache, batch, kvh, dt, "k")
-    vp = _paged_rows(v, cache, batch, kvh, dt, "v")
+    dev, dt, D = cache.index, k.dtype, cache.head_dim
+    shape = (batch.tokens, cache.kv_heads, D)
+    kp = _paged_rows(k, shape, dt, dev, "k")
+    vp = _paged_rows(v, shape, dt, dev, "v")
     qp = op = (None, 0, 0)
     heads = 0
     if (q is None) != (q_out is None):
         _refuse("q and q_out come together")
     if q is not None:
         heads = q.shape[1] if q.dim() == 3 else 0
-        qp = _paged_rows(q, cache, batch, heads, dt, "q")
-        op = _paged_rows(q_out, cache, batch, heads, dt, "q_out")
+        shape = (batch.tokens, heads, D)
+        qp = _paged_rows(q, shape, dt, dev, "q")
+        op = _paged_rows(q_out, shape, dt, dev, "q_out")
     if (cos is None) != (sin is None):
         _refuse("cos and sin come together")
     positions = rot = 0
@@ -708,7 +707,7 @@ def paged_append(cache, batch, k, v, q=None, q_out=None, cos=None, sin=None, int
             _refuse("cos and sin are alike: [positions, rot]")
         positions, rot = cos.shape
     for n in (q_norm, k_norm):
-        if n is not None and n.numel() != cache.head_dim:
+        if n is not None and n.numel() != D:
             _refuse("q_norm / k_norm: [head_dim]")
     rope = VBPagedRope(_array(cos, 0, dev, "cos", 2), _array(sin, 0, dev, "sin", 2), positions, rot,
                        1 if interleaved else 0, _array(q_norm, 0, dev, "q_norm"), _array(k_norm, 0, dev, "k_norm"), eps)
@@ -735,8 +734,9 @@ def paged_attn(cache, batch, q, out, lse=None, scale=None, window=0, workspace=N
     paged_attn_workspace (one is made for the call when None)."""
     _paged_pair(cache, batch)
     dev, heads = cache.index, q.shape[1] if q.dim() == 3 else 0
-    qp = _paged_rows(q, cache, batch, heads, q.dtype, "q")
-    op = _paged_rows(out, cache, batch, heads, q.dtype, "out")
+    shape = (batch.tokens, heads, cache.head_dim)
+    qp = _paged_rows(q, shape, q.dtype, dev, "q")
+    op = _paged_rows(out, shape, q.dtype, dev, "out")
     if lse is not None and lse.shape != (batch.tokens, heads):
         _refuse("lse: f32 [tokens, heads]")
     if workspace is None:
@@ -756,6 +756,7 @@ class LogitsRules:
 
     def __init__(self, hist_start=None, hist_ids=None, prompt_len=None, repetition=None, frequency=None,
                  presence=None, bias_start=None, bias_ids=None, bias_vals=None, mask=None):
+        _load_torch()
         given = [t for t in (hist_start, prompt_len, repetition, frequency, presence, bias_start, mask)
                  if t is not None]
         if (hist_start is None) != (hist_ids is None):
@@ -794,7 +795,7 @@ def logits_process(logits, out, rules, stream=None):
     if V > 1 and (st[1] != 1 or so[1] != 1):
         _refuse("logits_process: rows are contiguous")
     _here(dev)
-    if rules.rows not in (None, R) or rules.index not in (None, dev):
+    if (rules.rows != R and rules.rows is not None) or (rules.index != dev and rules.index is not None):
         _refuse("logits_process: the rules are for other rows, or on another device")
     if rules.words is not None and rules.words < (V + 31) // 32:
         _refuse("logits_process: the mask has too few words")
