@@ -285,7 +285,7 @@ typedef struct {
  * values only; q_out may equal q, with the same strides).  io is the type of q,
  * q_out, k and v: the cache's own, or VB_F32 with a VB_BF16 cache.  Strides are in elements, per row
  * and per head.  The rotation is the arithmetic of vb_rope, the norm that of
- * vb_rmsnorm. */
+ * vb_rmsnorm with the sum of squares in f32. */
 VB_API vb_status vb_paged_append(const vb_paged_cache* cache, const vb_paged_batch* batch,
                                  const vb_paged_rope* rope, int io, int heads, const void* q,
                                  int64_t q_row, int64_t q_head, void* q_out, int64_t qo_row,

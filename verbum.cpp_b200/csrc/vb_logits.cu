@@ -40,40 +40,31 @@ __device__ __forceinline__ void lg_range(const int* start, int64_t total, int ro
     hi = min(max(start[row + 1], lo), top);
 }
 
-// The rules of one row, and what the slice's tokens need of them.
+// The rules of one row.
 struct RowRules {
-    const uint32_t *seen;  // by token of the slice: top bit in the prompt, the rest its count behind it
-    const float* bias;
-    const uint32_t* mask;  // the row's words
-    bool count, add;
     float rep, freq, pres;
     bool has_rep;
 };
-__device__ __forceinline__ float lg_apply(const RowRules& w, float x, int i, int64_t tok) {
-    if (w.count) {
-        const uint32_t c = w.seen[i];
-        if (c) {
-            if (w.has_rep) x = x > 0.f ? __fdiv_rn(x, w.rep) : __fmul_rn(x, w.rep);
-            const uint32_t n = c & 0x7fffffffu;
-            if (n) x = __fsub_rn(__fsub_rn(x, __fmul_rn(w.freq, (float)n)), w.pres);
-        }
-    }
-    if (w.add) x = __fadd_rn(x, w.bias[i]);
-    if (w.mask && !((w.mask[tok >> 5] >> (tok & 31)) & 1u)) x = -INFINITY;
+// c: top bit set where the token stands in the prompt, the rest its count behind it
+__device__ __forceinline__ float lg_penalty(const RowRules& w, float x, uint32_t c) {
+    if (w.has_rep) x = x > 0.f ? __fdiv_rn(x, w.rep) : __fmul_rn(x, w.rep);
+    const uint32_t n = c & 0x7fffffffu;
+    if (n) x = __fsub_rn(__fsub_rn(x, __fmul_rn(w.freq, (float)n)), w.pres);
     return x;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kLgThreads) logits_process_kernel(const __grid_constant__ LogitsArgs a) {
-    __shared__ uint32_t seen[kLgSlice];
-    __shared__ float bias[kLgSlice];
     constexpr int E = 16 / (int)sizeof(T);  // logits of a 16-byte access
     constexpr int NV = 16 / E;              // accesses of a thread
+    // by token of the slice, moved so that an access's tokens start at a multiple of 4
+    __shared__ __align__(16) uint32_t seen[kLgSlice + E];
+    __shared__ __align__(16) float bias[kLgSlice + E];
     pdl_wait();
     pdl_trigger();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int row = blockIdx.x / a.slices;
-    const int64_t v0 = (int64_t)(blockIdx.x % a.slices) * kLgSlice;
+    const int v0 = (int)(blockIdx.x % a.slices) * kLgSlice;
     const int n = (int)min((int64_t)kLgSlice, a.vocab - v0);
     const T* in = reinterpret_cast<const T*>(a.in + row * a.stride_in) + v0;
     T* out = reinterpret_cast<T*>(a.out + row * a.stride_out) + v0;
@@ -82,78 +73,130 @@ __global__ void __launch_bounds__(kLgThreads) logits_process_kernel(const __grid
     const bool wide = mis == (reinterpret_cast<uintptr_t>(out) & 15u);
     const int head = wide ? min(n, (int)((16u - mis) & 15u) / (int)sizeof(T)) : n;
     const int vecs = (n - head) / E, tail = head + vecs * E;
+    const int shift = (E - head % E) % E;
     uint4 x[NV];
 #pragma unroll
     for (int k = 0; k < NV; k++)
         if (k * kLgThreads + t < vecs) x[k] = reinterpret_cast<const uint4*>(in + head)[k * kLgThreads + t];
 
-    RowRules w{};
-    w.seen = seen;
-    w.bias = bias;
-    w.mask = a.r.mask ? a.r.mask + row * a.r.mask_stride : nullptr;
+    const uint32_t* mask = a.r.mask ? a.r.mask + row * a.r.mask_stride : nullptr;
     int h0 = 0, h1 = 0, b0 = 0, b1 = 0;
     if (a.r.hist_start) lg_range(a.r.hist_start, a.r.hist_total, row, h0, h1);
     if (a.r.bias_start) lg_range(a.r.bias_start, a.r.bias_total, row, b0, b1);
-    w.count = h1 > h0;
-    w.add = b1 > b0;
-    if (w.count) {
+    const bool count = h1 > h0, add = b1 > b0;
+    // the first of the history, too, before the shared memory is ready for it
+    constexpr int NH = 4;
+    int id[NH];
+#pragma unroll
+    for (int k = 0; k < NH; k++) {
+        const int i = h0 + k * kLgThreads + t;
+        id[k] = i < h1 ? a.r.hist_ids[i] : -1;
+    }
+    RowRules w{1.f, 0.f, 0.f, false};
+    if (count) {
         w.has_rep = a.r.repetition != nullptr;
         w.rep = w.has_rep ? a.r.repetition[row] : 1.f;
         w.freq = a.r.frequency ? a.r.frequency[row] : 0.f;
         w.pres = a.r.presence ? a.r.presence[row] : 0.f;
-        for (int i = t; i < kLgSlice; i += kLgThreads) seen[i] = 0u;
+        for (int i = t; i < (kLgSlice + E) / 4; i += kLgThreads) reinterpret_cast<uint4*>(seen)[i] = make_uint4(0, 0, 0, 0);
     }
-    if (w.add)
-        for (int i = t; i < kLgSlice; i += kLgThreads) bias[i] = 0.f;
+    if (add)
+        for (int i = t; i < (kLgSlice + E) / 4; i += kLgThreads)
+            reinterpret_cast<float4*>(bias)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     __syncthreads();
-    if (w.count) {
+    if (count) {
         const int answer = h0 + (a.r.prompt_len ? max(a.r.prompt_len[row], 0) : 0);
-        for (int i = h0 + t; i < h1; i += kLgThreads) {
-            const int64_t at = (int64_t)a.r.hist_ids[i] - v0;
-            if (at >= 0 && at < n) {
-                if (i < answer)
-                    atomicOr(&seen[at], 0x80000000u);
-                else
-                    atomicAdd(&seen[at], 1u);
+        for (int i0 = h0; i0 < h1; i0 += NH * kLgThreads) {
+            int next[NH];
+#pragma unroll
+            for (int k = 0; k < NH; k++) {
+                const int i = i0 + (NH + k) * kLgThreads + t;
+                next[k] = i < h1 ? a.r.hist_ids[i] : -1;
+            }
+#pragma unroll
+            for (int k = 0; k < NH; k++) {
+                const unsigned at = (unsigned)id[k] - (unsigned)v0;  // (an id of -1 is at no slice)
+                if (id[k] >= 0 && at < (unsigned)n) {
+                    if (i0 + k * kLgThreads + t < answer)
+                        atomicOr(&seen[at + shift], 0x80000000u);
+                    else
+                        atomicAdd(&seen[at + shift], 1u);
+                }
+                id[k] = next[k];
             }
         }
     }
-    if (w.add) {
+    if (add) {
         // warp w sums the tokens whose number in the slice is w mod 8
         for (int i0 = b0; i0 < b1; i0 += 32) {
             const int i = i0 + lane;
-            const int64_t at = i < b1 ? (int64_t)a.r.bias_ids[i] - v0 : -1;
-            const bool mine = at >= 0 && at < n && (int)(at & 7) == warp;
+            const int tok = i < b1 ? a.r.bias_ids[i] : -1;
+            const unsigned at = (unsigned)tok - (unsigned)v0;
+            const bool mine = tok >= 0 && at < (unsigned)n && (int)(at & 7) == warp;
             unsigned left = __ballot_sync(0xffffffffu, mine);
             if (!left) continue;
             const float val = mine ? a.r.bias_vals[i] : 0.f;
             const unsigned same = __match_any_sync(0xffffffffu, mine ? (int)at : -1 - lane);
             while (left) {  // the first entry of each token that is left, until none is
                 const bool turn = ((left >> lane) & 1u) && !(same & left & ((1u << lane) - 1u));
-                if (turn) bias[at] = __fadd_rn(bias[at], val);
+                if (turn) bias[at + shift] = __fadd_rn(bias[at + shift], val);
                 __syncwarp();
                 left &= ~__ballot_sync(0xffffffffu, turn);
             }
         }
     }
     __syncthreads();
-    for (int i = t; i < head; i += kLgThreads) lg_store(out + i, lg_apply(w, lg_load(in + i), i, v0 + i));
+    auto single = [&](int i) {
+        float v = lg_load(in + i);
+        if (count && seen[i + shift]) v = lg_penalty(w, v, seen[i + shift]);
+        if (add) v = __fadd_rn(v, bias[i + shift]);
+        const int tok = v0 + i;
+        if (mask && !((mask[tok >> 5] >> (tok & 31)) & 1u)) v = -INFINITY;
+        lg_store(out + i, v);
+    };
+    for (int i = t; i < head; i += kLgThreads) single(i);
 #pragma unroll
     for (int k = 0; k < NV; k++) {
         const int j = k * kLgThreads + t;
-        if (j < vecs) {
-            const T* e = reinterpret_cast<const T*>(&x[k]);
-            uint4 y;
-            T* f = reinterpret_cast<T*>(&y);
+        if (j >= vecs) break;
+        const int i = head + j * E;
+        float v[E];
 #pragma unroll
-            for (int c = 0; c < E; c++) {
-                const int i = head + j * E + c;
-                lg_store(f + c, lg_apply(w, lg_load(e + c), i, v0 + i));
+        for (int c = 0; c < E; c++) v[c] = lg_load(reinterpret_cast<const T*>(&x[k]) + c);
+        if (count) {
+#pragma unroll
+            for (int q = 0; q < E; q += 4) {
+                const uint4 c = *reinterpret_cast<const uint4*>(&seen[i + shift + q]);
+                if (c.x | c.y | c.z | c.w) {
+                    if (c.x) v[q] = lg_penalty(w, v[q], c.x);
+                    if (c.y) v[q + 1] = lg_penalty(w, v[q + 1], c.y);
+                    if (c.z) v[q + 2] = lg_penalty(w, v[q + 2], c.z);
+                    if (c.w) v[q + 3] = lg_penalty(w, v[q + 3], c.w);
+                }
             }
-            reinterpret_cast<uint4*>(out + head)[j] = y;
         }
+        if (add) {
+#pragma unroll
+            for (int q = 0; q < E; q += 4) {
+                const float4 c = *reinterpret_cast<const float4*>(&bias[i + shift + q]);
+                v[q] = __fadd_rn(v[q], c.x), v[q + 1] = __fadd_rn(v[q + 1], c.y);
+                v[q + 2] = __fadd_rn(v[q + 2], c.z), v[q + 3] = __fadd_rn(v[q + 3], c.w);
+            }
+        }
+        if (mask) {
+            // the access's bits: of one word, or of two
+            const int tok = v0 + i, at = tok & 31;
+            uint32_t bits = mask[tok >> 5] >> at;
+            if (at > 32 - E) bits |= mask[(tok >> 5) + 1] << (32 - at);
+#pragma unroll
+            for (int c = 0; c < E; c++) v[c] = (bits >> c) & 1u ? v[c] : -INFINITY;
+        }
+        uint4 y;
+#pragma unroll
+        for (int c = 0; c < E; c++) lg_store(reinterpret_cast<T*>(&y) + c, v[c]);
+        reinterpret_cast<uint4*>(out + head)[j] = y;
     }
-    for (int i = tail + t; i < n; i += kLgThreads) lg_store(out + i, lg_apply(w, lg_load(in + i), i, v0 + i));
+    for (int i = tail + t; i < n; i += kLgThreads) single(i);
 }
 
 }  // namespace
