@@ -80,6 +80,16 @@ __global__ void __launch_bounds__(kLgThreads) logits_process_kernel(const __grid
         if (k * kLgThreads + t < vecs) x[k] = reinterpret_cast<const uint4*>(in + head)[k * kLgThreads + t];
 
     const uint32_t* mask = a.r.mask ? a.r.mask + row * a.r.mask_stride : nullptr;
+    // the words with the bits of each access's tokens: one, or two (shifted where they are used:
+    // here the shift would wait for them)
+    uint32_t lo[NV], hi[NV];
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        const int j = k * kLgThreads + t, tok = v0 + head + j * E;
+        const bool real = mask && j < vecs;
+        lo[k] = real ? mask[tok >> 5] : 0u;
+        hi[k] = real && (tok & 31) > 32 - E ? mask[(tok >> 5) + 1] : 0u;
+    }
     int h0 = 0, h1 = 0, b0 = 0, b1 = 0;
     if (a.r.hist_start) lg_range(a.r.hist_start, a.r.hist_total, row, h0, h1);
     if (a.r.bias_start) lg_range(a.r.bias_start, a.r.bias_total, row, b0, b1);
@@ -92,6 +102,7 @@ __global__ void __launch_bounds__(kLgThreads) logits_process_kernel(const __grid
         const int i = h0 + k * kLgThreads + t;
         id[k] = i < h1 ? a.r.hist_ids[i] : -1;
     }
+    int tok0 = b0 + lane < b1 ? a.r.bias_ids[b0 + lane] : -1;  // and of the biases
     RowRules w{1.f, 0.f, 0.f, false};
     if (count) {
         w.has_rep = a.r.repetition != nullptr;
@@ -129,8 +140,8 @@ __global__ void __launch_bounds__(kLgThreads) logits_process_kernel(const __grid
     if (add) {
         // warp w sums the tokens whose number in the slice is w mod 8
         for (int i0 = b0; i0 < b1; i0 += 32) {
-            const int i = i0 + lane;
-            const int tok = i < b1 ? a.r.bias_ids[i] : -1;
+            const int i = i0 + lane, tok = tok0;
+            tok0 = i + 32 < b1 ? a.r.bias_ids[i + 32] : -1;
             const unsigned at = (unsigned)tok - (unsigned)v0;
             const bool mine = tok >= 0 && at < (unsigned)n && (int)(at & 7) == warp;
             unsigned left = __ballot_sync(0xffffffffu, mine);
@@ -184,10 +195,7 @@ __global__ void __launch_bounds__(kLgThreads) logits_process_kernel(const __grid
             }
         }
         if (mask) {
-            // the access's bits: of one word, or of two
-            const int tok = v0 + i, at = tok & 31;
-            uint32_t bits = mask[tok >> 5] >> at;
-            if (at > 32 - E) bits |= mask[(tok >> 5) + 1] << (32 - at);
+            const uint32_t bits = __funnelshift_r(lo[k], hi[k], (v0 + i) & 31);
 #pragma unroll
             for (int c = 0; c < E; c++) v[c] = (bits >> c) & 1u ? v[c] : -INFINITY;
         }

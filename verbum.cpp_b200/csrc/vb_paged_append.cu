@@ -41,7 +41,7 @@ struct Raw {
 };
 
 template <typename IO, typename KV, int D>
-__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, 4) paged_append_kernel(const __grid_constant__ AppendArgs a) {
     constexpr int U = D / 16;  // threads of a head row
     pdl_wait();
     pdl_trigger();
