@@ -859,6 +859,11 @@ __device__ __forceinline__ void tmem_ld16(unsigned taddr, float* v) {
         : "r"(taddr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_st8(unsigned taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st16(unsigned taddr, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -914,6 +919,97 @@ __device__ __forceinline__ void find_tile(const AttnView& a, int64_t idx, int ro
     }
 }
 
+// The producers of a block: K and V of key tiles of 128 into a ring of stages, by 96 threads.
+// Key tiles that lie wholly inside the range come by TMA, a box of rows of one page by one
+// thread; at its edges, where places outside must read as zeros (weights of 0 do not silence
+// a NaN), and where pages do not tile 128 keys, by 16-byte cp.async.  Every push is 96
+// arrivals at its stage's barrier.
+template <int D, int STAGES>
+struct KvFeed {
+    static constexpr int kHalf = 128 * 128, kTile = kHalf * (D / 64);
+    static constexpr int RC = D / 8, RPP = kTcProducers / RC;  // 16-byte chunks of a row, rows a pass takes
+    const AttnView& a;
+    const CUtensorMap *mk, *mv;
+    int64_t (*place)[128];
+    volatile int* failed;
+    unsigned ring, full, empty;  // shared addresses: first stage, its two barriers (8 bytes a stage)
+    int b, kvh, lo, k_begin, k_end, n, pt, boxes;
+    int page0, page1, row0, row1;  // of tiles j & 1: page and position of box pt
+    int x = 0;            // pushes so far
+    bool ok = true;
+
+    // chunk c of row r in a tile: half c / 8, swizzled inside its 128 bytes
+    static __device__ __forceinline__ unsigned at(int r, int c) {
+        return (unsigned)((c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+    }
+    __device__ __forceinline__ bool by_tma(int j) const {
+        const int k0 = k_begin + j * 128;
+        return boxes > 0 && k0 >= lo && k0 + 128 <= k_end;
+    }
+    // asks for the pages of tile j (a tile ahead of its first push)
+    __device__ __forceinline__ void look(int j) {
+        if (j >= n || pt >= boxes || !by_tma(j)) return;
+        const int key = k_begin + j * 128 + pt * a.box, pg = key >> a.p.page_shift;
+        int id = a.p.table[(size_t)b * a.p.table_stride + pg];
+        if ((unsigned)id >= (unsigned)a.p.num_pages) {
+            paged_report(a.p, VB_PAGED_BAD_PAGE);
+            id = a.p.num_pages;  // beyond the map: zeros
+        }
+        const int at = key - (pg << a.p.page_shift);
+        if (j & 1)
+            page1 = id, row1 = at;
+        else
+            page0 = id, row0 = at;
+    }
+    // before the first push of tile j: the places of an edge's rows, -1: zeros
+    __device__ __forceinline__ void begin(int j) {
+        if (by_tma(j)) return;
+        asm volatile("bar.sync 1, %0;" ::"n"(kTcProducers) : "memory");  // the readers of the last such tile are done
+        for (int r = pt; r < 128; r += kTcProducers) {
+            const int key = k_begin + j * 128 + r;
+            place[j & 1][r] = key >= lo && key < k_end ? paged_offset(a.p, b, key) : -1;
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(kTcProducers) : "memory");
+    }
+    __device__ __forceinline__ void push(int j, bool v) {
+        const int st = x % STAGES;
+        const unsigned bar = full + 8 * st, dst = ring + st * kTile;
+        if (x >= STAGES) ok = tc_wait(empty + 8 * st, (unsigned)(x / STAGES - 1) & 1u, failed) && ok;
+        x++;
+        if (by_tma(j)) {
+            // all arrivals by one thread, with the bytes that are on their way
+            if (pt == 0) {
+                if (ok) mbar_expect_tx(bar, kTile);
+                mbar_arrive(bar, ok ? kTcProducers - 1 : kTcProducers);
+            }
+            if (pt < boxes && ok) {
+#pragma unroll
+                for (int h = 0; h < D / 64; h++)
+                    tma_load_4d(dst + h * kHalf + pt * a.box * 128, v ? mv : mk, 64 * h, j & 1 ? row1 : row0, kvh,
+                                j & 1 ? page1 : page0, bar);
+            }
+        } else {
+            const int pr = pt / RC, pc = pt % RC;
+            const char* src = (v ? a.p.v : a.p.k) + (int64_t)kvh * a.p.stride_head + pc * 16;
+            if (ok) {
+#pragma unroll 4
+                for (int r = pr; r < 128; r += RPP) {
+                    const int64_t o = place[j & 1][r];
+                    cp_async16(dst + at(r, pc), o < 0 ? a.p.k : src + o, o >= 0);
+                }
+            }
+            cp_async_arrive(bar);
+        }
+    }
+    // nothing in flight when the block ends: the products waited for every TMA copy, unless a wait gave up
+    __device__ __forceinline__ void end() {
+        if (*failed)
+            for (int i = max(0, x - STAGES); i < x; i++) tc_wait(full + 8 * (i % STAGES), (unsigned)(i / STAGES) & 1u, nullptr);
+        cp_async_commit();
+        cp_async_wait<0>();
+    }
+};
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __grid_constant__ AttnView a,
                                                                       const __grid_constant__ CUtensorMap mk,
@@ -930,7 +1026,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         p_full[2], o_full[2];
     __shared__ unsigned tmem_slot;
     __shared__ int failed;
-    __shared__ int64_t place[128];
+    __shared__ int64_t place[2][128];
     __shared__ float xch[2][2][128];
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31, wg = t >> 7;
     pdl_wait();
@@ -1199,103 +1295,338 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         } else {
             // ------------------------------------------------- producers
             const int pt = t - (kTcThreads - kTcProducers);
-            constexpr int RC = D / 8, RPP = kTcProducers / RC;  // 16-byte chunks of a row, rows a pass takes
-            const int pr = pt / RC, pc = pt % RC;
-            // chunk c of row r in a tile: half c / 8, swizzled inside its 128 bytes
-            const unsigned col = (unsigned)(pc >> 3) * C::kHalf;
-            auto at = [&](int r) { return (unsigned)(r * 128 + (((pc & 7) ^ (r & 7)) << 4)) + col; };
+            using Feed = KvFeed<D, kTcStages>;
+            const int pr = pt / Feed::RC, pc = pt % Feed::RC;
             for (int i = 0; i < 2; i++) {
                 if (nt[i] == 0) continue;
-                for (int r = pr; r < 128; r += RPP) {
+                for (int r = pr; r < 128; r += Feed::RPP) {
                     const int row = r0 + 128 * i + r;
                     const bool real = row < rows;
                     const int x = real ? row : 0;
-                    cp_async16(sb + i * C::kTile + at(r),
+                    cp_async16(sb + i * C::kTile + Feed::at(r, pc),
                                a.q + (int64_t)(s.start + x / a.group) * a.q_row +
                                    (int64_t)(kvh * a.group + x % a.group) * a.q_head + pc * 16,
                                real);
                 }
             }
             cp_async_arrive(smem_addr(&q_full));
-            // Key tiles that lie wholly inside the range come by TMA, a box of rows of one page
-            // by one thread; at its edges, where places outside must read as zeros (weights of
-            // 0 do not silence a NaN), and where pages do not tile 128 keys, by cp.async.
-            const int boxes = a.box ? 128 / a.box : 0;
-            auto by_tma = [&](int j) {
-                const int k0 = k_begin + j * 128;
-                return boxes > 0 && k0 >= kr.lo && k0 + 128 <= k_end;
-            };
-            // page and position of box pt of a tile that comes by TMA
-            int page = 0, row = 0;
-            auto look_up = [&](int j) {
-                if (j >= nmax || pt >= boxes || !by_tma(j)) return;
-                const int key = k_begin + j * 128 + pt * a.box, pg = key >> a.p.page_shift;
-                page = a.p.table[(size_t)b * a.p.table_stride + pg];
-                row = key - (pg << a.p.page_shift);
-                if ((unsigned)page >= (unsigned)a.p.num_pages) {
-                    paged_report(a.p, VB_PAGED_BAD_PAGE);
-                    page = a.p.num_pages;  // beyond the map: zeros
-                }
-            };
-            const int64_t head_off = (int64_t)kvh * a.p.stride_head + pc * 16;
-            look_up(0);
-            bool ok = true;
-            int push = 0;
+            Feed feed{a, &mk, &mv, place, &failed, sb + C::kOffKV, smem_addr(kv_full), smem_addr(kv_empty),
+                      b, kvh, kr.lo, k_begin, k_end, nmax, pt, a.box ? 128 / a.box : 0};
+            feed.look(0);
             for (int j = 0; j < nmax; j++) {
-                const int pg = page, py = row;
-                const bool tma = by_tma(j);
-                look_up(j + 1);
-                if (!tma) {
-                    // byte offset of every key's row, -1: zeros
-                    asm volatile("bar.sync 1, %0;" ::"n"(kTcProducers) : "memory");  // the last such tile's readers are done
-                    for (int r = pt; r < 128; r += kTcProducers) {
-                        const int key = k_begin + j * 128 + r;
-                        place[r] = key >= kr.lo && key < k_end ? paged_offset(a.p, b, key) : -1;
-                    }
-                    asm volatile("bar.sync 1, %0;" ::"n"(kTcProducers) : "memory");
-                }
-#pragma unroll 1
-                for (int kv = 0; kv < 2; kv++, push++) {
-                    const int st = push % kTcStages;
-                    const unsigned full = smem_addr(&kv_full[st]);
-                    if (push >= kTcStages)
-                        ok = tc_wait(smem_addr(&kv_empty[st]), (unsigned)(push / kTcStages - 1) & 1u, &failed) && ok;
-                    const unsigned dst = sb + C::kOffKV + st * C::kTile;
-                    if (tma) {
-                        // all arrivals by one thread, with the bytes that are on their way
-                        if (pt == 0) {
-                            if (ok) mbar_expect_tx(full, C::kTile);
-                            mbar_arrive(full, ok ? kTcProducers - 1 : kTcProducers);
-                        }
-                        if (pt < boxes && ok) {
-#pragma unroll
-                            for (int h = 0; h < NH; h++)
-                                tma_load_4d(dst + h * C::kHalf + pt * a.box * 128, kv ? &mv : &mk, 64 * h, py, kvh, pg, full);
-                        }
-                    } else {
-                        const char* src = kv ? a.p.v : a.p.k;
-                        if (ok) {
-#pragma unroll 4
-                            for (int r = pr; r < 128; r += RPP) {
-                                const int64_t o = place[r];
-                                cp_async16(dst + at(r), src + (o < 0 ? 0 : o + head_off), o >= 0);
-                            }
-                        }
-                        cp_async_arrive(full);
-                    }
-                }
+                feed.begin(j);
+                feed.look(j + 1);
+                feed.push(j, false);
+                feed.push(j, true);
             }
-            // nothing in flight when the block ends: the products waited for every TMA copy, unless a wait gave up
-            if (*(volatile int*)&failed)
-                for (int i = max(0, push - kTcStages); i < push; i++)
-                    tc_wait(smem_addr(&kv_full[i % kTcStages]), (unsigned)(i / kTcStages) & 1u, nullptr);
-            cp_async_commit();
-            cp_async_wait<0>();
+            feed.end();
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == 16)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512) : "memory");
+    if (t == 0 && failed) paged_report(a.p, VB_PAGED_TIMEOUT);
+}
+
+// The same for f32 rows over a bf16 cache, with f32's precision: one tile of 128 rows,
+// q and the weights as three bf16 terms (all 24 bits), so a product is three.  The scores
+// of two key tiles take turns in tensor memory, so that one's softmax runs while the
+// products of the other's do: 1536 clocks each for Q.K and P.V at D = 128, against about
+// 1500 of softmax.  P.V of a key tile is summed apart and added to the running sums, which
+// the softmax threads hold, by FMAs: the tensor cores' own accumulation cuts bits off.
+// Tensor memory: scores 2 x 128 columns, over which the high and middle terms of the
+// weights go; P.V 128; the low terms 2 x 64.
+constexpr int kExRows = 128;
+constexpr int kExThreads = 384;
+constexpr int kExStages = 3;
+
+template <int D>
+struct ExCfg {
+    static constexpr int kHalf = 128 * 128;
+    static constexpr int kTile = kHalf * (D / 64);
+    static constexpr int kOffKV = 3 * kTile;
+    static constexpr int kSmem = kOffKV + kExStages * kTile + 1024;
+    static constexpr int kPV = 256, kLow = 384;
+};
+
+template <int D>
+__global__ void __launch_bounds__(kExThreads, 1) paged_attn_exact_kernel(const __grid_constant__ AttnView a,
+                                                                         const __grid_constant__ CUtensorMap mk,
+                                                                         const __grid_constant__ CUtensorMap mv) {
+    using C = ExCfg<D>;
+    constexpr int NH = D / 64;
+    constexpr uint32_t kIdS = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+    constexpr uint32_t kIdPV = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
+    extern __shared__ char smem_raw[];
+    __shared__ __align__(8) unsigned long long q_full, kv_full[kExStages], kv_empty[kExStages], s_full[2], p_full[2],
+        pv_full, pv_free;
+    __shared__ unsigned tmem_slot;
+    __shared__ int failed;
+    __shared__ int64_t place[2][128];
+    __shared__ float xch[2][2][128];
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31, wg = t >> 7;
+    pdl_wait();
+    pdl_trigger();
+    int64_t idx = blockIdx.x;
+    const int split = (int)(idx % a.many.splits);
+    idx /= a.many.splits;
+    const int kvh = (int)(idx % a.p.kv_heads);
+    idx /= a.p.kv_heads;
+    int b, tile;
+    find_tile(a, idx, kExRows, lane, b, tile);
+    if (b < 0) return;
+    const PagedSeq s = paged_seq(a.p, b);
+    const int rows = s.n * a.group, r0 = tile * kExRows;
+    if (r0 >= rows) return;
+    const KeyRange kr = key_range(a, s, r0, a.many);
+    if (split >= splits_used(a.many, kr)) return;
+    const int k_begin = kr.base + split * a.many.len, k_end = min(k_begin + a.many.len, kr.hi);
+    const int n = max(0, (k_end - k_begin + 127) / 128);
+
+    const unsigned sb = (smem_addr(smem_raw) + 1023u) & ~1023u;
+    if (t == 0) {
+        mbar_init(smem_addr(&q_full), 8);
+        for (int i = 0; i < kExStages; i++) {
+            mbar_init(smem_addr(&kv_full[i]), kTcProducers);
+            mbar_init(smem_addr(&kv_empty[i]), 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(smem_addr(&s_full[i]), 1);
+            mbar_init(smem_addr(&p_full[i]), 8);
+        }
+        mbar_init(smem_addr(&pv_full), 1);
+        mbar_init(smem_addr(&pv_free), 8);
+        failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned tm = tmem_slot;
+
+    if (wg < 2) {
+        // ------------------------------------------------------ softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int hf = wg, row = t & 127, r = r0 + row;  // half of the keys (scores, weights) and of the dims (sums)
+        const bool live = r < rows;
+        const int pos = live ? s.len - s.n + r / a.group : -1;
+        const int rr = min(r, rows - 1);
+        const int token = s.start + rr / a.group, head = kvh * a.group + rr % a.group;
+        // q's three terms, 16 bytes of each a step
+        for (int i = t; i < 128 * (D / 8); i += 256) {
+            const int qr = i / (D / 8), c = i % (D / 8), y = min(r0 + qr, rows - 1);
+            const char* src = a.q + (int64_t)(s.start + y / a.group) * a.q_row +
+                              (int64_t)(kvh * a.group + y % a.group) * a.q_head + c * 32;
+            float f[8];
+            Eight<float>::load(src, f);
+            uint32_t w[3][4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                uint32_t tt[3];
+                split_terms<__nv_bfloat16, 3>(f[2 * e], f[2 * e + 1], tt);
+                w[0][e] = tt[0], w[1][e] = tt[1], w[2][e] = tt[2];
+            }
+            const unsigned at = KvFeed<D, kExStages>::at(qr, c);
+#pragma unroll
+            for (int x = 0; x < 3; x++)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sb + x * C::kTile + at), "r"(w[x][0]),
+                             "r"(w[x][1]), "r"(w[x][2]), "r"(w[x][3])
+                             : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&q_full), 1);
+
+        const unsigned lanes = (unsigned)(32 * (warp & 3)) << 16;
+        const unsigned tPV = tm + C::kPV + (D / 2) * hf + lanes;
+        const int pair = 2 + (warp & 3);
+        // (two places in turn: the next key tile's scores may be there before the other warp has read)
+        auto other = [&](float v, int turn) {
+            xch[turn][hf][row] = v;
+            asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+            return xch[turn][hf ^ 1][row];
+        };
+        float m = -INFINITY, l = 0.f, alpha = 0.f;
+        float o[D / 2];
+#pragma unroll
+        for (int d = 0; d < D / 2; d++) o[d] = 0.f;
+        bool ok = true;
+        // adds key tile j's P.V, which was scaled to the maximum that alpha leads from the sums' to
+        auto fold = [&](int j) {
+            ok = tc_wait(smem_addr(&pv_full), (unsigned)j & 1u, &failed) && ok;
+            __syncwarp();
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+            for (int d = 0; d < D / 2; d += 16) {
+                float v[16];
+                tmem_ld16(tPV + d, v);
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[d + e] = fmaf(o[d + e], alpha, v[e]);
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_addr(&pv_free), 1);
+        };
+        // (no way out of the loop when a wait fails: the other warp of the pair counts on this one)
+        for (int j = 0; j < n; j++) {
+            const unsigned tS = tm + 128u * (j & 1) + lanes, tL = tm + C::kLow + 64u * (j & 1) + 32 * hf + lanes;
+            ok = tc_wait(smem_addr(&s_full[j & 1]), (unsigned)(j >> 1) & 1u, &failed) && ok;
+            __syncwarp();
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            float x[64];
+            tmem_ld64(tS + 64 * hf, x);
+            const int k0 = k_begin + j * 128 + 64 * hf;
+            const int hi = min(pos, k_end - 1) - k0, lo = a.window > 0 ? pos - a.window + 1 - k0 : 0;
+            float top = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 64; c++) {
+                x[c] = c <= hi && c >= lo ? x[c] * a.scale_log2 : -INFINITY;
+                top = fmaxf(top, x[c]);
+            }
+            const float mn = fmaxf(m, fmaxf(top, other(top, j & 1)));
+            const float mb = mn == -INFINITY ? 0.f : mn;
+            const float f = ex2_approx(m - mb);
+            m = mn;
+            float sum = 0.f;
+#pragma unroll
+            for (int h = 0; h < 4; h++) {
+                uint32_t w[3][8];
+#pragma unroll
+                for (int c = 0; c < 16; c += 2) {
+                    const float p0 = ex2_approx(x[16 * h + c] - mb), p1 = ex2_approx(x[16 * h + c + 1] - mb);
+                    sum += p0 + p1;
+                    uint32_t tt[3];
+                    split_terms<__nv_bfloat16, 3>(p0, p1, tt);
+                    w[0][c / 2] = tt[0], w[1][c / 2] = tt[1], w[2][c / 2] = tt[2];
+                }
+                tmem_st8(tS + 32 * hf + 8 * h, w[0]);
+                tmem_st8(tS + 64 + 32 * hf + 8 * h, w[1]);
+                tmem_st8(tL + 8 * h, w[2]);
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_addr(&p_full[j & 1]), 1);
+            l = fmaf(l, f, sum);
+            if (j > 0) fold(j - 1);
+            alpha = f;
+        }
+        if (n > 0) fold(n - 1);
+        ok = __all_sync(0xffffffffu, ok);
+        asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");  // the last maximum has been read
+        l += other(l, 0);
+        const bool last = a.many.splits == 1;
+        const float inv = last ? (l > 0.f ? 1.f / l : 0.f) : 1.f;
+        const int64_t th = (int64_t)token * a.heads + head;
+        const int64_t pth = (int64_t)split * a.p.tokens * a.heads + th;
+        if (live && ok) {
+            float* dst = last ? reinterpret_cast<float*>(a.out + token * a.o_row + head * a.o_head) : a.part + pth * D;
+#pragma unroll
+            for (int d = 0; d < D / 2; d += 8) {
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[e] = o[d + e] * inv;
+                Eight<float>::store(dst + (D / 2) * hf + d, y);
+            }
+            if (hf == 0) {
+                if (!last)
+                    a.part_ml[pth] = make_float2(m, l);
+                else if (a.lse)
+                    a.lse[th] = l > 0.f ? (m + log2f(l)) * 0.693147180559945309f : -INFINITY;
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 8) {
+            // ------------------------------------------------- products (see the kernel above)
+            const unsigned leader = elect_one();
+            const unsigned utm = __shfl_sync(0xffffffffu, tm, 0);
+            const int nk = __shfl_sync(0xffffffffu, n, 0);
+            const int k_lo = __shfl_sync(0xffffffffu, kr.lo - k_begin, 0), k_hi = __shfl_sync(0xffffffffu, k_end - k_begin, 0);
+            const unsigned q_d = (sb & 0x3FFFFu) >> 4, kv_d = q_d + (C::kOffKV >> 4);
+            bool ok = nk > 0 && tc_wait(smem_addr(&q_full), 0u, &failed);
+            // K and V come in the order they are used: K0, K1, V0, K2, V1, ...
+            auto wait_kv = [&](int push, int j) {
+                ok = ok && tc_wait(smem_addr(&kv_full[push % kExStages]), (unsigned)(push / kExStages) & 1u, &failed);
+                if (!a.box || j * 128 < k_lo || j * 128 + 128 > k_hi) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                ok = __all_sync(0xffffffffu, ok);
+            };
+            int push = 0;
+            auto qk = [&](int j) {
+                wait_kv(push, j);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (ok) {
+                    const unsigned kd = kv_d + (push % kExStages) * (C::kTile >> 4);
+                    // the small terms first
+#pragma unroll
+                    for (int x = 2; x >= 0; x--)
+#pragma unroll
+                        for (int h = 0; h < NH; h++)
+#pragma unroll
+                            for (int k = 0; k < 4; k++)
+                                mma_ss(leader, utm + 128u * (j & 1), q_d + x * (C::kTile >> 4) + h * (C::kHalf >> 4) + 2 * k,
+                                       kd + h * (C::kHalf >> 4) + 2 * k, kIdS, x < 2 || h > 0 || k > 0);
+                }
+                commit_one(leader, smem_addr(&s_full[j & 1]));
+                commit_one(leader, smem_addr(&kv_empty[push % kExStages]));
+                push++;
+            };
+            if (nk > 0) qk(0);
+            for (int j = 0; j < nk; j++) {
+                if (j + 1 < nk) qk(j + 1);
+                wait_kv(push, j);
+                ok = ok && tc_wait(smem_addr(&p_full[j & 1]), (unsigned)(j >> 1) & 1u, &failed);
+                if (j > 0) ok = ok && tc_wait(smem_addr(&pv_free), (unsigned)(j - 1) & 1u, &failed);
+                ok = __all_sync(0xffffffffu, ok);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (ok) {
+                    const unsigned vd = kv_d + (push % kExStages) * (C::kTile >> 4);
+#pragma unroll
+                    for (int x = 2; x >= 0; x--) {
+                        const unsigned tp = x == 2 ? utm + C::kLow + 64u * (j & 1) : utm + 128u * (j & 1) + 64u * x;
+#pragma unroll
+                        for (int k = 0; k < 8; k++)
+                            mma_ts(leader, utm + C::kPV, tp + 8u * k, vd + 128 * k, kIdPV, x < 2 || k > 0);
+                    }
+                }
+                commit_one(leader, smem_addr(&pv_full));
+                commit_one(leader, smem_addr(&kv_empty[push % kExStages]));
+                push++;
+            }
+            // every product has landed before the tensor memory goes
+            if (nk > 0) tc_wait(smem_addr(&pv_full), (unsigned)(nk - 1) & 1u, nullptr);
+        } else {
+            // ------------------------------------------------- producers
+            KvFeed<D, kExStages> feed{a, &mk, &mv, place, &failed, sb + C::kOffKV, smem_addr(kv_full), smem_addr(kv_empty),
+                                      b, kvh, kr.lo, k_begin, k_end, n, t - (kExThreads - kTcProducers),
+                                      a.box ? 128 / a.box : 0};
+            feed.look(0);
+            feed.look(1);
+            if (n > 0) {
+                feed.begin(0);
+                feed.push(0, false);
+            }
+            for (int j = 0; j < n; j++) {
+                if (j + 1 < n) {
+                    feed.begin(j + 1);
+                    feed.push(j + 1, false);
+                }
+                feed.push(j, true);
+                feed.look(j + 2);
+            }
+            feed.end();
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 8)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512) : "memory");
     if (t == 0 && failed) paged_report(a.p, VB_PAGED_TIMEOUT);
 }
@@ -1423,10 +1754,11 @@ Plan make_plan(const PagedView& p, int io, int cache, int heads, int D, int wind
     Plan pl{};
     const int G = heads / p.kv_heads;
     const int64_t most = (int64_t)p.max_new * G, total = (int64_t)p.tokens * G;  // rows of a KV head
-    // 16-bit rows on the tensor cores' 256-row tiles from 33 rows a sequence on; one
-    // sequence alone takes one kernel for all it may hold
-    const bool tc = io != VB_F32 && most > kFewRows;
-    pl.few_rows = !tc ? 0x7fffffff : p.batch == 1 ? 0 : kFewRows;
+    // Over a 16-bit cache sequences with more than 32 rows (16 of f32) run on the tensor cores' tiles
+    // of 256 (128); one sequence alone takes one kernel for all it may hold.
+    const int few = io == VB_F32 ? 16 : kFewRows, many_rows = io == VB_F32 ? kExRows : kTcRows;
+    const bool tc = cache != VB_F32 && most > few;
+    pl.few_rows = !tc ? 0x7fffffff : p.batch == 1 ? 0 : few;
     const int64_t few_most = std::min<int64_t>(most, pl.few_rows);
     // rows of a tile: all of a sequence's where that is at most 32 (16 where q takes three terms or
     // 32 bits: more do not fit the registers)
@@ -1451,9 +1783,9 @@ Plan make_plan(const PagedView& p, int io, int cache, int heads, int D, int wind
         pl.stream = (int)std::min<int64_t>(cache == VB_F32 && D == 128 ? 148 : kStreamMost, most_units);
     }
     pl.few = make_cut(tile, 16, span(tile, 16), want, 64, 64);
-    const int64_t tiles2 = std::max<int64_t>(1, (total + kTcRows - 1) / kTcRows);
+    const int64_t tiles2 = std::max<int64_t>(1, (total + many_rows - 1) / many_rows);
     const int64_t want2 = std::max<int64_t>(1, 148 / (tiles2 * p.kv_heads));
-    pl.many = make_cut(kTcRows, 128, span(kTcRows, 128), want2, 128, 512);
+    pl.many = make_cut(many_rows, 128, span(many_rows, 128), want2, 128, 512);
     pl.max_splits = (int)std::max<int64_t>(pl.few_rows ? std::min<int64_t>(want, (all + 63) / 64) : 1,
                                            tc ? std::min<int64_t>(want2, (all + 511) / 512) : 1);
     if (!tc) pl.many.splits = 1;
@@ -1511,23 +1843,30 @@ vb_status launch_few(const AttnView& a, cudaStream_t s) {
 template <typename IO, typename KV, int D>
 vb_status launch_attn(const AttnView& a, cudaStream_t s) {
     cudaError_t e;
-    if constexpr (sizeof(IO) == 2) {
+    if constexpr (sizeof(KV) == 2) {
         if (a.few_rows != 0x7fffffff) {
-            static std::atomic<unsigned long long> done{0};
-            e = smem_attr_once(paged_attn_tc_kernel<IO, D>, TcCfg<D>::kSmem, done);
-            if (e != cudaSuccess) return cuda_fail(e, "paged attention: shared memory attribute");
-            const int64_t tiles = std::min<int64_t>(
-                (int64_t)a.p.batch * (((int64_t)a.p.max_new * a.group + kTcRows - 1) / kTcRows),
-                (int64_t)a.p.tokens * a.group / kTcRows + a.p.batch);
+            const int rows = a.many.rows;
+            const int64_t tiles = std::min<int64_t>((int64_t)a.p.batch * (((int64_t)a.p.max_new * a.group + rows - 1) / rows),
+                                                    (int64_t)a.p.tokens * a.group / rows + a.p.batch);
             const int64_t grid = tiles * a.many.splits * a.p.kv_heads;
             if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
             AttnView b = a;
             CUtensorMap mk{}, mv{};
-            b.box = page_map(a.p, a.p.k, D, std::is_same<IO, __half>::value, &mk);
-            if (b.box && !page_map(a.p, a.p.v, D, std::is_same<IO, __half>::value, &mv)) b.box = 0;
-            e = launch_pdl(paged_attn_tc_kernel<IO, D>, dim3((unsigned)grid), dim3(kTcThreads), TcCfg<D>::kSmem, s, b, mk,
-                           mv);
-            if (e != cudaSuccess) return cuda_fail(e, "paged_attn_tc_kernel");
+            b.box = page_map(a.p, a.p.k, D, std::is_same<KV, __half>::value, &mk);
+            if (b.box && !page_map(a.p, a.p.v, D, std::is_same<KV, __half>::value, &mv)) b.box = 0;
+            static std::atomic<unsigned long long> done{0};
+            if constexpr (sizeof(IO) == 4) {
+                e = smem_attr_once(paged_attn_exact_kernel<D>, ExCfg<D>::kSmem, done);
+                if (e == cudaSuccess)
+                    e = launch_pdl(paged_attn_exact_kernel<D>, dim3((unsigned)grid), dim3(kExThreads), ExCfg<D>::kSmem, s, b,
+                                   mk, mv);
+            } else {
+                e = smem_attr_once(paged_attn_tc_kernel<IO, D>, TcCfg<D>::kSmem, done);
+                if (e == cudaSuccess)
+                    e = launch_pdl(paged_attn_tc_kernel<IO, D>, dim3((unsigned)grid), dim3(kTcThreads), TcCfg<D>::kSmem, s,
+                                   b, mk, mv);
+            }
+            if (e != cudaSuccess) return cuda_fail(e, "paged attention, many rows");
         }
     }
     if (a.few_rows) {
