@@ -294,7 +294,10 @@ VB_API vb_status vb_paged_append(const vb_paged_cache* cache, const vb_paged_bat
 
 /* Causal attention of the new tokens over their sequences' pages (appended
  * before): row with position p sees positions j <= p, with window > 0 only
- * j > p - window.  out [tokens][heads][D] = softmax(scale * q.k) v; an empty
+ * j > p - window.  Places that no row of the call sees -- behind a sequence's
+ * length, in pages of nobody -- may hold anything, NaN too; an infinity or NaN
+ * in a v that some rows of a chunk see and others do not reaches all of them.
+ * out [tokens][heads][D] = softmax(scale * q.k) v; an empty
  * row gives zeros.  lse (f32 [tokens][heads], may be NULL) gets the natural
  * logarithm of the sum of exp(scale * q.k), -inf for an empty row.  heads is a
  * multiple of kv_heads; query heads h*G .. h*G + G-1 read KV head h.  io as in

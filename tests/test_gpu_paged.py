@@ -188,6 +188,49 @@ def test_mixed_batch(io, cache, H, KVH):
 
 
 @pytest.mark.parametrize("io,cache", PAIRS)
+@pytest.mark.parametrize("D,H,KVH,page,order", [(128, 16, 8, 16, "phd"), (64, 7, 7, 24, "hpd"), (128, 20, 1, 1, "phd"),
+                                               (64, 12, 2, 64, "phd"), (128, 32, 2, 16, "hpd")])
+def test_decode_many_sequences(io, cache, D, H, KVH, page, order):
+    # more tiles than a card's clusters: the keys are shared out over blocks that end inside tiles
+    B = 300 // KVH + 3
+    news = [0 if b % 11 == 5 else 1 for b in range(B)]
+    lens = [(b * 97) % 700 + 1 if b % 7 else 0 for b in range(B)]
+    check_attn(Setup(news, [max(n, m) if n and m else m for n, m in zip(news, lens)], io, cache, H=H, KVH=KVH, D=D,
+                     page=page, order=order, seed=B))
+
+
+@pytest.mark.parametrize("io,cache", PAIRS)
+@pytest.mark.parametrize("new", [2, 4, 7, 8, 11, 16])
+def test_a_few_tokens_of_many_sequences(io, cache, new):
+    B = 45
+    news = [1 + (b * 5) % new for b in range(B)]
+    news[3] = new
+    check_attn(Setup(news, [n + (b * 131) % 500 for b, n in enumerate(news)], io, cache, H=16, KVH=8, seed=new))
+
+
+@pytest.mark.parametrize("io,cache", PAIRS)
+@pytest.mark.parametrize("G", [1, 2, 8, 9, 16, 17, 33])
+def test_decodes_beside_prompts(io, cache, G):
+    # every third sequence reads a chunk, the others decode: both kernels of a call, their halves apart
+    B = 40
+    news = [120 + b if b % 3 == 1 else 1 for b in range(B)]
+    check_attn(Setup(news, [n + (b * 211) % 900 for b, n in enumerate(news)], io, cache, H=2 * G, KVH=2, seed=G))
+
+
+@pytest.mark.parametrize("io,cache", PAIRS)
+def test_window_over_many_sequences(io, cache):
+    B = 50
+    check_attn(Setup([1] * B, [(b * 61) % 800 + 1 for b in range(B)], io, cache, H=16, KVH=8, seed=3), window=200)
+
+
+@pytest.mark.parametrize("io,cache", PAIRS)
+@pytest.mark.parametrize("ctx", [3000, 9000])
+def test_a_chunk_of_a_long_document(io, cache, ctx):
+    # few row tiles and many keys: the keys are split and joined
+    check_attn(Setup([40, 70], [ctx, ctx // 2], io, cache, seed=ctx, page=32))
+
+
+@pytest.mark.parametrize("io,cache", PAIRS)
 @pytest.mark.parametrize("window", [1, 2, 15, 16, 17, 100, 128, 1000])
 def test_window(io, cache, window):
     check_attn(Setup([1, 200, 1], [700, 600, 40], io, cache, seed=window), window=window)
@@ -388,6 +431,35 @@ def test_append_bad_descriptors():
     s.q_start[1] = 9
     vb200.paged_append(s.pc, s.pb, s.kn, s.vn)
     assert int(s.status) & vb200.PAGED_BAD_ROWS
+
+
+@pytest.mark.parametrize("io,cache", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16")])
+def test_offsets_past_32_bits(io, cache):
+    # a pool of more than 2^31 elements: the pages in use lie at its end
+    pages, page, KVH, D = 140000, 16, 8, 128
+    if torch.cuda.mem_get_info()[0] < 25 << 30:
+        pytest.skip("needs 25 GB")
+    k = torch.empty(pages, page, KVH, D, device="cuda", dtype=TYPES[cache])
+    assert k.numel() > 2**31
+    v = torch.empty_like(k)
+    s = Setup([1, 30], [300, 200], io, cache, H=16, KVH=KVH, D=D, page=page, seed=2, status=False)
+    table = s.table.clone()
+    for b in range(2):
+        for j in range((s.lens_h[b] + page - 1) // page):
+            to = pages - 1 - 40 * b - j
+            k[to], v[to] = s.k[s.table[b, j].long()], s.v[s.table[b, j].long()]
+            table[b, j] = to
+    want = check_attn(s)
+    pb = vb200.PagedBatch(s.q_start, s.lens, table, max_new=30, max_len=300, tokens=31)
+    out = s.out()
+    vb200.paged_attn(vb200.PagedCache(k, v), pb, s.q, out)
+    assert torch.equal(out, want)
+    s.k[:], s.v[:] = 0, 0
+    vb200.paged_append(vb200.PagedCache(k, v), pb, s.kn, s.vn)
+    b, pos = 1, s.lens_h[1] - 1
+    assert torch.equal(k[table[b, pos // page].long(), pos % page], s.kn[30].to(k.dtype))
+    del k, v
+    torch.cuda.empty_cache()
 
 
 # ------------------------------------------------- as a user runs them together

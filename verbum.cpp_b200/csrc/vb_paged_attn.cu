@@ -81,6 +81,7 @@ struct AttnView {
     bool cluster;       // a cluster of blocks for each tile (one row tile a sequence, few and short)
     int stream;         // blocks that share all its keys evenly (one row tile a sequence); 0: a block per tile and split
     Cut few, many;
+    bool after_many;    // the few-rows kernel of this call follows its many-rows kernel
     int box;            // rows of a page that one TMA copy brings (many rows); 0: no tensor maps
     float* part;        // [split][token][head][D] sums of a split, relative to its maximum
     float2* part_ml;    // [split][token][head] (maximum in base 2, sum of weights)
@@ -621,8 +622,17 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
     using C = FewCfg<KV, D, NR>;
     extern __shared__ __align__(1024) char smem[];
     __shared__ float2 ml[kFewWarps][C::kRows];
-    pdl_wait();
+    // Behind the many-rows kernel of the same call the work itself needs no wait: nothing here
+    // reads what that one writes, and it lets this one start only when every block of its own
+    // has waited for what came before.  The wait at the end keeps the order for what follows.
+    if (!a.after_many) pdl_wait();
     pdl_trigger();
+    struct AtEnd {
+        bool wait;
+        __device__ ~AtEnd() {
+            if (wait) pdl_wait();
+        }
+    } at_end{a.after_many};
     if constexpr (MODE == kCluster) {
         __shared__ float2 kept[C::kRows];
         const int rank = (int)cl_rank(), tile = (int)blockIdx.x / kCl;
@@ -1737,7 +1747,6 @@ struct Plan {
     Cut few, many;
     int max_splits;  // for any window
 };
-constexpr int kFewRows = 32;
 constexpr int kStreamMost = 148 * 3;  // blocks that share out a batch's keys
 
 Cut make_cut(int rows, int align, int64_t keys, int64_t want, int step, int least) {
@@ -1754,11 +1763,13 @@ Plan make_plan(const PagedView& p, int io, int cache, int heads, int D, int wind
     Plan pl{};
     const int G = heads / p.kv_heads;
     const int64_t most = (int64_t)p.max_new * G, total = (int64_t)p.tokens * G;  // rows of a KV head
-    // Over a 16-bit cache sequences with more than 32 rows (16 of f32) run on the tensor cores' tiles
-    // of 256 (128); one sequence alone takes one kernel for all it may hold.
-    const int few = io == VB_F32 ? 16 : kFewRows, many_rows = io == VB_F32 ? kExRows : kTcRows;
-    const bool tc = cache != VB_F32 && most > few;
-    pl.few_rows = !tc ? 0x7fffffff : p.batch == 1 ? 0 : few;
+    // Over a 16-bit cache batches that may hold more than 16 rows of a KV head a sequence (8 of f32;
+    // one decoded token's G in any case) run on the tensor cores' tiles of 256 (128) rows, all but the
+    // sequences of a token or few.  64 x 4096 keys, bf16: 16 rows 252 us here and 391 there, 32 rows
+    // 464 and 344.  One sequence alone takes one kernel for all it may hold.
+    const int least = G <= 8 ? 8 : G <= 16 || io == VB_F32 ? 16 : 32, many_rows = io == VB_F32 ? kExRows : kTcRows;
+    const bool tc = cache != VB_F32 && most > (io == VB_F32 ? least : std::max(least, 16));
+    pl.few_rows = !tc ? 0x7fffffff : p.batch == 1 ? 0 : least;
     const int64_t few_most = std::min<int64_t>(most, pl.few_rows);
     // rows of a tile: all of a sequence's where that is at most 32 (16 where q takes three terms or
     // 32 bits: more do not fit the registers)
@@ -1778,7 +1789,7 @@ Plan make_plan(const PagedView& p, int io, int cache, int heads, int D, int wind
         const int64_t most_units = (int64_t)p.batch * p.kv_heads * ((span(tile, 16) + kUnit - 1) / kUnit);
         if (most_units > 0x3fffffff) return pl;  // (the caller refuses)
         // Clusters where all fit the card at once and a block's share is at most 512 keys: one token
-        // of one sequence of 777 keys takes one launch and CLUSTER_US instead of two and STREAM_US.
+        // of one sequence of 777 keys takes one launch and 7.2 us of its caller instead of two and 9.8.
         pl.cluster = (int64_t)p.batch * p.kv_heads * kCl <= 148 * 2 && span(tile, 16) <= kCl * 512;
         pl.stream = (int)std::min<int64_t>(cache == VB_F32 && D == 128 ? 148 : kStreamMost, most_units);
     }
@@ -1870,13 +1881,15 @@ vb_status launch_attn(const AttnView& a, cudaStream_t s) {
         }
     }
     if (a.few_rows) {
+        AttnView f = a;
+        f.after_many = a.few_rows != 0x7fffffff;
         vb_status st = VB_OK;
         if (a.few.rows == 8) {
-            st = launch_few<IO, KV, D, 1>(a, s);
+            st = launch_few<IO, KV, D, 1>(f, s);
         } else if (sizeof(IO) == 4 || a.few.rows == 16) {
-            st = launch_few<IO, KV, D, 2>(a, s);
+            st = launch_few<IO, KV, D, 2>(f, s);
         } else {
-            if constexpr (sizeof(IO) == 2) st = launch_few<IO, KV, D, 4>(a, s);
+            if constexpr (sizeof(IO) == 2) st = launch_few<IO, KV, D, 4>(f, s);
         }
         if (st) return st;
     }
