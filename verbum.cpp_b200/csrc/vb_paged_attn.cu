@@ -243,25 +243,25 @@ __device__ __forceinline__ void cut_tf32(float x, uint32_t& hi, uint32_t& lo) {
     hi = __float_as_uint(x) & 0xffffe000u;
     lo = __float_as_uint(x - __uint_as_float(hi));
 }
-constexpr int kFewWarps = 4;
 constexpr int kBK = 16;  // keys a warp takes at a time
 
 template <typename KV, int D, int NR>
 struct FewCfg {
     static constexpr int kRows = 8 * NR;
+    static constexpr int kWarps = sizeof(KV) == 4 && D == 128 ? 6 : 4;
     static constexpr int kRowBytes = D * (int)sizeof(KV);
     static constexpr int kBlockBytes = kBK * kRowBytes;  // K or V of a block
-    // 64 KB of ring per CTA and three CTAs on an SM, or (f32, D = 128) 128 KB and one.  (A third
+    // 64 KB of ring per CTA and three CTAs on an SM, or (f32, D = 128) 192 KB, six warps and one.  (A third
     // stage and two CTAs moved less: a piece's end and the next one's start leave a CTA without
     // loads in flight, and more of the others' fill in.)
     static constexpr int kStages = kRowBytes == 128 ? 4 : 2;
     static constexpr int kWarpBytes = kStages * 2 * kBlockBytes;
     static constexpr int kLd = D + 4;  // row of the warps' sums, floats
-    static constexpr int kMerge = kFewWarps * kRows * kLd * 4;
-    static constexpr int kSmem = kFewWarps * kWarpBytes > kMerge ? kFewWarps * kWarpBytes : kMerge;
+    static constexpr int kMerge = kWarps * kRows * kLd * 4;
+    static constexpr int kSmem = kWarps * kWarpBytes > kMerge ? kWarps * kWarpBytes : kMerge;
 };
 
-// Attention of 8 NR rows of a KV head by 4 warps.  The warps share the rows and
+// Attention of 8 NR rows of a KV head by the warps of a block.  They share the rows and
 // take turns at blocks of 16 keys, each with a ring of its own in shared memory
 // (no barrier in the loop); at the end they join their (m, l, sum).
 //
@@ -298,13 +298,13 @@ __device__ __forceinline__ void few_piece(const AttnView& a, const PagedSeq& s, 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     const int rows = s.n * a.group;
     const int blocks = max(0, (k_end - k_begin + kBK - 1) / kBK);
-    const int mine = blocks > warp ? (blocks - warp + kFewWarps - 1) / kFewWarps : 0;  // blocks warp, warp + 4, ...
+    const int mine = blocks > warp ? (blocks - warp + C::kWarps - 1) / C::kWarps : 0;  // blocks warp, warp + kWarps, ...
 
     const unsigned ring = smem_addr(smem) + warp * C::kWarpBytes;
     const int64_t head_off = (int64_t)kvh * a.p.stride_head;
     // lane l looks up the place of key l % 16 of a block; -1: outside, read as zeros
     auto look_up = [&](int i) -> int64_t {
-        const int key = k_begin + (warp + i * kFewWarps) * kBK + (lane & 15);
+        const int key = k_begin + (warp + i * C::kWarps) * kBK + (lane & 15);
         return i < mine && key >= kr.lo && key < k_end ? paged_offset(a.p, b, key) : -1;
     };
     // 16-byte chunk c of row r sits at chunk c ^ swz(r): no load below meets a bank twice, be it
@@ -386,7 +386,7 @@ __device__ __forceinline__ void few_piece(const AttnView& a, const PagedSeq& s, 
         fetch(i + C::kStages - 1, next);
         next = look_up(i + C::kStages);
         const unsigned kb = ring + (unsigned)(i % C::kStages) * 2 * C::kBlockBytes, vb = kb + C::kBlockBytes;
-        const int key0 = k_begin + (warp + i * kFewWarps) * kBK;
+        const int key0 = k_begin + (warp + i * C::kWarps) * kBK;
         // scores: keys g (e 0, 1) and g + 8 (e 2, 3), rows 2 t4 + (e & 1); the small terms apart
         float sc[NR][4] = {}, sl[NR][4] = {}, sm[kF32 ? NR : 1][4] = {};
         if constexpr (kF32) {
@@ -567,15 +567,15 @@ __device__ __forceinline__ void few_piece(const AttnView& a, const PagedSeq& s, 
                 sums[(warp * C::kRows + 8 * n + 2 * t4 + (e & 1)) * C::kLd + d] = o[n][i][e];
             }
     __syncthreads();
-    for (int it = threadIdx.x; it < C::kRows * (D / 8); it += kFewWarps * 32) {
+    for (int it = threadIdx.x; it < C::kRows * (D / 8); it += C::kWarps * 32) {
         const int row = it / (D / 8), r = r0 + row, d = it % (D / 8) * 8;
         if (r >= rows) break;
         float M = -INFINITY, L = 0.f;
         float y[8] = {};
 #pragma unroll
-        for (int x = 0; x < kFewWarps; x++) M = fmaxf(M, ml[x][row].x);
+        for (int x = 0; x < C::kWarps; x++) M = fmaxf(M, ml[x][row].x);
 #pragma unroll
-        for (int x = 0; x < kFewWarps; x++) {
+        for (int x = 0; x < C::kWarps; x++) {
             const float w = ex2_approx(ml[x][row].x - (M == -INFINITY ? 0.f : M));
             L = fmaf(ml[x][row].y, w, L);
             float z[8];
@@ -618,10 +618,10 @@ enum FewMode { kGrid, kStream, kCluster };
 constexpr int kCl = 8;
 
 template <typename IO, typename KV, int D, int NR, int MODE>
-__global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __grid_constant__ AttnView a) {
+__global__ void __launch_bounds__(FewCfg<KV, D, NR>::kWarps * 32) paged_attn_few_kernel(const __grid_constant__ AttnView a) {
     using C = FewCfg<KV, D, NR>;
     extern __shared__ __align__(1024) char smem[];
-    __shared__ float2 ml[kFewWarps][C::kRows];
+    __shared__ float2 ml[C::kWarps][C::kRows];
     // Behind the many-rows kernel of the same call the work itself needs no wait: nothing here
     // reads what that one writes, and it lets this one start only when every block of its own
     // has waited for what came before.  The wait at the end keeps the order for what follows.
@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
         const Sink sink{false, nullptr, nullptr, 0, false, true};
         few_piece<IO, KV, D, NR>(a, s, b, kvh, 0, kr, k_begin, k_end, sink, smem, ml, kept);
         cluster_sync_all();
-        for (int it = rank * kFewWarps * 32 + threadIdx.x; it < C::kRows * (D / 4); it += kCl * kFewWarps * 32) {
+        for (int it = rank * C::kWarps * 32 + threadIdx.x; it < C::kRows * (D / 4); it += kCl * C::kWarps * 32) {
             const int row = it / (D / 4), d = it % (D / 4) * 4;
             if (row >= rows) break;
             float2 q[kCl];
@@ -692,7 +692,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_attn_few_kernel(const __
         // this block's units, piece by piece: a piece is what it has of one tile
         const int lane = threadIdx.x & 31;
         if (a.p.status && blockIdx.x == 0)  // the sequences that get no units are reported too
-            for (int i = threadIdx.x; i < a.p.batch; i += kFewWarps * 32) paged_seq(a.p, i);
+            for (int i = threadIdx.x; i < a.p.batch; i += C::kWarps * 32) paged_seq(a.p, i);
         int all, unused;
         stream_sums(a, 0, lane, all, unused);
         const int blocks = min(a.stream, all);  // no block between others is empty
@@ -768,7 +768,6 @@ constexpr int kTcThreads = 640;
 constexpr int kTcProducers = 96;
 constexpr int kTcRows = 256;
 constexpr int kTcStages = 4;
-constexpr int kPoly = 4;  // one pair of exponentials in so many on the FMA pipe
 
 template <int D>
 struct TcCfg {
@@ -824,26 +823,6 @@ __device__ __forceinline__ f2 f2add(f2 a, f2 b) {
     f2 d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
-}
-// 2^y of a pair on the FMA pipe, for y <= 8: y = n + f with n whole and |f| <= 1/2 (n
-// falls out of the mantissa of 1.5 * 2^23 + y), 2^f by a polynomial of degree 4 fitted to
-// the least relative error on [-1/2, 1/2] (2.6e-6, of both signs: the weights' sum, which
-// lse shows, stays good to f32's last bits), n added to the exponent.
-__device__ __forceinline__ void exp2_poly(f2 y, float& p0, float& p1) {
-    float y0, y1;
-    f2unpack(y, y0, y1);
-    y = f2pack(fmaxf(y0, -126.f), fmaxf(y1, -126.f));  // the exponent stays a number's
-    const f2 magic = f2pack(12582912.f, 12582912.f);
-    const f2 n = f2add(y, magic), f = f2sub(y, f2sub(n, magic));
-    f2 p = f2fma(f, f2pack(0.0095701f, 0.0095701f), f2pack(0.05591786f, 0.05591786f));
-    p = f2fma(f, p, f2pack(0.24024745f, 0.24024745f));
-    p = f2fma(f, p, f2pack(0.69312181f, 0.69312181f));
-    p = f2fma(f, p, f2pack(0.99999926f, 0.99999926f));
-    float n0, n1;
-    f2unpack(p, p0, p1);
-    f2unpack(n, n0, n1);
-    p0 = __int_as_float(__float_as_int(p0) + (__float_as_int(n0) << 23));
-    p1 = __int_as_float(__float_as_int(p1) + (__float_as_int(n1) << 23));
 }
 __device__ __forceinline__ void tma_load_4d(unsigned dst, const CUtensorMap* map, int x, int y, int z, int w, unsigned mbar) {
     asm volatile(
@@ -1033,7 +1012,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
     extern __shared__ char smem_raw[];
     __shared__ __align__(8) unsigned long long q_full, kv_full[kTcStages], kv_empty[kTcStages], s_full[2],
-        p_full[2], o_full[2];
+        p_full[2][2], o_full[2];
     __shared__ unsigned tmem_slot;
     __shared__ int failed;
     __shared__ int64_t place[2][128];
@@ -1067,14 +1046,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
 
     const unsigned sb = (smem_addr(smem_raw) + 1023u) & ~1023u;
     if (t == 0) {
-        mbar_init(smem_addr(&q_full), kTcProducers);
+        mbar_init(smem_addr(&q_full), 512);
         for (int i = 0; i < kTcStages; i++) {
             mbar_init(smem_addr(&kv_full[i]), kTcProducers);
             mbar_init(smem_addr(&kv_empty[i]), 1);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(smem_addr(&s_full[i]), 1);
-            mbar_init(smem_addr(&p_full[i]), 8);
+            mbar_init(smem_addr(&p_full[i][0]), 8);
+            mbar_init(smem_addr(&p_full[i][1]), 8);
             mbar_init(smem_addr(&o_full[i]), 1);
         }
         failed = 0;
@@ -1100,6 +1080,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         const int pos = live ? s.len - s.n + r / a.group : -1;
         const unsigned lanes = (unsigned)(32 * (warp & 3)) << 16;
         const unsigned tS = tm + 128u * i + lanes, tO = tm + C::kO + 128u * i + (D / 2) * hf + lanes;
+        // q: this half's chunks of 16 bytes of its tile's rows (rows behind the last one: zeros)
+        if (nt[i] > 0) {
+            constexpr int RC = D / 8;
+            for (int x = hf * 128 + row; x < 128 * RC; x += 256) {
+                const int qr = x / RC, c = x % RC, y = r0 + 128 * i + qr;
+                const bool real = y < rows;
+                const int z = real ? y : 0;
+                cp_async16(sb + i * C::kTile + KvFeed<D, kTcStages>::at(qr, c),
+                           a.q + (int64_t)(s.start + z / a.group) * a.q_row +
+                               (int64_t)(kvh * a.group + z % a.group) * a.q_head + c * 16,
+                           real);
+            }
+        }
+        cp_async_arrive(smem_addr(&q_full));
         const float sc = fabsf(a.scale_log2);
         const bool flip = a.scale_log2 < 0.f;
         float m = -INFINITY, l = 0.f;  // m: the maximum the sums are relative to; l: this half's sum
@@ -1113,6 +1107,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         bool ok = true;
         // (no way out of the loop when a wait fails: the other warp of the pair counts on this one)
         for (int j = 0; j < n; j++) {
+            // columns this row sees: lo .. hi
+            const int k0 = k_begin + j * 128 + 64 * hf;
+            const int hi = min(pos, k_end - 1) - k0, lo = a.window > 0 ? pos - a.window + 1 - k0 : 0;
+            const bool edge = __any_sync(0xffffffffu, hi < 63 || lo > 0);
             ok = tc_wait(smem_addr(&s_full[i]), (unsigned)j & 1u, &failed) && ok;
             __syncwarp();
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -1122,10 +1120,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
 #pragma unroll
                 for (int c = 0; c < 64; c++) x[c] = -x[c];
             }
-            // columns this row sees: lo .. hi
-            const int k0 = k_begin + j * 128 + 64 * hf;
-            const int hi = min(pos, k_end - 1) - k0, lo = a.window > 0 ? pos - a.window + 1 - k0 : 0;
-            const bool edge = __any_sync(0xffffffffu, hi < 63 || lo > 0);
             if (edge) {
 #pragma unroll
                 for (int c = 0; c < 64; c++) x[c] = c <= hi && c >= lo ? x[c] : -INFINITY;
@@ -1157,37 +1151,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             const float mb = m == -INFINITY ? 0.f : m;
             f2 sum[2] = {0ull, 0ull};
             const f2 sc2 = f2pack(sc, sc), mb2 = f2pack(-mb, -mb);
-            auto weights = [&](auto inner) {
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    uint32_t w[16];
-#pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
-                        const f2 y = f2fma(f2pack(x[32 * h + c], x[32 * h + c + 1]), sc2, mb2);
-                        float p0, p1;
-                        // some pairs on the FMA pipe, where no score is masked
-                        if (decltype(inner)::value && (c / 2) % kPoly == kPoly - 1) {
-                            exp2_poly(y, p0, p1);
-                        } else {
-                            f2unpack(y, p0, p1);
-                            p0 = ex2_approx(p0);
-                            p1 = ex2_approx(p1);
-                        }
-                        sum[(c >> 1) & 1] = f2add(sum[(c >> 1) & 1], f2pack(p0, p1));
-                        w[c / 2] = pack2<T>(p0, p1);
-                    }
-                    tmem_st16(tS + 32 * hf + 16 * h, w);
-                }
-            };
             // the scores of both halves have been read (other() above): the weights may go over them
-            if (edge)
-                weights(std::false_type{});
-            else
-                weights(std::true_type{});
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_addr(&p_full[i]), 1);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                uint32_t w[16];
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) {
+                    const f2 y = f2fma(f2pack(x[32 * h + c], x[32 * h + c + 1]), sc2, mb2);
+                    float p0, p1;
+                    f2unpack(y, p0, p1);
+                    p0 = ex2_approx(p0);
+                    p1 = ex2_approx(p1);
+                    sum[(c >> 1) & 1] = f2add(sum[(c >> 1) & 1], f2pack(p0, p1));
+                    w[c / 2] = pack2<T>(p0, p1);
+                }
+                tmem_st16(tS + 32 * hf + 16 * h, w);
+                // the products of these 32 keys (of each half) may start while the other 32 are made
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_addr(&p_full[i][h]), 1);
+            }
             l += f2sum(sum[0]) + f2sum(sum[1]);
         }
         if (n > 0) ok = tc_wait(smem_addr(&o_full[i]), 0u, &failed) && ok;
@@ -1278,13 +1262,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
                 for (int i = 0; i < 2; i++) {
                     const int ni = i ? n1 : n0;
                     if (j >= ni) continue;
-                    ok = ok && tc_wait(smem_addr(&p_full[i]), (unsigned)j & 1u, &failed);
-                    ok = __all_sync(0xffffffffu, ok);
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (ok) {
 #pragma unroll
-                        for (int k = 0; k < 8; k++)
-                            mma_ts(leader, utm + C::kO + 128u * i, utm + 128u * i + 8u * k, vd + 128 * k, kIdPV, j > 0 || k > 0);
+                    for (int h = 0; h < 2; h++) {
+                        ok = ok && tc_wait(smem_addr(&p_full[i][h]), (unsigned)j & 1u, &failed);
+                        ok = __all_sync(0xffffffffu, ok);
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        if (!ok) continue;
+                        // keys 32 h .. and 64 + 32 h ..
+#pragma unroll
+                        for (int y = 0; y < 4; y++) {
+                            const int k = 2 * h + (y & 1) + 4 * (y >> 1);
+                            mma_ts(leader, utm + C::kO + 128u * i, utm + 128u * i + 8u * k, vd + 128 * k, kIdPV,
+                                   j > 0 || h > 0 || y > 0);
+                        }
                     }
                     if (j + 1 < ni)
                         qk(i, j + 1);
@@ -1305,22 +1295,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         } else {
             // ------------------------------------------------- producers
             const int pt = t - (kTcThreads - kTcProducers);
-            using Feed = KvFeed<D, kTcStages>;
-            const int pr = pt / Feed::RC, pc = pt % Feed::RC;
-            for (int i = 0; i < 2; i++) {
-                if (nt[i] == 0) continue;
-                for (int r = pr; r < 128; r += Feed::RPP) {
-                    const int row = r0 + 128 * i + r;
-                    const bool real = row < rows;
-                    const int x = real ? row : 0;
-                    cp_async16(sb + i * C::kTile + Feed::at(r, pc),
-                               a.q + (int64_t)(s.start + x / a.group) * a.q_row +
-                                   (int64_t)(kvh * a.group + x % a.group) * a.q_head + pc * 16,
-                               real);
-                }
-            }
-            cp_async_arrive(smem_addr(&q_full));
-            Feed feed{a, &mk, &mv, place, &failed, sb + C::kOffKV, smem_addr(kv_full), smem_addr(kv_empty),
+            KvFeed<D, kTcStages> feed{a, &mk, &mv, place, &failed, sb + C::kOffKV, smem_addr(kv_full), smem_addr(kv_empty),
                       b, kvh, kr.lo, k_begin, k_end, nmax, pt, a.box ? 128 / a.box : 0};
             feed.look(0);
             for (int j = 0; j < nmax; j++) {
@@ -1835,13 +1810,13 @@ vb_status launch_few(const AttnView& a, cudaStream_t s) {
     if (e != cudaSuccess) return cuda_fail(e, "paged attention: shared memory attribute");
     if (MODE == kCluster) {
         const int64_t blocks = (int64_t)a.p.batch * a.p.kv_heads * kCl;
-        e = launch_pdl_cluster(paged_attn_few_kernel<IO, KV, D, NR, MODE>, dim3((unsigned)blocks), dim3(kFewWarps * 32),
+        e = launch_pdl_cluster(paged_attn_few_kernel<IO, KV, D, NR, MODE>, dim3((unsigned)blocks), dim3(C::kWarps * 32),
                                C::kSmem, dim3(kCl, 1, 1), s, a);
         return e == cudaSuccess ? VB_OK : cuda_fail(e, "paged_attn_few_kernel");
     }
     const int64_t grid = MODE == kStream ? a.stream : (int64_t)a.few.splits * a.p.kv_heads * a.row_tiles * a.p.batch;
     if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
-    e = launch_pdl(paged_attn_few_kernel<IO, KV, D, NR, MODE>, dim3((unsigned)grid), dim3(kFewWarps * 32), C::kSmem, s, a);
+    e = launch_pdl(paged_attn_few_kernel<IO, KV, D, NR, MODE>, dim3((unsigned)grid), dim3(C::kWarps * 32), C::kSmem, s, a);
     return e == cudaSuccess ? VB_OK : cuda_fail(e, "paged_attn_few_kernel");
 }
 
