@@ -800,11 +800,12 @@ __device__ __forceinline__ void mma_ss(unsigned leader, unsigned tmem, unsigned 
         : "memory");
 }
 // D[tmem] (+)= A[tmem] B[smem], B N-major
-__device__ __forceinline__ void mma_ts(unsigned leader, unsigned tmem, unsigned a, unsigned b, uint32_t idesc, bool acc) {
+__device__ __forceinline__ void mma_ts(unsigned leader, unsigned tmem, unsigned a, unsigned b, uint32_t desc, uint32_t idesc,
+                                       bool acc) {
     asm volatile(
         "{ .reg .pred p, q; .reg .b64 db; setp.ne.u32 p, %4, 0; setp.ne.u32 q, %5, 0; mov.b64 db, {%2, %6};"
         " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p; }" ::"r"(tmem),
-        "r"(a), "r"(b | kDescV), "r"(idesc), "r"((unsigned)acc), "r"(leader), "r"(kDescHi)
+        "r"(a), "r"(b | desc), "r"(idesc), "r"((unsigned)acc), "r"(leader), "r"(kDescHi)
         : "memory");
 }
 __device__ __forceinline__ void commit_one(unsigned leader, unsigned mbar) {
@@ -1272,7 +1273,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
 #pragma unroll
                         for (int y = 0; y < 4; y++) {
                             const int k = 2 * h + (y & 1) + 4 * (y >> 1);
-                            mma_ts(leader, utm + C::kO + 128u * i, utm + 128u * i + 8u * k, vd + 128 * k, kIdPV,
+                            mma_ts(leader, utm + C::kO + 128u * i, utm + 128u * i + 8u * k, vd + 128 * k, kDescV, kIdPV,
                                    j > 0 || h > 0 || y > 0);
                         }
                     }
@@ -1314,37 +1315,118 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     if (t == 0 && failed) paged_report(a.p, VB_PAGED_TIMEOUT);
 }
 
-// The same for f32 rows over a bf16 cache, with f32's precision: one tile of 128 rows,
-// q and the weights as three bf16 terms (all 24 bits), so a product is three.  The scores
-// of two key tiles take turns in tensor memory, so that one's softmax runs while the
-// products of the other's do: 1536 clocks each for Q.K and P.V at D = 128, against about
-// 1500 of softmax.  P.V of a key tile is summed apart and added to the running sums, which
-// the softmax threads hold, by FMAs: the tensor cores' own accumulation cuts bits off.
+// The same for f32 rows, with f32's precision: one tile of 128 rows, q and the weights as
+// three bf16 terms (all 24 bits).  Over a bf16 cache a product is three; over an f32 cache
+// K and V are three terms too, made by the producers, and a product is the six that reach
+// 24 bits (high x high down to the pairs of weight 2^-16).  The scores of two key tiles
+// take turns in tensor memory, so that one's softmax runs while the products of the
+// other's do: 1536 clocks each for Q.K and P.V of 128 keys at D = 128 (bf16 cache) against
+// about 1500 of softmax.  P.V of a key tile is summed apart and added to the running sums,
+// which the softmax threads hold, by FMAs: the tensor cores' own accumulation cuts bits off.
 // Tensor memory: scores 2 x 128 columns, over which the high and middle terms of the
 // weights go; P.V 128; the low terms 2 x 64.
 constexpr int kExRows = 128;
-constexpr int kExThreads = 384;
-constexpr int kExStages = 3;
 
-template <int D>
+template <typename KV, int D>
 struct ExCfg {
-    static constexpr int kHalf = 128 * 128;
-    static constexpr int kTile = kHalf * (D / 64);
-    static constexpr int kOffKV = 3 * kTile;
-    static constexpr int kSmem = kOffKV + kExStages * kTile + 1024;
+    static constexpr bool kF32 = sizeof(KV) == 4;
+    static constexpr int kKeys = kF32 ? 64 : 128;       // of a tile
+    static constexpr int kThreads = kF32 ? 512 : 384;   // 8 warps of softmax, one of products, the rest producers
+    static constexpr int kProducers = kThreads - 288;
+    static constexpr int kStages = kF32 ? 2 : 3;
+    static constexpr int kQ = 128 * 128 * (D / 64);     // a term of q
+    static constexpr int kHalf = kKeys * 128;           // 64 dims of K's or V's rows
+    static constexpr int kTerm = kHalf * (D / 64);      // a term of K or V
+    static constexpr int kStage = kTerm * (kF32 ? 3 : 1);
+    static constexpr int kOffKV = 3 * kQ;
+    static constexpr int kSmem = kOffKV + kStages * kStage + 1024;
     static constexpr int kPV = 256, kLow = 384;
+    // which terms of the left and the right operand make a product, the small ones first
+    static constexpr int kProducts = kF32 ? 6 : 3;
+    static __device__ __forceinline__ constexpr int left(int i) {
+        return kF32 ? (i == 0 ? 2 : i == 2 || i == 3 ? 1 : 0) : 2 - i;
+    }
+    static __device__ __forceinline__ constexpr int right(int i) {
+        return kF32 ? (i == 1 ? 2 : i == 2 || i == 4 ? 1 : 0) : 0;
+    }
+};
+static_assert(ExCfg<float, 128>::kProducers == 224 && ExCfg<__nv_bfloat16, 128>::kProducers == kTcProducers, "warps");
+
+// KvFeed's counterpart for an f32 cache: rows of the pages, eight elements at a time, through
+// registers into three bf16 tiles.
+template <int D>
+struct SplitFeed {
+    using C = ExCfg<float, D>;
+    const AttnView& a;
+    int64_t (*place)[128];
+    volatile int* failed;
+    unsigned ring, full, empty;
+    int b, kvh, lo, k_begin, k_end, n, pt;
+    int x = 0;
+    bool ok = true;
+
+    __device__ __forceinline__ void look(int) {}
+    __device__ __forceinline__ void begin(int j) {
+        asm volatile("bar.sync 1, %0;" ::"n"(C::kProducers) : "memory");  // the readers of tile j - 2 are done
+        if (pt < C::kKeys) {
+            const int key = k_begin + j * C::kKeys + pt;
+            place[j & 1][pt] = key >= lo && key < k_end ? paged_offset(a.p, b, key) : -1;
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(C::kProducers) : "memory");
+    }
+    __device__ __forceinline__ void push(int j, bool v) {
+        constexpr int RC = D / 8, ITEMS = C::kKeys * RC, PER = (ITEMS + C::kProducers - 1) / C::kProducers;
+        const int st = x % C::kStages;
+        const char* src = (v ? a.p.v : a.p.k) + (int64_t)kvh * a.p.stride_head;
+        float f[PER][8];
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int it = i * C::kProducers + pt, r = it / RC, c = it % RC;
+            const int64_t o = it < ITEMS ? place[j & 1][r] : -1;
+            if (o >= 0) {
+                Eight<float>::load(src + o + c * 32, f[i]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) f[i][e] = 0.f;
+            }
+        }
+        if (x >= C::kStages) ok = tc_wait(empty + 8 * st, (unsigned)(x / C::kStages - 1) & 1u, failed) && ok;
+        x++;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int it = i * C::kProducers + pt, r = it / RC, c = it % RC;
+            if (it >= ITEMS) break;
+            uint32_t w[3][4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                uint32_t tt[3];
+                split_terms<__nv_bfloat16, 3>(f[i][2 * e], f[i][2 * e + 1], tt);
+                w[0][e] = tt[0], w[1][e] = tt[1], w[2][e] = tt[2];
+            }
+            const unsigned at = ring + st * C::kStage + (unsigned)((c >> 3) * C::kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+#pragma unroll
+            for (int y = 0; y < 3; y++)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + y * C::kTerm), "r"(w[y][0]), "r"(w[y][1]),
+                             "r"(w[y][2]), "r"(w[y][3])
+                             : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(full + 8 * st, 1);
+    }
+    __device__ __forceinline__ void end() {}
 };
 
-template <int D>
-__global__ void __launch_bounds__(kExThreads, 1) paged_attn_exact_kernel(const __grid_constant__ AttnView a,
-                                                                         const __grid_constant__ CUtensorMap mk,
-                                                                         const __grid_constant__ CUtensorMap mv) {
-    using C = ExCfg<D>;
-    constexpr int NH = D / 64;
-    constexpr uint32_t kIdS = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+template <typename KV, int D>
+__global__ void __launch_bounds__(ExCfg<KV, D>::kThreads, 1)
+    paged_attn_exact_kernel(const __grid_constant__ AttnView a, const __grid_constant__ CUtensorMap mk,
+                            const __grid_constant__ CUtensorMap mv) {
+    using C = ExCfg<KV, D>;
+    constexpr int NH = D / 64, kStages = C::kStages, W = C::kKeys / 2;  // W: keys of a softmax thread
+    constexpr uint32_t kIdS = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(C::kKeys >> 3) << 17) | ((128u >> 4) << 24);
+    constexpr uint32_t kDescVE = (uint32_t)(C::kHalf >> 4) << 16;  // from 64 dims of V to the next
     constexpr uint32_t kIdPV = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
     extern __shared__ char smem_raw[];
-    __shared__ __align__(8) unsigned long long q_full, kv_full[kExStages], kv_empty[kExStages], s_full[2], p_full[2],
+    __shared__ __align__(8) unsigned long long q_full, kv_full[kStages], kv_empty[kStages], s_full[2], p_full[2],
         pv_full, pv_free;
     __shared__ unsigned tmem_slot;
     __shared__ int failed;
@@ -1367,13 +1449,13 @@ __global__ void __launch_bounds__(kExThreads, 1) paged_attn_exact_kernel(const _
     const KeyRange kr = key_range(a, s, r0, a.many);
     if (split >= splits_used(a.many, kr)) return;
     const int k_begin = kr.base + split * a.many.len, k_end = min(k_begin + a.many.len, kr.hi);
-    const int n = max(0, (k_end - k_begin + 127) / 128);
+    const int n = max(0, (k_end - k_begin + C::kKeys - 1) / C::kKeys);
 
     const unsigned sb = (smem_addr(smem_raw) + 1023u) & ~1023u;
     if (t == 0) {
         mbar_init(smem_addr(&q_full), 8);
-        for (int i = 0; i < kExStages; i++) {
-            mbar_init(smem_addr(&kv_full[i]), kTcProducers);
+        for (int i = 0; i < kStages; i++) {
+            mbar_init(smem_addr(&kv_full[i]), C::kProducers);
             mbar_init(smem_addr(&kv_empty[i]), 1);
         }
         for (int i = 0; i < 2; i++) {
@@ -1398,7 +1480,10 @@ __global__ void __launch_bounds__(kExThreads, 1) paged_attn_exact_kernel(const _
 
     if (wg < 2) {
         // ------------------------------------------------------ softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        if constexpr (C::kF32)
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        else
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int hf = wg, row = t & 127, r = r0 + row;  // half of the keys (scores, weights) and of the dims (sums)
         const bool live = r < rows;
         const int pos = live ? s.len - s.n + r / a.group : -1;
@@ -1418,10 +1503,10 @@ __global__ void __launch_bounds__(kExThreads, 1) paged_attn_exact_kernel(const _
                 split_terms<__nv_bfloat16, 3>(f[2 * e], f[2 * e + 1], tt);
                 w[0][e] = tt[0], w[1][e] = tt[1], w[2][e] = tt[2];
             }
-            const unsigned at = KvFeed<D, kExStages>::at(qr, c);
+            const unsigned at = KvFeed<D, 3>::at(qr, c);
 #pragma unroll
             for (int x = 0; x < 3; x++)
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sb + x * C::kTile + at), "r"(w[x][0]),
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sb + x * C::kQ + at), "r"(w[x][0]),
                              "r"(w[x][1]), "r"(w[x][2]), "r"(w[x][3])
                              : "memory");
         }
@@ -1461,17 +1546,20 @@ __global__ void __launch_bounds__(kExThreads, 1) paged_attn_exact_kernel(const _
         };
         // (no way out of the loop when a wait fails: the other warp of the pair counts on this one)
         for (int j = 0; j < n; j++) {
-            const unsigned tS = tm + 128u * (j & 1) + lanes, tL = tm + C::kLow + 64u * (j & 1) + 32 * hf + lanes;
+            const unsigned tS = tm + 128u * (j & 1) + lanes, tL = tm + C::kLow + 64u * (j & 1) + W / 2 * hf + lanes;
             ok = tc_wait(smem_addr(&s_full[j & 1]), (unsigned)(j >> 1) & 1u, &failed) && ok;
             __syncwarp();
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            float x[64];
-            tmem_ld64(tS + 64 * hf, x);
-            const int k0 = k_begin + j * 128 + 64 * hf;
+            float x[W];
+            if constexpr (W == 64)
+                tmem_ld64(tS + W * hf, x);
+            else
+                tmem_ld32(tS + W * hf, x);
+            const int k0 = k_begin + j * C::kKeys + W * hf;
             const int hi = min(pos, k_end - 1) - k0, lo = a.window > 0 ? pos - a.window + 1 - k0 : 0;
             float top = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < 64; c++) {
+            for (int c = 0; c < W; c++) {
                 x[c] = c <= hi && c >= lo ? x[c] * a.scale_log2 : -INFINITY;
                 top = fmaxf(top, x[c]);
             }
@@ -1481,7 +1569,7 @@ __global__ void __launch_bounds__(kExThreads, 1) paged_attn_exact_kernel(const _
             m = mn;
             float sum = 0.f;
 #pragma unroll
-            for (int h = 0; h < 4; h++) {
+            for (int h = 0; h < W / 16; h++) {
                 uint32_t w[3][8];
 #pragma unroll
                 for (int c = 0; c < 16; c += 2) {
@@ -1491,8 +1579,8 @@ __global__ void __launch_bounds__(kExThreads, 1) paged_attn_exact_kernel(const _
                     split_terms<__nv_bfloat16, 3>(p0, p1, tt);
                     w[0][c / 2] = tt[0], w[1][c / 2] = tt[1], w[2][c / 2] = tt[2];
                 }
-                tmem_st8(tS + 32 * hf + 8 * h, w[0]);
-                tmem_st8(tS + 64 + 32 * hf + 8 * h, w[1]);
+                tmem_st8(tS + W / 2 * hf + 8 * h, w[0]);
+                tmem_st8(tS + W + W / 2 * hf + 8 * h, w[1]);
                 tmem_st8(tL + 8 * h, w[2]);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -1528,7 +1616,10 @@ __global__ void __launch_bounds__(kExThreads, 1) paged_attn_exact_kernel(const _
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if constexpr (C::kF32)
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        else
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 8) {
             // ------------------------------------------------- products (see the kernel above)
             const unsigned leader = elect_one();
@@ -1539,8 +1630,10 @@ __global__ void __launch_bounds__(kExThreads, 1) paged_attn_exact_kernel(const _
             bool ok = nk > 0 && tc_wait(smem_addr(&q_full), 0u, &failed);
             // K and V come in the order they are used: K0, K1, V0, K2, V1, ...
             auto wait_kv = [&](int push, int j) {
-                ok = ok && tc_wait(smem_addr(&kv_full[push % kExStages]), (unsigned)(push / kExStages) & 1u, &failed);
-                if (!a.box || j * 128 < k_lo || j * 128 + 128 > k_hi) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                ok = ok && tc_wait(smem_addr(&kv_full[push % kStages]), (unsigned)(push / kStages) & 1u, &failed);
+                // rows that came by cp.async, not TMA (the f32 producers put the fence themselves)
+                if (!C::kF32 && (!a.box || j * 128 < k_lo || j * 128 + 128 > k_hi))
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 ok = __all_sync(0xffffffffu, ok);
             };
             int push = 0;
@@ -1548,19 +1641,19 @@ __global__ void __launch_bounds__(kExThreads, 1) paged_attn_exact_kernel(const _
                 wait_kv(push, j);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (ok) {
-                    const unsigned kd = kv_d + (push % kExStages) * (C::kTile >> 4);
-                    // the small terms first
+                    const unsigned kd = kv_d + (push % kStages) * (C::kStage >> 4);
 #pragma unroll
-                    for (int x = 2; x >= 0; x--)
+                    for (int x = 0; x < C::kProducts; x++)
 #pragma unroll
                         for (int h = 0; h < NH; h++)
 #pragma unroll
                             for (int k = 0; k < 4; k++)
-                                mma_ss(leader, utm + 128u * (j & 1), q_d + x * (C::kTile >> 4) + h * (C::kHalf >> 4) + 2 * k,
-                                       kd + h * (C::kHalf >> 4) + 2 * k, kIdS, x < 2 || h > 0 || k > 0);
+                                mma_ss(leader, utm + 128u * (j & 1), q_d + C::left(x) * (C::kQ >> 4) + h * ((128 * 128) >> 4) + 2 * k,
+                                       kd + C::right(x) * (C::kTerm >> 4) + h * (C::kHalf >> 4) + 2 * k, kIdS,
+                                       x > 0 || h > 0 || k > 0);
                 }
                 commit_one(leader, smem_addr(&s_full[j & 1]));
-                commit_one(leader, smem_addr(&kv_empty[push % kExStages]));
+                commit_one(leader, smem_addr(&kv_empty[push % kStages]));
                 push++;
             };
             if (nk > 0) qk(0);
@@ -1572,26 +1665,34 @@ __global__ void __launch_bounds__(kExThreads, 1) paged_attn_exact_kernel(const _
                 ok = __all_sync(0xffffffffu, ok);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (ok) {
-                    const unsigned vd = kv_d + (push % kExStages) * (C::kTile >> 4);
+                    const unsigned vd = kv_d + (push % kStages) * (C::kStage >> 4);
 #pragma unroll
-                    for (int x = 2; x >= 0; x--) {
-                        const unsigned tp = x == 2 ? utm + C::kLow + 64u * (j & 1) : utm + 128u * (j & 1) + 64u * x;
+                    for (int x = 0; x < C::kProducts; x++) {
+                        const unsigned tp = C::left(x) == 2 ? utm + C::kLow + 64u * (j & 1) : utm + 128u * (j & 1) + W * C::left(x);
 #pragma unroll
-                        for (int k = 0; k < 8; k++)
-                            mma_ts(leader, utm + C::kPV, tp + 8u * k, vd + 128 * k, kIdPV, x < 2 || k > 0);
+                        for (int k = 0; k < C::kKeys / 16; k++)
+                            mma_ts(leader, utm + C::kPV, tp + 8u * k, vd + C::right(x) * (C::kTerm >> 4) + 128 * k, kDescVE,
+                                   kIdPV, x > 0 || k > 0);
                     }
                 }
                 commit_one(leader, smem_addr(&pv_full));
-                commit_one(leader, smem_addr(&kv_empty[push % kExStages]));
+                commit_one(leader, smem_addr(&kv_empty[push % kStages]));
                 push++;
             }
             // every product has landed before the tensor memory goes
             if (nk > 0) tc_wait(smem_addr(&pv_full), (unsigned)(nk - 1) & 1u, nullptr);
         } else {
             // ------------------------------------------------- producers
-            KvFeed<D, kExStages> feed{a, &mk, &mv, place, &failed, sb + C::kOffKV, smem_addr(kv_full), smem_addr(kv_empty),
-                                      b, kvh, kr.lo, k_begin, k_end, n, t - (kExThreads - kTcProducers),
-                                      a.box ? 128 / a.box : 0};
+            const int pt = t - 288;
+            auto feed = [&] {
+                if constexpr (C::kF32)
+                    return SplitFeed<D>{a, place, &failed, sb + C::kOffKV, smem_addr(kv_full), smem_addr(kv_empty),
+                                        b, kvh, kr.lo, k_begin, k_end, n, pt};
+                else
+                    return KvFeed<D, kStages>{a, &mk, &mv, place, &failed, sb + C::kOffKV, smem_addr(kv_full),
+                                              smem_addr(kv_empty), b, kvh, kr.lo, k_begin, k_end, n, pt,
+                                              a.box ? 128 / a.box : 0};
+            }();
             feed.look(0);
             feed.look(1);
             if (n > 0) {
@@ -1738,12 +1839,12 @@ Plan make_plan(const PagedView& p, int io, int cache, int heads, int D, int wind
     Plan pl{};
     const int G = heads / p.kv_heads;
     const int64_t most = (int64_t)p.max_new * G, total = (int64_t)p.tokens * G;  // rows of a KV head
-    // Over a 16-bit cache batches that may hold more than 16 rows of a KV head a sequence (8 of f32;
+    // Batches that may hold more than 16 rows of a KV head a sequence (8 of f32;
     // one decoded token's G in any case) run on the tensor cores' tiles of 256 (128) rows, all but the
     // sequences of a token or few.  64 x 4096 keys, bf16: 16 rows 252 us here and 391 there, 32 rows
     // 464 and 344.  One sequence alone takes one kernel for all it may hold.
     const int least = G <= 8 ? 8 : G <= 16 || io == VB_F32 ? 16 : 32, many_rows = io == VB_F32 ? kExRows : kTcRows;
-    const bool tc = cache != VB_F32 && most > (io == VB_F32 ? least : std::max(least, 16));
+    const bool tc = most > (io == VB_F32 ? least : std::max(least, 16));
     pl.few_rows = !tc ? 0x7fffffff : p.batch == 1 ? 0 : least;
     const int64_t few_most = std::min<int64_t>(most, pl.few_rows);
     // rows of a tile: all of a sequence's where that is at most 32 (16 where q takes three terms or
@@ -1829,31 +1930,31 @@ vb_status launch_few(const AttnView& a, cudaStream_t s) {
 template <typename IO, typename KV, int D>
 vb_status launch_attn(const AttnView& a, cudaStream_t s) {
     cudaError_t e;
-    if constexpr (sizeof(KV) == 2) {
-        if (a.few_rows != 0x7fffffff) {
-            const int rows = a.many.rows;
-            const int64_t tiles = std::min<int64_t>((int64_t)a.p.batch * (((int64_t)a.p.max_new * a.group + rows - 1) / rows),
-                                                    (int64_t)a.p.tokens * a.group / rows + a.p.batch);
-            const int64_t grid = tiles * a.many.splits * a.p.kv_heads;
-            if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
-            AttnView b = a;
-            CUtensorMap mk{}, mv{};
+    if (a.few_rows != 0x7fffffff) {
+        const int rows = a.many.rows;
+        const int64_t tiles = std::min<int64_t>((int64_t)a.p.batch * (((int64_t)a.p.max_new * a.group + rows - 1) / rows),
+                                                (int64_t)a.p.tokens * a.group / rows + a.p.batch);
+        const int64_t grid = tiles * a.many.splits * a.p.kv_heads;
+        if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
+        AttnView b = a;
+        CUtensorMap mk{}, mv{};
+        if constexpr (sizeof(KV) == 2) {
             b.box = page_map(a.p, a.p.k, D, std::is_same<KV, __half>::value, &mk);
             if (b.box && !page_map(a.p, a.p.v, D, std::is_same<KV, __half>::value, &mv)) b.box = 0;
-            static std::atomic<unsigned long long> done{0};
-            if constexpr (sizeof(IO) == 4) {
-                e = smem_attr_once(paged_attn_exact_kernel<D>, ExCfg<D>::kSmem, done);
-                if (e == cudaSuccess)
-                    e = launch_pdl(paged_attn_exact_kernel<D>, dim3((unsigned)grid), dim3(kExThreads), ExCfg<D>::kSmem, s, b,
-                                   mk, mv);
-            } else {
-                e = smem_attr_once(paged_attn_tc_kernel<IO, D>, TcCfg<D>::kSmem, done);
-                if (e == cudaSuccess)
-                    e = launch_pdl(paged_attn_tc_kernel<IO, D>, dim3((unsigned)grid), dim3(kTcThreads), TcCfg<D>::kSmem, s,
-                                   b, mk, mv);
-            }
-            if (e != cudaSuccess) return cuda_fail(e, "paged attention, many rows");
         }
+        static std::atomic<unsigned long long> done{0};
+        if constexpr (sizeof(IO) == 4) {
+            using C = ExCfg<KV, D>;
+            e = smem_attr_once(paged_attn_exact_kernel<KV, D>, C::kSmem, done);
+            if (e == cudaSuccess)
+                e = launch_pdl(paged_attn_exact_kernel<KV, D>, dim3((unsigned)grid), dim3(C::kThreads), C::kSmem, s, b, mk, mv);
+        } else {
+            e = smem_attr_once(paged_attn_tc_kernel<IO, D>, TcCfg<D>::kSmem, done);
+            if (e == cudaSuccess)
+                e = launch_pdl(paged_attn_tc_kernel<IO, D>, dim3((unsigned)grid), dim3(kTcThreads), TcCfg<D>::kSmem, s, b, mk,
+                               mv);
+        }
+        if (e != cudaSuccess) return cuda_fail(e, "paged attention, many rows");
     }
     if (a.few_rows) {
         AttnView f = a;
