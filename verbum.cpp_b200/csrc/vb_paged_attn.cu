@@ -77,10 +77,8 @@ struct AttnView {
     float scale_log2;   // scale * log2(e): the softmax runs in base 2
     int window;
     int few_rows;       // sequences with at most this many rows a KV head run in the few-rows kernel
-    int row_tiles;      // its row tiles of a sequence
-    bool cluster;       // a cluster of blocks for each tile (one row tile a sequence, few and short)
-    int stream;         // blocks that share all its keys evenly (one row tile a sequence); 0: a block per tile and split
     Cut few, many;
+    int stream;         // blocks that share all keys of the few-rows kernel evenly; 0: clusters of blocks, one a tile
     bool after_many;    // the few-rows kernel of this call follows its many-rows kernel
     int box;            // rows of a page that one TMA copy brings (many rows); 0: no tensor maps
     float* part;        // [split][token][head][D] sums of a split, relative to its maximum
@@ -277,17 +275,15 @@ struct FewCfg {
 // accumulation truncates, which over thousands of keys would show.
 // Where a piece of a tile's keys leaves its rows: the output, or sums to be joined.
 struct Sink {
-    bool last;       // the piece is the whole tile
-    float* part;     // row `row` of the tile at part + row_of(row) * D
+    bool last;       // the piece is the whole tile: the output
+    bool keep;       // the sums stay in shared memory, row `row` at row * (D + 4), its (m, l) in kept
+    float* part;     // else: row `row`'s sums at part + row * D, its (m, l) at ml + row
     float2* ml;
-    int64_t base;    // row_of: split * tokens * heads + token * heads + head, or (by_row) the tile's row
-    bool by_row;
-    bool keep;       // neither: the sums stay in shared memory, row `row` at row * (D + 4), its (m, l) in kept
 };
 
-// Rows r0 .. of KV head kvh of sequence b over keys k_begin .. k_end - 1, by the block.
+// The rows of KV head kvh of sequence b over keys k_begin .. k_end - 1, by the block.
 template <typename IO, typename KV, int D, int NR>
-__device__ __forceinline__ void few_piece(const AttnView& a, const PagedSeq& s, int b, int kvh, int r0, const KeyRange& kr,
+__device__ __forceinline__ void few_piece(const AttnView& a, const PagedSeq& s, int b, int kvh, const KeyRange& kr,
                                           int k_begin, int k_end, const Sink& sink, char* smem,
                                           float2 (*ml)[8 * NR], float2* kept = nullptr) {
     using C = FewCfg<KV, D, NR>;
@@ -337,7 +333,7 @@ __device__ __forceinline__ void few_piece(const AttnView& a, const PagedSeq& s, 
     uint32_t qh[kF32 ? 1 : NR][NK][NT][2];
 #pragma unroll
     for (int n = 0; n < NR; n++) {
-        const int r = min(r0 + 8 * n + g, rows - 1);
+        const int r = min(8 * n + g, rows - 1);
         const char* qp = a.q + (int64_t)(s.start + r / a.group) * a.q_row + (int64_t)(kvh * a.group + r % a.group) * a.q_head;
 #pragma unroll
         for (int kk = 0; kk < NK; kk++) {
@@ -369,7 +365,7 @@ __device__ __forceinline__ void few_piece(const AttnView& a, const PagedSeq& s, 
     for (int n = 0; n < NR; n++) {
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            const int r = r0 + 8 * n + 2 * t4 + e;
+            const int r = 8 * n + 2 * t4 + e;
             pos[n][e] = r < rows ? s.len - s.n + r / a.group : -1;
             m[n][e] = -INFINITY;
             l[n][e] = 0.f;
@@ -568,8 +564,8 @@ __device__ __forceinline__ void few_piece(const AttnView& a, const PagedSeq& s, 
             }
     __syncthreads();
     for (int it = threadIdx.x; it < C::kRows * (D / 8); it += C::kWarps * 32) {
-        const int row = it / (D / 8), r = r0 + row, d = it % (D / 8) * 8;
-        if (r >= rows) break;
+        const int row = it / (D / 8), d = it % (D / 8) * 8;
+        if (row >= rows) break;
         float M = -INFINITY, L = 0.f;
         float y[8] = {};
 #pragma unroll
@@ -583,7 +579,7 @@ __device__ __forceinline__ void few_piece(const AttnView& a, const PagedSeq& s, 
 #pragma unroll
             for (int e = 0; e < 8; e++) y[e] = fmaf(w, z[e], y[e]);
         }
-        const int token = s.start + r / a.group, head = kvh * a.group + r % a.group;
+        const int token = s.start + row / a.group, head = kvh * a.group + row % a.group;
         const int64_t th = (int64_t)token * a.heads + head;
         if (sink.keep) {
             Eight<float>::store(sums + row * C::kLd + d, y);  // (over what this thread alone has read)
@@ -595,9 +591,8 @@ __device__ __forceinline__ void few_piece(const AttnView& a, const PagedSeq& s, 
             Eight<IO>::store(a.out + token * a.o_row + head * a.o_head + d * sizeof(IO), y);
             if (d == 0 && a.lse) a.lse[th] = L > 0.f ? (M + log2f(L)) * 0.693147180559945309f : -INFINITY;
         } else {
-            const int64_t at = sink.base + (sink.by_row ? row : th);
-            Eight<float>::store(sink.part + at * D + d, y);
-            if (d == 0) sink.ml[at] = make_float2(M, L);
+            Eight<float>::store(sink.part + row * D + d, y);
+            if (d == 0) sink.ml[row] = make_float2(M, L);
         }
     }
 }
@@ -611,13 +606,12 @@ __device__ __forceinline__ float4 cl_ld4(unsigned addr) {
     return v;
 }
 
-// How the kernel's blocks share the work: a grid of (split, KV head, row tile, sequence) in
-// one axis; the keys of all tiles shared out evenly; or a cluster of 8 blocks for a tile,
-// which join their pieces through each other's shared memory (no second launch).
-enum FewMode { kGrid, kStream, kCluster };
+// CLUSTER: a cluster of 8 blocks for a tile (sequence, KV head), which join their pieces
+// through each other's shared memory (no second launch).  Else the keys of all tiles are
+// shared out evenly over the blocks.
 constexpr int kCl = 8;
 
-template <typename IO, typename KV, int D, int NR, int MODE>
+template <typename IO, typename KV, int D, int NR, bool CLUSTER>
 __global__ void __launch_bounds__(FewCfg<KV, D, NR>::kWarps * 32) paged_attn_few_kernel(const __grid_constant__ AttnView a) {
     using C = FewCfg<KV, D, NR>;
     extern __shared__ __align__(1024) char smem[];
@@ -633,7 +627,7 @@ __global__ void __launch_bounds__(FewCfg<KV, D, NR>::kWarps * 32) paged_attn_few
             if (wait) pdl_wait();
         }
     } at_end{a.after_many};
-    if constexpr (MODE == kCluster) {
+    if constexpr (CLUSTER) {
         __shared__ float2 kept[C::kRows];
         const int rank = (int)cl_rank(), tile = (int)blockIdx.x / kCl;
         const int kvh = tile % a.p.kv_heads, b = tile / a.p.kv_heads;
@@ -643,8 +637,8 @@ __global__ void __launch_bounds__(FewCfg<KV, D, NR>::kWarps * 32) paged_attn_few
         const KeyRange kr = key_range(a, s, 0, a.few);
         const int n = (kr.hi - kr.base + kBK - 1) / kBK;  // blocks of 16 keys
         const int k_begin = kr.base + n * rank / kCl * kBK, k_end = min(kr.base + n * (rank + 1) / kCl * kBK, kr.hi);
-        const Sink sink{false, nullptr, nullptr, 0, false, true};
-        few_piece<IO, KV, D, NR>(a, s, b, kvh, 0, kr, k_begin, k_end, sink, smem, ml, kept);
+        const Sink sink{false, true, nullptr, nullptr};
+        few_piece<IO, KV, D, NR>(a, s, b, kvh, kr, k_begin, k_end, sink, smem, ml, kept);
         cluster_sync_all();
         for (int it = rank * C::kWarps * 32 + threadIdx.x; it < C::kRows * (D / 4); it += kCl * C::kWarps * 32) {
             const int row = it / (D / 4), d = it % (D / 4) * 4;
@@ -673,21 +667,6 @@ __global__ void __launch_bounds__(FewCfg<KV, D, NR>::kWarps * 32) paged_attn_few
                 a.lse[(int64_t)token * a.heads + head] = L > 0.f ? (M + log2f(L)) * 0.693147180559945309f : -INFINITY;
         }
         cluster_sync_all();  // no block leaves while others read its shared memory
-    } else if constexpr (MODE == kGrid) {
-        int64_t idx = blockIdx.x;
-        const int split = (int)(idx % a.few.splits);
-        idx /= a.few.splits;
-        const int kvh = (int)(idx % a.p.kv_heads);
-        idx /= a.p.kv_heads;
-        const int r0 = (int)(idx % a.row_tiles) * C::kRows, b = (int)(idx / a.row_tiles);
-        const PagedSeq s = paged_seq(a.p, b);
-        const int rows = s.n * a.group;
-        if (r0 >= rows || rows > a.few_rows) return;
-        const KeyRange kr = key_range(a, s, r0, a.few);
-        if (split >= splits_used(a.few, kr)) return;
-        const int k_begin = kr.base + split * a.few.len;
-        const Sink sink{a.few.splits == 1, a.part, a.part_ml, (int64_t)split * a.p.tokens * a.heads, false, false};
-        few_piece<IO, KV, D, NR>(a, s, b, kvh, r0, kr, k_begin, min(k_begin + a.few.len, kr.hi), sink, smem, ml);
     } else {
         // this block's units, piece by piece: a piece is what it has of one tile
         const int lane = threadIdx.x & 31;
@@ -732,9 +711,10 @@ __global__ void __launch_bounds__(FewCfg<KV, D, NR>::kWarps * 32) paged_attn_few
             const KeyRange kr = key_range(a, s, 0, a.few);
             const int kvh = off / n, first = off % n, take = min(n - first, u_end - u);
             const int slot = first > 0 ? 0 : 1;  // a tile begun by an earlier block; begun here
-            const Sink sink{take == n, a.strm, a.strm_ml, ((int64_t)blockIdx.x * 2 + slot) * C::kRows, true, false};
+            const int64_t at = ((int64_t)blockIdx.x * 2 + slot) * C::kRows;
+            const Sink sink{take == n, false, a.strm + at * D, a.strm_ml + at};
             const int k_begin = kr.base + first * kUnit;
-            few_piece<IO, KV, D, NR>(a, s, b, kvh, 0, kr, k_begin, min(k_begin + take * kUnit, kr.hi), sink, smem, ml);
+            few_piece<IO, KV, D, NR>(a, s, b, kvh, kr, k_begin, min(k_begin + take * kUnit, kr.hi), sink, smem, ml);
             u += take;
             off += take;
             __syncthreads();  // the shared memory is free for the next piece
@@ -1717,7 +1697,7 @@ __global__ void __launch_bounds__(ExCfg<KV, D>::kThreads, 1)
     if (t == 0 && failed) paged_report(a.p, VB_PAGED_TIMEOUT);
 }
 
-// Joins the splits of a row: a warp per (token, head), grid over them.
+// Joins the splits of a row of the many-rows kernels: a warp per (token, head).
 template <typename IO, int D>
 __global__ void __launch_bounds__(128) paged_attn_merge_kernel(const __grid_constant__ AttnView a) {
     pdl_wait();
@@ -1730,9 +1710,8 @@ __global__ void __launch_bounds__(128) paged_attn_merge_kernel(const __grid_cons
     const PagedSeq s = paged_seq(a.p, b);
     if (!s.ok || token < s.start || token >= s.start + s.n) return;
     const int r = (token - s.start) * a.group + head % a.group;
-    const Cut& cut = s.n * a.group > a.few_rows ? a.many : a.few;
-    if (cut.splits == 1) return;  // written by the kernel itself
-    const int used = splits_used(cut, key_range(a, s, r / cut.rows * cut.rows, cut));
+    if (s.n * a.group <= a.few_rows) return;
+    const int used = splits_used(a.many, key_range(a, s, r / a.many.rows * a.many.rows, a.many));
     const int64_t step = (int64_t)a.p.tokens * a.heads;
     constexpr int E = D / 32;
     float y[E] = {}, M = -INFINITY, L = 0.f;
@@ -1818,70 +1797,52 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const 
 // launch holds for any lengths within them.  A tile's keys are split where the
 // tiles alone do not fill the card.
 struct Plan {
-    int few_rows, row_tiles, stream;
-    bool cluster;
+    int few_rows, stream;
     Cut few, many;
     int max_splits;  // for any window
 };
 constexpr int kStreamMost = 148 * 3;  // blocks that share out a batch's keys
 
-Cut make_cut(int rows, int align, int64_t keys, int64_t want, int step, int least) {
-    Cut c;
-    c.rows = rows;
-    c.align = align;
-    const int64_t n = std::max<int64_t>(1, std::min<int64_t>(want, (keys + least - 1) / least));
-    c.len = (int)(((keys + n - 1) / n + step - 1) / step * step);
-    c.splits = (int)((keys + c.len - 1) / c.len);
-    return c;
-}
-
 Plan make_plan(const PagedView& p, int io, int cache, int heads, int D, int window) {
     Plan pl{};
     const int G = heads / p.kv_heads;
     const int64_t most = (int64_t)p.max_new * G, total = (int64_t)p.tokens * G;  // rows of a KV head
-    // Batches that may hold more than 16 rows of a KV head a sequence (8 of f32;
-    // one decoded token's G in any case) run on the tensor cores' tiles of 256 (128) rows, all but the
-    // sequences of a token or few.  64 x 4096 keys, bf16: 16 rows 252 us here and 391 there, 32 rows
-    // 464 and 344.  One sequence alone takes one kernel for all it may hold.
+    // Batches that may hold more than 16 rows of a KV head a sequence (8 of f32; one decoded token's G
+    // in any case) run on the tensor cores' tiles of 256 (128) rows, all but the sequences of a token
+    // or few.  64 x 4096 keys, bf16: 16 rows 252 us here and 391 there, 32 rows 464 and 344.  One
+    // sequence alone takes one kernel for all it may hold.
     const int least = G <= 8 ? 8 : G <= 16 || io == VB_F32 ? 16 : 32, many_rows = io == VB_F32 ? kExRows : kTcRows;
     const bool tc = most > (io == VB_F32 ? least : std::max(least, 16));
     pl.few_rows = !tc ? 0x7fffffff : p.batch == 1 ? 0 : least;
-    const int64_t few_most = std::min<int64_t>(most, pl.few_rows);
-    // rows of a tile: all of a sequence's where that is at most 32 (16 where q takes three terms or
-    // 32 bits: more do not fit the registers)
-    const int tile = few_most <= 8 ? 8 : few_most <= 16 || io == VB_F32 ? 16 : 32;
-    pl.row_tiles = (int)((few_most + tile - 1) / tile);
     const int64_t all = std::max(p.max_len, 1);
     // keys from a tile's base (its first row's lowest, rounded down) to its last row's
     auto span = [&](int rows, int align) {
         return window > 0 ? std::min<int64_t>(all, (int64_t)window + (rows + G - 1) / G + align - 1) : all;
     };
-    // few rows: where a sequence's rows are one tile its keys are shared out evenly over as many
-    // blocks as the card runs at a time; else about four CTAs for each SM of at least 64 keys (one
-    // block of 16 a warp).  Many: one CTA for each SM of at least 512 keys.
-    const int64_t tiles = std::max<int64_t>(1, std::min<int64_t>((int64_t)p.batch * pl.row_tiles, total / tile + p.batch));
-    const int64_t want = pl.row_tiles == 1 ? 1 : std::max<int64_t>(1, 148 * 4 / (tiles * p.kv_heads));
-    if (pl.row_tiles == 1) {
-        const int64_t most_units = (int64_t)p.batch * p.kv_heads * ((span(tile, 16) + kUnit - 1) / kUnit);
-        if (most_units > 0x3fffffff) return pl;  // (the caller refuses)
-        // Clusters where all fit the card at once and a block's share is at most 512 keys: one token
-        // of one sequence of 777 keys takes one launch and 7.2 us of its caller instead of two and 9.8.
-        pl.cluster = (int64_t)p.batch * p.kv_heads * kCl <= 148 * 2 && span(tile, 16) <= kCl * 512;
-        pl.stream = (int)std::min<int64_t>(cache == VB_F32 && D == 128 ? 148 : kStreamMost, most_units);
-    }
-    pl.few = make_cut(tile, 16, span(tile, 16), want, 64, 64);
-    const int64_t tiles2 = std::max<int64_t>(1, (total + many_rows - 1) / many_rows);
-    const int64_t want2 = std::max<int64_t>(1, 148 / (tiles2 * p.kv_heads));
-    pl.many = make_cut(many_rows, 128, span(many_rows, 128), want2, 128, 512);
-    pl.max_splits = (int)std::max<int64_t>(pl.few_rows ? std::min<int64_t>(want, (all + 63) / 64) : 1,
-                                           tc ? std::min<int64_t>(want2, (all + 511) / 512) : 1);
-    if (!tc) pl.many.splits = 1;
-    if (!pl.few_rows) pl.few.splits = 1;
+    // few rows: one tile holds all of a sequence's
+    const int64_t few_most = std::min<int64_t>(most, pl.few_rows);
+    pl.few = Cut{few_most <= 8 ? 8 : few_most <= 16 ? 16 : 32, 1, 0, 16};
+    const int64_t keys = span(pl.few.rows, 16);
+    // Clusters where all fit the card at once and a block's share is at most 512 keys: one token of
+    // one sequence of 777 keys takes one launch and 7.2 us of its caller instead of two and 9.8.
+    // Else as many blocks as the card runs at a time.
+    if ((int64_t)p.batch * p.kv_heads * kCl > 148 * 2 || keys > kCl * 512)
+        pl.stream = (int)std::min<int64_t>(cache == VB_F32 && D == 128 ? 148 : kStreamMost,
+                                           (int64_t)p.batch * p.kv_heads * ((keys + kUnit - 1) / kUnit));
+    // many rows: one CTA for each SM, of at least 512 keys
+    const int64_t tiles = std::max<int64_t>(1, (total + many_rows - 1) / many_rows);
+    const int64_t want = std::max<int64_t>(1, 148 / (tiles * p.kv_heads));
+    const int64_t span_many = span(many_rows, 128);
+    const int64_t n = tc ? std::min<int64_t>(want, (span_many + 511) / 512) : 1;
+    pl.many = Cut{many_rows, 1, (int)(((span_many + n - 1) / n + 127) / 128 * 128), 128};
+    pl.many.splits = (int)((span_many + pl.many.len - 1) / pl.many.len);
+    pl.max_splits = tc ? (int)std::min<int64_t>(want, (all + 511) / 512) : 1;
     return pl;
 }
+// The workspace: first the shared-out tiles' pieces, then the splits'.
+size_t stream_floats(const Plan& pl, int D) { return pl.few_rows ? (size_t)kStreamMost * 2 * pl.few.rows * (D + 2) : 0; }
 size_t plan_bytes(const Plan& pl, const PagedView& p, int heads, int D) {
-    return (pl.max_splits > 1 ? (size_t)pl.max_splits * p.tokens * heads * (D + 2) * 4 : 0) +
-           (pl.row_tiles == 1 ? (size_t)kStreamMost * 2 * pl.few.rows * (D + 2) * 4 : 0);
+    return 4 * (stream_floats(pl, D) + (pl.max_splits > 1 ? (size_t)pl.max_splits * p.tokens * heads * (D + 2) : 0));
 }
 
 // Tensor map of a pool as [page][kv head][position][dim], boxes of one page's rows (128 at
@@ -1903,28 +1864,23 @@ int page_map(const PagedView& p, const char* base, int D, bool half, CUtensorMap
     return r == CUDA_SUCCESS ? box : 0;
 }
 
-template <typename IO, typename KV, int D, int NR, int MODE>
-vb_status launch_few(const AttnView& a, cudaStream_t s) {
-    using C = FewCfg<KV, D, NR>;
-    static std::atomic<unsigned long long> done{0};
-    cudaError_t e = smem_attr_once(paged_attn_few_kernel<IO, KV, D, NR, MODE>, C::kSmem, done);
-    if (e != cudaSuccess) return cuda_fail(e, "paged attention: shared memory attribute");
-    if (MODE == kCluster) {
-        const int64_t blocks = (int64_t)a.p.batch * a.p.kv_heads * kCl;
-        e = launch_pdl_cluster(paged_attn_few_kernel<IO, KV, D, NR, MODE>, dim3((unsigned)blocks), dim3(C::kWarps * 32),
-                               C::kSmem, dim3(kCl, 1, 1), s, a);
-        return e == cudaSuccess ? VB_OK : cuda_fail(e, "paged_attn_few_kernel");
-    }
-    const int64_t grid = MODE == kStream ? a.stream : (int64_t)a.few.splits * a.p.kv_heads * a.row_tiles * a.p.batch;
-    if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
-    e = launch_pdl(paged_attn_few_kernel<IO, KV, D, NR, MODE>, dim3((unsigned)grid), dim3(C::kWarps * 32), C::kSmem, s, a);
-    return e == cudaSuccess ? VB_OK : cuda_fail(e, "paged_attn_few_kernel");
-}
-
 template <typename IO, typename KV, int D, int NR>
 vb_status launch_few(const AttnView& a, cudaStream_t s) {
-    if (a.cluster) return launch_few<IO, KV, D, NR, kCluster>(a, s);
-    return a.stream ? launch_few<IO, KV, D, NR, kStream>(a, s) : launch_few<IO, KV, D, NR, kGrid>(a, s);
+    using C = FewCfg<KV, D, NR>;
+    static std::atomic<unsigned long long> done[2];
+    const dim3 block(C::kWarps * 32);
+    cudaError_t e;
+    if (a.stream) {
+        e = smem_attr_once(paged_attn_few_kernel<IO, KV, D, NR, false>, C::kSmem, done[0]);
+        if (e == cudaSuccess)
+            e = launch_pdl(paged_attn_few_kernel<IO, KV, D, NR, false>, dim3(a.stream), block, C::kSmem, s, a);
+    } else {
+        e = smem_attr_once(paged_attn_few_kernel<IO, KV, D, NR, true>, C::kSmem, done[1]);
+        if (e == cudaSuccess)
+            e = launch_pdl_cluster(paged_attn_few_kernel<IO, KV, D, NR, true>, dim3(a.p.batch * a.p.kv_heads * kCl), block,
+                                   C::kSmem, dim3(kCl, 1, 1), s, a);
+    }
+    return e == cudaSuccess ? VB_OK : cuda_fail(e, "paged_attn_few_kernel");
 }
 
 template <typename IO, typename KV, int D>
@@ -1962,10 +1918,10 @@ vb_status launch_attn(const AttnView& a, cudaStream_t s) {
         vb_status st = VB_OK;
         if (a.few.rows == 8) {
             st = launch_few<IO, KV, D, 1>(f, s);
-        } else if (sizeof(IO) == 4 || a.few.rows == 16) {
+        } else if (a.few.rows == 16) {
             st = launch_few<IO, KV, D, 2>(f, s);
         } else {
-            if constexpr (sizeof(IO) == 2) st = launch_few<IO, KV, D, 4>(f, s);
+            if constexpr (sizeof(IO) == 2) st = launch_few<IO, KV, D, 4>(f, s);  // (f32: 16 rows at most)
         }
         if (st) return st;
     }
@@ -1976,7 +1932,7 @@ vb_status launch_attn(const AttnView& a, cudaStream_t s) {
         e = launch_pdl(paged_attn_join_kernel<IO, D>, dim3((unsigned)grid), dim3(kJoinWarps * 32), 0, s, a, rows);
         if (e != cudaSuccess) return cuda_fail(e, "paged_attn_join_kernel");
     }
-    if (a.few.splits > 1 || a.many.splits > 1) {
+    if (a.many.splits > 1) {
         const int64_t grid = ((int64_t)a.p.tokens * a.heads + 3) / 4;
         if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
         e = launch_pdl(paged_attn_merge_kernel<IO, D>, dim3((unsigned)grid), dim3(128), 0, s, a);
@@ -2023,7 +1979,9 @@ extern "C" vb_status vb_paged_attn(const vb_paged_cache* cache, const vb_paged_b
     if (!paged_aligned(q, q_row, q_head, es) || !paged_aligned(out, o_row, o_head, es) || !paged_aligned(workspace, 0, 0, 1))
         return fail(VB_ERR_UNSUPPORTED, "paged_attn: 16-byte alignment required");
     const Plan pl = make_plan(a.p, io, cache->dtype, heads, D, window);
-    if (pl.row_tiles == 1 && !pl.stream) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many keys");
+    // the units of shared-out keys are counted in 32 bits
+    if ((int64_t)a.p.batch * a.p.kv_heads * ((int64_t)a.p.max_len / kUnit + 1) > 0x3fffffff)
+        return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many keys");
     const size_t need = plan_bytes(pl, a.p, heads, D);
     if (need > workspace_bytes || (need && !workspace))
         return fail(VB_ERR_ARG, "paged_attn: the workspace is too small");
@@ -2037,19 +1995,13 @@ extern "C" vb_status vb_paged_attn(const vb_paged_cache* cache, const vb_paged_b
     a.scale_log2 = (scale == 0.f ? 1.17549435e-38f : scale) * 1.44269504088896341f;
     a.window = window;
     a.few_rows = pl.few_rows;
-    a.row_tiles = pl.row_tiles;
-    a.cluster = pl.cluster;
-    a.stream = pl.cluster ? 0 : pl.stream;
     a.few = pl.few;
     a.many = pl.many;
-    float* w = static_cast<float*>(workspace);
-    if (pl.row_tiles == 1) {
-        const size_t parts = (size_t)kStreamMost * 2 * pl.few.rows;
-        a.strm = w;
-        a.strm_ml = reinterpret_cast<float2*>(w + parts * D);
-        w += parts * (D + 2);
-    }
-    a.part = w;
+    a.stream = pl.stream;
+    const size_t parts = (size_t)kStreamMost * 2 * pl.few.rows;
+    a.strm = static_cast<float*>(workspace);
+    a.strm_ml = reinterpret_cast<float2*>(a.strm + parts * D);
+    a.part = a.strm + stream_floats(pl, D);
     a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)pl.max_splits * a.p.tokens * heads * D);
     return D == 128 ? launch_attn<128>(a, io, cache->dtype, as_stream(stream))
                     : launch_attn<64>(a, io, cache->dtype, as_stream(stream));
