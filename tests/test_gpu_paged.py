@@ -462,6 +462,82 @@ def test_offsets_past_32_bits(io, cache):
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("io,cache", PAIRS)
+@pytest.mark.parametrize("n", [1, 3, 20, 200])
+def test_a_nan_in_a_query_stays_in_its_row(io, cache, n):
+    s = Setup([n, 1, n], [300, 77, 250], io, cache, seed=n)
+    want, lse = check_attn(s), None
+    s.q[n // 2, 1, 5] = float("nan")
+    s.q[n, 2, 0] = float("inf")
+    out, lse = s.out(), torch.zeros(s.T, s.H, device="cuda")
+    vb200.paged_attn(s.pc, s.pb, s.q, out, lse=lse)
+    for t, h in ((n // 2, 1), (n, 2)):
+        assert torch.isnan(out[t, h]).all() and torch.isnan(lse[t, h])
+        out[t, h] = want[t, h]
+    assert torch.equal(out, want)
+
+
+def test_windows_beyond_every_position():
+    s = Setup([1, 5, 40], [90, 3, 200], "bf16", "bf16", seed=14)
+    want = check_attn(s)
+    for window in (200, 201, 2**31 - 1, 2**40):
+        out = s.out()
+        vb200.paged_attn(s.pc, s.pb, s.q, out, window=window)
+        assert torch.equal(out, want)
+    with pytest.raises(vb200.VBError):
+        vb200.paged_attn(s.pc, s.pb, s.q, out, window=-1)
+    with pytest.raises(vb200.VBError):  # a workspace of the call's own, on a stream that is not the current one
+        vb200.paged_attn(s.pc, s.pb, s.q, out, stream=torch.cuda.Stream().cuda_stream)
+
+
+@pytest.mark.parametrize("io,cache", PAIRS)
+def test_thousands_of_sequences(io, cache):
+    B = 2100
+    news = [1 if b % 3 else 0 for b in range(B)]
+    news[700] = 1
+    s = Setup(news, [n + (b * 13) % 90 for b, n in enumerate(news)], io, cache, H=4, KVH=2, D=64, seed=1)
+    check_attn(s)
+
+
+@pytest.mark.parametrize("io,cache", PAIRS)
+def test_a_captured_mixed_batch(io, cache):
+    """The kernels of a call that run beside each other, captured with the append before and replayed."""
+    B = 45
+    news = [100 if b % 15 == 2 else 1 for b in range(B)]
+    lens = [n + (b * 97) % 600 for b, n in enumerate(news)]
+    s = Setup(news, lens, io, cache, H=16, KVH=8, seed=77)
+    s.table.clamp_(min=0)
+    cos, sin = tables(max(lens), 128)
+    q, out = s.out(), s.out()
+    ws = vb200.paged_attn_workspace(s.pc, s.pb, s.H)
+
+    def step():
+        vb200.paged_append(s.pc, s.pb, s.kn, s.vn, q=s.q, q_out=q, cos=cos, sin=sin)
+        vb200.paged_attn(s.pc, s.pb, q, out, workspace=ws)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    s.k.copy_(torch.randn(s.k.shape, device="cuda"))
+    s.v.copy_(torch.randn(s.v.shape, device="cuda"))
+    for _ in range(4):
+        for x in (s.q, s.kn, s.vn):
+            x.copy_(torch.randn(x.shape, device="cuda"))
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        keep, s.q = s.q, q
+        ref, _, tol, _ = attn_reference(s)
+        s.q = keep
+        assert ((out.double() - ref).abs() <= tol).all()
+    assert int(s.status) == 0
+
+
 # ------------------------------------------------- as a user runs them together
 
 def test_captured_step_replays_with_new_lengths():

@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kLgThreads) logits_process_kernel(const __grid
             reinterpret_cast<float4*>(bias)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     __syncthreads();
     if (count) {
-        const int answer = h0 + (a.r.prompt_len ? max(a.r.prompt_len[row], 0) : 0);
+        const int answer = h0 + (a.r.prompt_len ? min(max(a.r.prompt_len[row], 0), h1 - h0) : 0);
         for (int i0 = h0; i0 < h1; i0 += NH * kLgThreads) {
             int next[NH];
 #pragma unroll
@@ -226,6 +226,8 @@ extern "C" vb_status vb_logits_process(const void* logits, int64_t stride_in, vo
         return fail(VB_ERR_ARG, "logits_process: in place needs equal strides");
     const vb_logits_rules& r = *rules;
     if (r.hist_total < 0 || r.bias_total < 0) return fail(VB_ERR_ARG, "logits_process: negative size");
+    if (r.hist_total > 0x70000000ll || r.bias_total > 0x70000000ll)
+        return fail(VB_ERR_UNSUPPORTED, "logits_process: lists are counted in 32 bits");
     if ((r.repetition || r.frequency || r.presence) && !r.hist_start)
         return fail(VB_ERR_ARG, "logits_process: penalties need a history");
     if ((r.hist_start && r.hist_total && !r.hist_ids) ||

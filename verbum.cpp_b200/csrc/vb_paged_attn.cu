@@ -117,12 +117,13 @@ __device__ __forceinline__ int stream_units(const AttnView& a, int b) {
                     (int64_t)s.n * a.group <= a.few_rows;
     return ok ? max(1, (k.hi - k.base + kUnit - 1) / kUnit) : 0;
 }
-// Units of all sequences, and of those before sequence b; by the whole warp.  (The host
-// sees to it that they fit 32 bits.)
-__device__ __forceinline__ void stream_sums(const AttnView& a, int b, int lane, int& all, int& before) {
+// Units of all sequences, and of those before sequence b; by the whole block of WARPS warps.
+// (The host sees to it that they fit 32 bits.)
+template <int WARPS>
+__device__ __forceinline__ void stream_sums(const AttnView& a, int b, int& all, int& before) {
+    __shared__ int2 sums[WARPS];
     int x = 0, y = 0;
-#pragma unroll 2
-    for (int i = lane; i < a.p.batch; i += 32) {
+    for (int i = threadIdx.x; i < a.p.batch; i += WARPS * 32) {
         const int u = stream_units(a, i);
         x += u;
         if (i < b) y += u;
@@ -132,6 +133,11 @@ __device__ __forceinline__ void stream_sums(const AttnView& a, int b, int lane, 
         x += __shfl_xor_sync(0xffffffffu, x, o);
         y += __shfl_xor_sync(0xffffffffu, y, o);
     }
+    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = make_int2(x, y);
+    __syncthreads();
+    x = y = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) x += sums[w].x, y += sums[w].y;
     all = x * a.p.kv_heads;
     before = y * a.p.kv_heads;
 }
@@ -585,11 +591,11 @@ __device__ __forceinline__ void few_piece(const AttnView& a, const PagedSeq& s, 
             Eight<float>::store(sums + row * C::kLd + d, y);  // (over what this thread alone has read)
             if (d == 0) kept[row] = make_float2(M, L);
         } else if (sink.last) {
-            const float inv = L > 0.f ? 1.f / L : 0.f;
+            const float inv = 1.f / L;
 #pragma unroll
-            for (int e = 0; e < 8; e++) y[e] *= inv;
+            for (int e = 0; e < 8; e++) y[e] = L == 0.f ? 0.f : y[e] * inv;  // (a sum that is NaN stays one)
             Eight<IO>::store(a.out + token * a.o_row + head * a.o_head + d * sizeof(IO), y);
-            if (d == 0 && a.lse) a.lse[th] = L > 0.f ? (M + log2f(L)) * 0.693147180559945309f : -INFINITY;
+            if (d == 0 && a.lse) a.lse[th] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
         } else {
             Eight<float>::store(sink.part + row * D + d, y);
             if (d == 0) sink.ml[row] = make_float2(M, L);
@@ -659,12 +665,14 @@ __global__ void __launch_bounds__(FewCfg<KV, D, NR>::kWarps * 32) paged_attn_few
                 L = fmaf(q[c].y, w, L);
                 y.x = fmaf(w, z.x, y.x), y.y = fmaf(w, z.y, y.y), y.z = fmaf(w, z.z, y.z), y.w = fmaf(w, z.w, y.w);
             }
-            const float inv = L > 0.f ? 1.f / L : 0.f;
+            const float inv = 1.f / L;
+            if (L == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
             const int token = s.start + row / a.group, head = kvh * a.group + row % a.group;
             IO* dst = reinterpret_cast<IO*>(a.out + token * a.o_row + head * a.o_head) + d;
-            dst[0] = (IO)(y.x * inv), dst[1] = (IO)(y.y * inv), dst[2] = (IO)(y.z * inv), dst[3] = (IO)(y.w * inv);
+            if (L != 0.f) y.x *= inv, y.y *= inv, y.z *= inv, y.w *= inv;
+            dst[0] = (IO)y.x, dst[1] = (IO)y.y, dst[2] = (IO)y.z, dst[3] = (IO)y.w;
             if (d == 0 && a.lse)
-                a.lse[(int64_t)token * a.heads + head] = L > 0.f ? (M + log2f(L)) * 0.693147180559945309f : -INFINITY;
+                a.lse[(int64_t)token * a.heads + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
         }
         cluster_sync_all();  // no block leaves while others read its shared memory
     } else {
@@ -673,7 +681,7 @@ __global__ void __launch_bounds__(FewCfg<KV, D, NR>::kWarps * 32) paged_attn_few
         if (a.p.status && blockIdx.x == 0)  // the sequences that get no units are reported too
             for (int i = threadIdx.x; i < a.p.batch; i += C::kWarps * 32) paged_seq(a.p, i);
         int all, unused;
-        stream_sums(a, 0, lane, all, unused);
+        stream_sums<C::kWarps>(a, 0, all, unused);
         const int blocks = min(a.stream, all);  // no block between others is empty
         const int c = (int)blockIdx.x;
         if (c >= blocks) return;
@@ -1161,7 +1169,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");  // the last maximum has been read
         l += other(l);
         const bool last = a.many.splits == 1;
-        const float inv = last ? (l > 0.f ? 1.f / l : 0.f) : 1.f;
+        const float inv = last ? 1.f / l : 1.f;
         const int rr = min(r, rows - 1);
         const int token = s.start + rr / a.group, head = kvh * a.group + rr % a.group;
         const int64_t th = (int64_t)token * a.heads + head;
@@ -1178,7 +1186,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             if (live && ok) {
                 const int d = (D / 2) * hf + c;
 #pragma unroll
-                for (int e = 0; e < 32; e++) o[e] = l > 0.f ? o[e] * inv : 0.f;
+                for (int e = 0; e < 32; e++) o[e] = l == 0.f ? 0.f : o[e] * inv;
 #pragma unroll
                 for (int e = 0; e < 32; e += 8) {
                     if (last)
@@ -1190,9 +1198,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         }
         if (live && ok && hf == 0) {
             if (!last)
-                a.part_ml[pth] = make_float2(l > 0.f ? m : -INFINITY, l);
+                a.part_ml[pth] = make_float2(l == 0.f ? -INFINITY : m, l);
             else if (a.lse)
-                a.lse[th] = l > 0.f ? (m + log2f(l)) * 0.693147180559945309f : -INFINITY;
+                a.lse[th] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f;
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
@@ -1576,7 +1584,7 @@ __global__ void __launch_bounds__(ExCfg<KV, D>::kThreads, 1)
         asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");  // the last maximum has been read
         l += other(l, 0);
         const bool last = a.many.splits == 1;
-        const float inv = last ? (l > 0.f ? 1.f / l : 0.f) : 1.f;
+        const float inv = last ? 1.f / l : 1.f;
         const int64_t th = (int64_t)token * a.heads + head;
         const int64_t pth = (int64_t)split * a.p.tokens * a.heads + th;
         if (live && ok) {
@@ -1585,14 +1593,14 @@ __global__ void __launch_bounds__(ExCfg<KV, D>::kThreads, 1)
             for (int d = 0; d < D / 2; d += 8) {
                 float y[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) y[e] = o[d + e] * inv;
+                for (int e = 0; e < 8; e++) y[e] = l == 0.f ? 0.f : o[d + e] * inv;
                 Eight<float>::store(dst + (D / 2) * hf + d, y);
             }
             if (hf == 0) {
                 if (!last)
                     a.part_ml[pth] = make_float2(m, l);
                 else if (a.lse)
-                    a.lse[th] = l > 0.f ? (m + log2f(l)) * 0.693147180559945309f : -INFINITY;
+                    a.lse[th] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f;
             }
         }
     } else {
@@ -1726,71 +1734,79 @@ __global__ void __launch_bounds__(128) paged_attn_merge_kernel(const __grid_cons
 #pragma unroll
         for (int e = 0; e < E; e++) y[e] = fmaf(w, src[e], y[e]);
     }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const float inv = 1.f / L;
     IO* dst = reinterpret_cast<IO*>(a.out + token * a.o_row + head * a.o_head) + lane * E;
 #pragma unroll
-    for (int e = 0; e < E; e++) dst[e] = (IO)(y[e] * inv);
-    if (a.lse && lane == 0) a.lse[th] = L > 0.f ? (M + log2f(L)) * 0.693147180559945309f : -INFINITY;
+    for (int e = 0; e < E; e++) dst[e] = (IO)(L == 0.f ? 0.f : y[e] * inv);
+    if (a.lse && lane == 0) a.lse[th] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
 }
 
-// Joins the pieces of one row of a shared-out tile: grid over (sequence, KV head, tile
-// row), 8 warps take turns at the pieces.
+// Joins the pieces of a shared-out tile's rows: grid over (sequence, KV head, group of ROWS
+// tile rows), 8 warps, 8 / ROWS of them for a row, taking turns at its pieces.  One row a
+// block where there are few blocks (a long sequence has dozens of pieces), eight otherwise
+// (every block adds up the batch's lengths).
 constexpr int kJoinWarps = 8;
-template <typename IO, int D>
-__global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const __grid_constant__ AttnView a, int tile_rows) {
+template <typename IO, int D, int ROWS>
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const __grid_constant__ AttnView a, int groups) {
+    constexpr int W = kJoinWarps / ROWS;  // warps of a row
     __shared__ float sums[kJoinWarps][D];
-    // (before the wait only what the kernel before, which has waited itself, did not write)
+    // (before the wait only what the kernel before did not write, and the ones before that had
+    // finished when it let this one start)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int r = blockIdx.x % tile_rows, kvh = blockIdx.x / tile_rows % a.p.kv_heads;
-    const int b = blockIdx.x / (tile_rows * a.p.kv_heads);
+    const int r = (int)(blockIdx.x % groups) * ROWS + warp / W, kvh = (int)(blockIdx.x / groups % a.p.kv_heads);
+    const int b = (int)(blockIdx.x / groups / a.p.kv_heads);
     int all, u0;
-    stream_sums(a, b, lane, all, u0);
+    stream_sums<kJoinWarps>(a, b, all, u0);
     const int n = stream_units(a, b);
     pdl_wait();
     pdl_trigger();
     if (n == 0) return;
     const PagedSeq s = paged_seq(a.p, b);
-    if (r >= s.n * a.group) return;
     u0 += kvh * n;
     // the block of unit u: the last c with c W / N <= u, rounded down
     const int blocks = min(a.stream, all);
     const int c0 = (int)(((int64_t)(u0 + 1) * blocks - 1) / all), c1 = (int)(((int64_t)(u0 + n) * blocks - 1) / all);
     const int used = c1 - c0 + 1;
     if (used == 1) return;  // written by the kernel itself
+    const bool live = r < s.n * a.group;
     // slot 1 of block c0, then slot 0 of the next ones
     auto at = [&](int x) { return ((int64_t)(c0 + x) * 2 + (x == 0)) * a.few.rows + r; };
-    float M = -INFINITY;
-    for (int x = lane; x < used; x += 32) M = fmaxf(M, a.strm_ml[at(x)].x);
-    M = warp_max(M);
-    const float mb = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
-    for (int x = lane; x < used; x += 32) {
-        const float2 p = a.strm_ml[at(x)];
-        L = fmaf(p.y, ex2_approx(p.x - mb), L);
-    }
-    L = warp_sum(L);
+    float M = -INFINITY, L = 0.f;
     constexpr int E = D / 32;
     float y[E] = {};
+    if (live) {
+        for (int x = lane; x < used; x += 32) M = fmaxf(M, a.strm_ml[at(x)].x);
+        M = warp_max(M);
+        const float mb = M == -INFINITY ? 0.f : M;
+        for (int x = lane; x < used; x += 32) {
+            const float2 p = a.strm_ml[at(x)];
+            L = fmaf(p.y, ex2_approx(p.x - mb), L);
+        }
+        L = warp_sum(L);
 #pragma unroll 4
-    for (int x = warp; x < used; x += kJoinWarps) {
-        const float w = ex2_approx(a.strm_ml[at(x)].x - mb);
-        const float* src = a.strm + at(x) * D + lane * E;
+        for (int x = warp % W; x < used; x += W) {
+            const float w = ex2_approx(a.strm_ml[at(x)].x - mb);
+            const float* src = a.strm + at(x) * D + lane * E;
 #pragma unroll
-        for (int e = 0; e < E; e++) y[e] = fmaf(w, src[e], y[e]);
+            for (int e = 0; e < E; e++) y[e] = fmaf(w, src[e], y[e]);
+        }
     }
 #pragma unroll
     for (int e = 0; e < E; e++) sums[warp][lane * E + e] = y[e];
     __syncthreads();
+    if (!live || warp % W) return;
     const int token = s.start + r / a.group, head = kvh * a.group + r % a.group;
-    if (threadIdx.x < D) {
+    const float inv = 1.f / L;
+    IO* dst = reinterpret_cast<IO*>(a.out + token * a.o_row + head * a.o_head);
+#pragma unroll
+    for (int e = 0; e < E; e++) {
         float z = 0.f;
 #pragma unroll
-        for (int x = 0; x < kJoinWarps; x++) z += sums[x][threadIdx.x];
-        z *= L > 0.f ? 1.f / L : 0.f;
-        reinterpret_cast<IO*>(a.out + token * a.o_row + head * a.o_head)[threadIdx.x] = (IO)z;
+        for (int x = 0; x < W; x++) z += sums[warp + x][lane + 32 * e];
+        dst[lane + 32 * e] = (IO)(L == 0.f ? 0.f : z * inv);
     }
-    if (a.lse && threadIdx.x == 0)
-        a.lse[(int64_t)token * a.heads + head] = L > 0.f ? (M + log2f(L)) * 0.693147180559945309f : -INFINITY;
+    if (a.lse && lane == 0)
+        a.lse[(int64_t)token * a.heads + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
 }
 
 // How the work is cut up: from the host's bounds alone, so that a captured
@@ -1927,9 +1943,13 @@ vb_status launch_attn(const AttnView& a, cudaStream_t s) {
     }
     if (a.stream > 1) {
         const int rows = (int)std::min<int64_t>(a.few.rows, (int64_t)a.p.max_new * a.group);
-        const int64_t grid = (int64_t)a.p.batch * a.p.kv_heads * rows;
-        if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
-        e = launch_pdl(paged_attn_join_kernel<IO, D>, dim3((unsigned)grid), dim3(kJoinWarps * 32), 0, s, a, rows);
+        const int64_t heads = (int64_t)a.p.batch * a.p.kv_heads;
+        const bool one = heads * rows <= 2048;
+        const int groups = one ? rows : (rows + 7) / 8;
+        if (heads * groups > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
+        const dim3 grid((unsigned)(heads * groups)), block(kJoinWarps * 32);
+        e = one ? launch_pdl(paged_attn_join_kernel<IO, D, 1>, grid, block, 0, s, a, groups)
+                : launch_pdl(paged_attn_join_kernel<IO, D, 8>, grid, block, 0, s, a, groups);
         if (e != cudaSuccess) return cuda_fail(e, "paged_attn_join_kernel");
     }
     if (a.many.splits > 1) {
@@ -1974,6 +1994,7 @@ extern "C" vb_status vb_paged_attn(const vb_paged_cache* cache, const vb_paged_b
     if (st) return st;
     if (window < 0) return fail(VB_ERR_ARG, "paged_attn: negative window");
     if (!batch->batch || !batch->tokens || !batch->max_new) return VB_OK;
+    if (window >= batch->max_len) window = 0;  // every position is within it
     if (!q || !out) return fail(VB_ERR_ARG, "paged_attn: null pointer");
     const int es = paged_elem_bytes(io), D = cache->head_dim;
     if (!paged_aligned(q, q_row, q_head, es) || !paged_aligned(out, o_row, o_head, es) || !paged_aligned(workspace, 0, 0, 1))

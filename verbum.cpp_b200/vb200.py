@@ -655,6 +655,8 @@ class PagedBatch:
         ps = None if status is None else _array(status.reshape(1), _I32, dev, "status")
         self.q_start, self.lens, self.table, self.status = q_start, lens, table, status
         self.tokens, self.max_len, self.width = int(tokens), int(max_len), table.shape[1]
+        if max(self.tokens, self.max_len, int(max_new), table.stride(0) if B > 1 else 0) > 0x7fffffff:
+            _refuse("paged batch: sizes are 32-bit")
         if B > 1 and table.stride(0) < table.shape[1]:
             _refuse("paged batch: rows of the table overlap")
         self.s = VBPagedBatch(B, self.tokens, int(max_new), int(max_len),
@@ -740,12 +742,14 @@ def paged_attn(cache, batch, q, out, lse=None, scale=None, window=0, workspace=N
     if lse is not None and lse.shape != (batch.tokens, heads):
         _refuse("lse: f32 [tokens, heads]")
     if workspace is None:
+        if stream is not None:  # the allocator would hand the memory on in the current stream's order
+            _refuse("a call on another stream brings its own workspace")
         workspace = paged_attn_workspace(cache, batch, heads)
     elif workspace.get_device() != dev or not workspace.is_contiguous():
         _refuse("workspace: contiguous memory on the cache's device")
     check(lib().vb_paged_attn(cache.ref, batch.ref, _dtype(q, "q"), heads, *qp, *op,
                               _array(lse, 0, dev, "lse", 2),
-                              cache.head_dim ** -0.5 if scale is None else scale, window, workspace.data_ptr(),
+                              cache.head_dim ** -0.5 if scale is None else scale, min(window, 0x7fffffff), workspace.data_ptr(),
                               workspace.numel() * workspace.element_size(), _raw_stream(stream, dev)))
 
 
