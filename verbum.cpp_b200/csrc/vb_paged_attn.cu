@@ -757,8 +757,8 @@ __global__ void __launch_bounds__(FewCfg<KV, D, NR>::kWarps * 32) paged_attn_few
 // to the cache's 16 bits as the products take them, their sum is not.
 // Of the two tiles' 128 x 128 scores the exponentials take 2048 clocks (16 a
 // clock on an SM) and, at D = 128, the products as many.  A prompt of 8192
-// tokens, 16/8 heads, bf16: 278 us, 990 TFLOP/s, 0.60 of the measured bf16 rate;
-// a key tile of the pair takes about 3200 clocks, bound by the chain scores ->
+// tokens, 16/8 heads, bf16: 254 us, 1083 TFLOP/s, 0.66 of the measured bf16 rate;
+// a key tile of the pair takes about 3000 clocks, bound by the chain scores ->
 // weights -> P.V -> next scores of one tile.
 constexpr int kTcThreads = 640;
 constexpr int kTcProducers = 96;
@@ -1149,12 +1149,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             f2 sum[2] = {0ull, 0ull};
             const f2 sc2 = f2pack(sc, sc), mb2 = f2pack(-mb, -mb);
             // the scores of both halves have been read (other() above): the weights may go over them
+            // 16 keys a step.  The products of the first 32 (of each half) may start while the others
+            // are made; their stores are waited for a step later, when they have long landed.
+            auto publish = [&](int h) {
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_addr(&p_full[i][h]), 1);
+            };
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                uint32_t w[16];
+            for (int h = 0; h < 4; h++) {
+                uint32_t w[8];
 #pragma unroll
-                for (int c = 0; c < 32; c += 2) {
-                    const f2 y = f2fma(f2pack(x[32 * h + c], x[32 * h + c + 1]), sc2, mb2);
+                for (int c = 0; c < 16; c += 2) {
+                    const f2 y = f2fma(f2pack(x[16 * h + c], x[16 * h + c + 1]), sc2, mb2);
                     float p0, p1;
                     f2unpack(y, p0, p1);
                     p0 = ex2_approx(p0);
@@ -1162,13 +1170,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
                     sum[(c >> 1) & 1] = f2add(sum[(c >> 1) & 1], f2pack(p0, p1));
                     w[c / 2] = pack2<T>(p0, p1);
                 }
-                tmem_st16(tS + 32 * hf + 16 * h, w);
-                // the products of these 32 keys (of each half) may start while the other 32 are made
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_addr(&p_full[i][h]), 1);
+                if (h == 2) publish(0);
+                tmem_st8(tS + 32 * hf + 8 * h, w);
             }
+            publish(1);
             l += f2sum(sum[0]) + f2sum(sum[1]);
         }
         if (n > 0) ok = tc_wait(smem_addr(&o_full[i]), 0u, &failed) && ok;
