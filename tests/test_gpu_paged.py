@@ -250,6 +250,20 @@ def test_scales_and_large_scores(io, cache, scale):
     check_attn(Setup([1, 140], [300, 200], io, cache, seed=3), scale=scale)
 
 
+@pytest.mark.parametrize("n", [1, 2, 40, 226])
+@pytest.mark.parametrize("seed", range(4))
+def test_small_weights_keep_their_bits(n, seed):
+    """f16 has no normal numbers below 2^-14: where the v of the largest weight is next to nothing,
+    the weights of 2^-14 of it and less make the output."""
+    s = Setup([n, 1, n], [297, 328, 267], "f16", "f16", H=18, KVH=2, seed=seed)
+    for b in range(3):
+        # every sequence's first key is far ahead of the others, and its v is tiny
+        slot = s.table[b, 0].long(), 0
+        s.k[slot] = 0.25 * s.q[s.rows(b)][0].reshape(2, 9, 128).sum(1).half()
+        s.v[slot] = 1e-6
+    check_attn(s, scale=0.9)
+
+
 @pytest.mark.parametrize("io,cache", PAIRS)
 def test_long_context(io, cache):
     check_attn(Setup([1, 2], [20011, 33333], io, cache, H=2, KVH=1, seed=4, page=64))

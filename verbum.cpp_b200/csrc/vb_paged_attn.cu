@@ -240,6 +240,13 @@ __device__ __forceinline__ uint32_t mat_t(uint32_t a) {
     return d;
 }
 
+// Weights are e^(s - reference); f16 ones take a reference so far (in powers of two) below the
+// maximum, for f16 has no normal numbers under 2^-14: a weight of 2^-14 of the largest would
+// lose bits that show where the largest one's v is small.  lse and the joins see the
+// reference, whatever it is.
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 6.f : 0.f;
+
 // ------------------------------------------------------------- few rows
 // The same by cutting the bits off: cheaper, for the operand whose other one is rounded
 // (the product of two cut-off rests would be of one sign, and add up).
@@ -455,7 +462,7 @@ __device__ __forceinline__ void few_piece(const AttnView& a, const PagedSeq& s, 
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                mx = fmaxf(mx, m[n][e]);
+                mx = fmaxf(mx - kLift<KV>, m[n][e]);
                 const float mb = mx == -INFINITY ? 0.f : mx;
                 alpha[n][e] = ex2_approx(m[n][e] - mb);
                 m[n][e] = mx;
@@ -752,8 +759,8 @@ __global__ void __launch_bounds__(FewCfg<KV, D, NR>::kWarps * 32) paged_attn_few
 //                    128-byte-swizzled layout the products read, by TMA or
 //                    16-byte cp.async; K and V take turns in a ring of four stages.
 // The running maximum is raised, and the sums rescaled, only when a score
-// exceeds it by more than 2^8: weights stay below 256, which changes no
-// rounding (they are relative), and rescaling is rare.  The weights are rounded
+// exceeds it by more than 2^8: weights stay below 256 (f16: 2^14), which changes
+// no rounding (they are relative), and rescaling is rare.  The weights are rounded
 // to the cache's 16 bits as the products take them, their sum is not.
 // Of the two tiles' 128 x 128 scores the exponentials take 2048 clocks (16 a
 // clock on an SM) and, at D = 128, the products as many.  A prompt of 8192
@@ -1128,6 +1135,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
                 for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], x[c + 2 * e], x[c + 2 * e + 1]);
             float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
             top = fmaxf(top, other(top));
+            top -= kLift<T>;
             const bool raise = top > m + 8.f || (m == -INFINITY && top > m);
             if (__any_sync(0xffffffffu, raise)) {  // in both warps of the pair alike
                 const float mn = raise ? top : m;
