@@ -601,6 +601,44 @@ def test_on_another_stream():
     assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("io,cache", PAIRS)
+def test_two_calls_at_once(io, cache):
+    # a decode batch and a mixed one on two streams of the caller's choice, over and over
+    s = [Setup([1] * 50, [(b * 37) % 900 + 1 for b in range(50)], io, cache, H=16, KVH=8, seed=1),
+         Setup([1, 90, 1, 40], [800, 300, 1500, 40], io, cache, H=16, KVH=8, seed=2)]
+    want = [check_attn(x) for x in s]
+    ws = [vb200.paged_attn_workspace(x.pc, x.pb, x.H) for x in s]
+    outs = [[x.out() for _ in range(6)] for x in s]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in s]
+    for i in range(6):
+        for x, st, w, o in zip(s, streams, ws, outs):
+            vb200.paged_attn(x.pc, x.pb, x.q, o[i], workspace=w, stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert all(torch.equal(x, w) for x in o)
+
+
+@pytest.mark.parametrize("io,cache", PAIRS)
+def test_k_and_v_in_one_pool_and_a_wider_table(io, cache):
+    s = Setup([1, 70, 3], [200, 300, 50], io, cache, seed=6)
+    want = check_attn(s)
+    both = torch.stack([s.k, s.v], 1)  # [page, 2, position, head, dim]
+    pc = vb200.PagedCache(both[:, 0], both[:, 1])
+    wide = torch.full((3, s.table.shape[1] + 5), -9, dtype=torch.int32, device="cuda")
+    wide[:, :s.table.shape[1]] = s.table
+    pb = vb200.PagedBatch(s.q_start, s.lens, wide[:, :s.table.shape[1]], max_new=70, max_len=300, tokens=s.T)
+    out = s.out()
+    vb200.paged_attn(pc, pb, s.q, out)
+    assert torch.equal(out, want)
+    k, v = s.k.clone(), s.v.clone()
+    vb200.paged_append(s.pc, s.pb, s.kn, s.vn)
+    vb200.paged_append(pc, pb, s.kn, s.vn)
+    for x, y in ((both[:, 0], s.k), (both[:, 1], s.v)):
+        assert torch.equal(x.nan_to_num(9.0), y.nan_to_num(9.0))
+    assert not torch.equal(k.nan_to_num(9.0), s.k.nan_to_num(9.0)) and not torch.equal(v.nan_to_num(9.0), s.v.nan_to_num(9.0))
+
+
 def test_the_same_call_gives_the_same_bits():
     s = Setup([1, 130, 1], [3000, 400, 1700], "f32", "f32", seed=41)
     a = check_attn(s)

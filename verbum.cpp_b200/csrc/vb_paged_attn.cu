@@ -272,6 +272,14 @@ struct FewCfg {
     static constexpr int kSmem = kWarps * kWarpBytes > kMerge ? kWarps * kWarpBytes : kMerge;
 };
 
+// Where a piece of a tile's keys leaves its rows: the output, or sums to be joined.
+struct Sink {
+    bool last;       // the piece is the whole tile: the output
+    bool keep;       // the sums stay in shared memory, row `row` at row * (D + 4), its (m, l) in kept
+    float* part;     // else: row `row`'s sums at part + row * D, its (m, l) at ml + row
+    float2* ml;
+};
+
 // Attention of 8 NR rows of a KV head by the warps of a block.  They share the rows and
 // take turns at blocks of 16 keys, each with a ring of its own in shared memory
 // (no barrier in the loop); at the end they join their (m, l, sum).
@@ -290,14 +298,7 @@ struct FewCfg {
 // each, relative, and of both signs), their sum is not.
 // 64 sequences of up to 4096 keys, bf16, 16/8 heads: 88 us, 5.6 TB/s, 0.85 of the measured
 // copy rate; 64 x 2112 f32 192 us, 0.88; 2 x up to 131072 f16 72.5 us, 0.89.
-// Where a piece of a tile's keys leaves its rows: the output, or sums to be joined.
-struct Sink {
-    bool last;       // the piece is the whole tile: the output
-    bool keep;       // the sums stay in shared memory, row `row` at row * (D + 4), its (m, l) in kept
-    float* part;     // else: row `row`'s sums at part + row * D, its (m, l) at ml + row
-    float2* ml;
-};
-
+//
 // The rows of KV head kvh of sequence b over keys k_begin .. k_end - 1, by the block.
 template <typename IO, typename KV, int D, int NR>
 __device__ __forceinline__ void few_piece(const AttnView& a, const PagedSeq& s, int b, int kvh, const KeyRange& kr,
