@@ -1295,7 +1295,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
                 commit_one(leader, smem_addr(&kv_empty[(2 * j + 1) % kTcStages]));
                 if (j + 1 < nm) {
                     commit_one(leader, smem_addr(&kv_empty[(2 * j + 2) % kTcStages]));
-                    // the next round's V and K, asked after while this round's products run
+                    // the next key tile's V and the K after it, asked after while these products run
                     wait_kv(2 * j + 3);
                     if (j + 2 < nm) wait_kv(2 * j + 4);
                 }
