@@ -294,9 +294,9 @@ VB_API vb_status vb_paged_append(const vb_paged_cache* cache, const vb_paged_bat
 
 /* Causal attention of the new tokens over their sequences' pages (appended
  * before): row with position p sees positions j <= p, with window > 0 only
- * j > p - window.  Places that no row of the call sees -- behind a sequence's
- * length, in pages of nobody -- may hold anything, NaN too; an infinity or NaN
- * in a v that some rows of a chunk see and others do not reaches all of them.
+ * j > p - window.  Places that a row does not see -- later tokens of its chunk,
+ * positions before its window, behind its sequence's length -- may hold
+ * anything, infinities and NaN too.
  * out [tokens][heads][D] = softmax(scale * q.k) v; an empty
  * row gives zeros.  lse (f32 [tokens][heads], may be NULL) gets the natural
  * logarithm of the sum of exp(scale * q.k), -inf for an empty row.  heads is a

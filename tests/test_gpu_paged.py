@@ -491,6 +491,40 @@ def test_a_nan_in_a_query_stays_in_its_row(io, cache, n):
     assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("io,cache", PAIRS)
+@pytest.mark.parametrize("n", [2, 7, 40, 300])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_what_a_row_does_not_see_does_not_reach_it(io, cache, n, value):
+    # k and v of a later token of the chunk, and of a position that has left the later rows' window
+    s = Setup([n, 1, n], [n + 100, 50, n], io, cache, seed=n)
+    window = n + 20
+    first = 100  # position of sequence 0's first new token
+    at = {0: first + n // 2, 2: n - 1}  # sequence: a poisoned position among its new ones
+    old = first - window + 1 + n // 3  # seen by the first rows of sequence 0 only; negative: from the table's end
+    poisoned = {0: [at[0], old % (s.table.shape[1] * s.page)], 2: [at[2]]}
+    slots = [(s.table[b, p // s.page].long(), p % s.page) for b, p in list(at.items()) + [(0, old)]]
+    for x in (s.k, s.v):
+        for slot in slots:
+            x[slot] = 0
+    ref, _, tol, _ = attn_reference(s, window)
+    for slot in slots:
+        s.k[slot], s.v[slot] = float("nan"), value
+    out = s.out()
+    vb200.paged_attn(s.pc, s.pb, s.q, out, window=window)
+    clean = 0
+    for b in (0, 2):
+        p = s.pos(b)
+        sees = torch.zeros_like(p, dtype=torch.bool)
+        for j in poisoned[b]:
+            sees |= (p >= j) & (p - window < j)
+        r = s.rows(b)
+        assert torch.isnan(out[r][sees]).all()
+        assert ((out[r].double() - ref[r]).abs() <= tol[r])[~sees].all()
+        clean += int((~sees).sum())
+    assert clean > 0  # (of two tokens both of sequence 0 see one, and the first of sequence 2 none)
+    assert ((out[s.rows(1)].double() - ref[s.rows(1)]).abs() <= tol[s.rows(1)]).all()
+
+
 def test_windows_beyond_every_position():
     s = Setup([1, 5, 40], [90, 3, 200], "bf16", "bf16", seed=14)
     want = check_attn(s)
