@@ -80,6 +80,7 @@ struct AttnView {
     Cut few, many;
     int stream;         // blocks that share all keys of the few-rows kernel evenly; 0: clusters of blocks, one a tile
     bool after_many;    // the few-rows kernel of this call follows its many-rows kernel
+    unsigned* ready;    // then: 1 once what came before the call can be read, by the many-rows kernel; else NULL
     int box;            // rows of a page that one TMA copy brings (many rows); 0: no tensor maps
     float* part;        // [split][token][head][D] sums of a split, relative to its maximum
     float2* part_ml;    // [split][token][head] (maximum in base 2, sum of weights)
@@ -624,6 +625,22 @@ __device__ __forceinline__ float4 cl_ld4(unsigned addr) {
     return v;
 }
 
+// A call's two kernels beside each other.  The few-rows kernel of a mixed call must not wait for
+// the many-rows kernel (griddepcontrol.wait would), but reads what came before the call, and only
+// a wait, or an acquire of what was released behind one, makes that visible.  So the word `ready`
+// is cleared by a launch of its own (a workspace has no contents to count on), set by the
+// many-rows kernel behind its wait, and acquired by each block of the few-rows kernel; a block that
+// finds it clear waits for the many-rows kernel after all.
+__global__ void paged_attn_clear_kernel(unsigned* ready) {
+    pdl_wait();
+    pdl_trigger();
+    *ready = 0;
+}
+__device__ __forceinline__ void release_ready(const AttnView& a) {
+    if (a.ready && blockIdx.x == 0 && threadIdx.x == 0)
+        asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(a.ready), "r"(1u) : "memory");
+}
+
 // CLUSTER: a cluster of 8 blocks for a tile (sequence, KV head), which join their pieces
 // through each other's shared memory (no second launch).  Else the keys of all tiles are
 // shared out evenly over the blocks.
@@ -634,10 +651,16 @@ __global__ void __launch_bounds__(FewCfg<KV, D, NR>::kWarps * 32) paged_attn_few
     using C = FewCfg<KV, D, NR>;
     extern __shared__ __align__(1024) char smem[];
     __shared__ float2 ml[C::kWarps][C::kRows];
-    // Behind the many-rows kernel of the same call the work itself needs no wait: nothing here
-    // reads what that one writes, and it lets this one start only when every block of its own
-    // has waited for what came before.  The wait at the end keeps the order for what follows.
-    if (!a.after_many) pdl_wait();
+    // Behind the many-rows kernel of the same call nothing here reads what that one writes, so
+    // the order that `ready` gives is enough.  The wait at the end keeps it for what follows.
+    if (a.after_many) {
+        __shared__ unsigned ready;
+        if (threadIdx.x == 0) ready = ld_acquire(a.ready);
+        __syncthreads();
+        if (ready != 1) pdl_wait();
+    } else {
+        pdl_wait();
+    }
     pdl_trigger();
     struct AtEnd {
         bool wait;
@@ -1024,6 +1047,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     __shared__ float xch[2][2][128];
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31, wg = t >> 7;
     pdl_wait();
+    release_ready(a);
     pdl_trigger();
     int64_t idx = blockIdx.x;
     const int split = (int)(idx % a.many.splits);
@@ -1446,6 +1470,7 @@ __global__ void __launch_bounds__(ExCfg<KV, D>::kThreads, 1)
     __shared__ float xch[2][2][128];
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31, wg = t >> 7;
     pdl_wait();
+    release_ready(a);
     pdl_trigger();
     int64_t idx = blockIdx.x;
     const int split = (int)(idx % a.many.splits);
@@ -1774,16 +1799,14 @@ template <typename IO, int D, int ROWS>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const __grid_constant__ AttnView a, int groups) {
     constexpr int W = kJoinWarps / ROWS;  // warps of a row
     __shared__ float sums[kJoinWarps][D];
-    // (before the wait only what the kernel before did not write, and the ones before that had
-    // finished when it let this one start)
+    pdl_wait();
+    pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int r = (int)(blockIdx.x % groups) * ROWS + warp / W, kvh = (int)(blockIdx.x / groups % a.p.kv_heads);
     const int b = (int)(blockIdx.x / groups / a.p.kv_heads);
     int all, u0;
     stream_sums<kJoinWarps>(a, b, all, u0);
     const int n = stream_units(a, b);
-    pdl_wait();
-    pdl_trigger();
     if (n == 0) return;
     const PagedSeq s = paged_seq(a.p, b);
     u0 += kvh * n;
@@ -1963,10 +1986,14 @@ Plan make_plan(const PagedView& p, int io, int cache, int heads, int D, int wind
     pl.max_splits = tc ? (int)std::min<int64_t>(want, (all + 511) / 512) : 1;
     return pl;
 }
-// The workspace: first the shared-out tiles' pieces, then the splits'.
+// The workspace: first the shared-out tiles' pieces, then the splits', then (both kernels) 16 bytes for `ready`.
+bool both_kernels(const Plan& pl) { return pl.few_rows && pl.few_rows != 0x7fffffff; }
 size_t stream_floats(const Plan& pl, int D) { return pl.few_rows ? (size_t)kStreamMost * 2 * pl.few.rows * (D + 2) : 0; }
+size_t split_floats(const Plan& pl, const PagedView& p, int heads, int D) {
+    return pl.max_splits > 1 ? (size_t)pl.max_splits * p.tokens * heads * (D + 2) : 0;
+}
 size_t plan_bytes(const Plan& pl, const PagedView& p, int heads, int D) {
-    return 4 * (stream_floats(pl, D) + (pl.max_splits > 1 ? (size_t)pl.max_splits * p.tokens * heads * (D + 2) : 0));
+    return 4 * (stream_floats(pl, D) + split_floats(pl, p, heads, D) + (both_kernels(pl) ? 4 : 0));
 }
 
 // Tensor map of a pool as [page][kv head][position][dim], boxes of one page's rows (128 at
@@ -2016,6 +2043,10 @@ vb_status launch_attn(const AttnView& a, cudaStream_t s) {
                                                 (int64_t)a.p.tokens * a.group / rows + a.p.batch);
         const int64_t grid = tiles * a.many.splits * a.p.kv_heads;
         if (grid > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
+        if (a.ready) {
+            e = launch_pdl(paged_attn_clear_kernel, dim3(1), dim3(1), 0, s, a.ready);
+            if (e != cudaSuccess) return cuda_fail(e, "paged_attn_clear_kernel");
+        }
         AttnView b = a;
         CUtensorMap mk{}, mv{};
         if constexpr (sizeof(KV) == 2) {
@@ -2038,7 +2069,7 @@ vb_status launch_attn(const AttnView& a, cudaStream_t s) {
     }
     if (a.few_rows) {
         AttnView f = a;
-        f.after_many = a.few_rows != 0x7fffffff;
+        f.after_many = a.ready != nullptr;
         vb_status st = VB_OK;
         if (a.few.rows == 8) {
             st = launch_few<IO, KV, D, 1>(f, s);
@@ -2139,6 +2170,7 @@ extern "C" vb_status vb_paged_attn(const vb_paged_cache* cache, const vb_paged_b
     a.strm_ml = reinterpret_cast<float2*>(a.strm + parts * D);
     a.part = a.strm + stream_floats(pl, D);
     a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)pl.max_splits * a.p.tokens * heads * D);
+    if (both_kernels(pl)) a.ready = reinterpret_cast<unsigned*>(a.part + split_floats(pl, a.p, heads, D));
     return D == 128 ? launch_attn<128>(a, io, cache->dtype, as_stream(stream))
                     : launch_attn<64>(a, io, cache->dtype, as_stream(stream));
 }
