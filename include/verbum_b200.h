@@ -248,8 +248,11 @@ enum {
  * max_new and max_len bound what they say.  The kernels check them: a sequence
  * with bad rows is not computed, one with a bad length counts as length 0, a
  * bad page is not written and reads as zeros, and each sets its bit in
- * *status (a device word that the caller clears; NULL: not reported).  Pages
- * that receive new tokens must belong to one sequence of the batch. */
+ * *status (a device word that the caller clears; NULL: not reported).  The
+ * other sequences come out as they would without it, as long as q_start
+ * ascends; where it descends, rows that more than one sequence claims, and the
+ * other rows of those sequences, may be left as they were.  Pages that receive
+ * new tokens must belong to one sequence of the batch. */
 typedef struct {
     int batch;
     int tokens;

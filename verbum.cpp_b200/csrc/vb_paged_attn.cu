@@ -915,8 +915,12 @@ __device__ __forceinline__ void find_tile(const AttnView& a, int64_t idx, int ro
         const int i = hi - 1 - lane;
         int n = 0;
         if (i >= 0) {
-            const int64_t d = (int64_t)a.p.q_start[i + 1] - a.p.q_start[i];
-            n = d > 0 && d <= a.p.max_new && d * a.group > a.few_rows ? (int)((d * a.group + rows - 1) / rows) : 0;
+            // (a sequence whose rows are not all there has no tiles: the grid counts those of `tokens` rows)
+            const int start = a.p.q_start[i], end = a.p.q_start[i + 1];
+            const int64_t d = (int64_t)end - start;
+            n = start >= 0 && end <= a.p.tokens && d > 0 && d <= a.p.max_new && d * a.group > a.few_rows
+                    ? (int)((d * a.group + rows - 1) / rows)
+                    : 0;
         }
         int sum = n;  // tiles of lanes 0..lane
 #pragma unroll
