@@ -22,3 +22,36 @@ def test_a_sequence_behind_the_rows_takes_no_other_ones_place(io, cache, starts)
     vb200.paged_attn(s.pc, s.pb, s.q, out)
     assert int(s.status) == vb200.PAGED_BAD_ROWS
     assert ((out.double() - want).abs() <= tol).all()
+
+
+def _status(s, call, q_start=None, lens=None, tokens=None, max_new=None, max_len=None):
+    q_start = s.q_start if q_start is None else torch.tensor(q_start, dtype=torch.int32, device="cuda")
+    lens = s.lens if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    s.status.zero_()
+    pb = vb200.PagedBatch(q_start, lens, s.table, max_new=max_new or s.pb.s.max_new, max_len=s.pb.max_len, tokens=s.T,
+                          status=s.status)
+    if call == "attn":
+        vb200.paged_attn(s.pc, pb, s.q, s.out())
+    else:
+        vb200.paged_append(s.pc, pb, s.kn, s.vn)
+    return int(s.status)
+
+
+@pytest.mark.parametrize("call", ["attn", "append"])
+@pytest.mark.parametrize("kind", ["one", "few", "decode", "prompt", "mixed"])
+def test_every_bad_sequence_is_reported(call, kind):
+    # whichever kernel takes the batch, and whether or not a row leads to the sequence
+    news = {"one": [1], "few": [8, 8], "decode": [1] * 50, "prompt": [200], "mixed": [1, 150, 1, 1]}[kind]
+    s = Setup(news, [n + 60 for n in news], "bf16", "bf16", H=16, KVH=8, seed=2)
+    starts, lens, B, T = s.q_start.tolist(), s.lens_h, len(news), s.T
+    rows, length = vb200.PAGED_BAD_ROWS, vb200.PAGED_BAD_LEN
+    assert _status(s, call) == 0
+    assert _status(s, call, q_start=starts[:-1] + [T + 1]) == rows            # rows behind the last one
+    assert _status(s, call, q_start=starts[:-1] + [T + 10**6]) == rows
+    assert _status(s, call, q_start=starts[:-1] + [starts[-2] - 1]) == rows   # fewer than none
+    assert _status(s, call, q_start=[-1] + starts[1:]) == rows
+    assert _status(s, call, q_start=[T] * B + [T + 7]) == rows                # and no sequence has rows
+    assert _status(s, call, lens=lens[:-1] + [-1]) == length
+    assert _status(s, call, q_start=[0] * (B + 1), lens=lens[:-1] + [s.pb.max_len + 1]) == length
+    if max(news) > 20:
+        assert _status(s, call, max_new=max(news) - 1) == rows

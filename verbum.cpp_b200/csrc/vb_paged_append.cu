@@ -47,6 +47,8 @@ __global__ void __launch_bounds__(kAppendThreads, 4) paged_append_kernel(const _
     constexpr int U = D / 16;  // threads of a head row
     pdl_wait();
     pdl_trigger();
+    if (a.p.status && blockIdx.x == 0)  // the sequences that no row leads to are reported too
+        for (int i = threadIdx.x; i < a.p.batch; i += kAppendThreads) paged_seq(a.p, i);
     const int lane = threadIdx.x & 31, nk = a.p.kv_heads, rot = a.rope.rot;
     const unsigned g = blockIdx.x * (unsigned)kAppendThreads + threadIdx.x;  // (the host keeps it in 32 bits)
     const int t = (int)(g / (unsigned)a.row_units);

@@ -905,6 +905,11 @@ __device__ __forceinline__ bool tc_wait(unsigned bar, unsigned parity, volatile 
     }
 }
 
+// Where the many-rows kernel runs without the other (one sequence), it reports what gets no tile.
+__device__ __forceinline__ void report_one(const AttnView& a) {
+    if (a.few_rows == 0 && blockIdx.x == 0 && threadIdx.x == 0 && a.p.status) paged_seq(a.p, 0);
+}
+
 // Sequence and tile of the idx-th of all tiles of `rows` rows (sequences with more than
 // a.few_rows rows only), the last ones -- which see most keys -- first; b = -1: none.
 __device__ __forceinline__ void find_tile(const AttnView& a, int64_t idx, int rows, int lane, int& b, int& tile) {
@@ -1059,6 +1064,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     const int kvh = (int)(idx % a.p.kv_heads);
     idx /= a.p.kv_heads;
     int b, tile;
+    report_one(a);
     find_tile(a, idx, kTcRows, lane, b, tile);
     if (b < 0) return;
     const PagedSeq s = paged_seq(a.p, b);
@@ -1482,6 +1488,7 @@ __global__ void __launch_bounds__(ExCfg<KV, D>::kThreads, 1)
     const int kvh = (int)(idx % a.p.kv_heads);
     idx /= a.p.kv_heads;
     int b, tile;
+    report_one(a);
     find_tile(a, idx, kExRows, lane, b, tile);
     if (b < 0) return;
     const PagedSeq s = paged_seq(a.p, b);
