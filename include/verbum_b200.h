@@ -55,9 +55,12 @@ VB_API const char* vb_version(void);
  * (vb_engine_step / decode on path 2) -- one CTA waits for an exchange word no
  * CTA writes; site 2: the next tensor-core GEMM launched outside a stream
  * capture (vb_matmul_nt_tc with M <= 64) -- its first CTA never fills its first
- * stage.  The kernel records the timeout, lets its own copies and MMAs land,
- * releases its tensor memory and returns; the call returns VB_ERR_TIMEOUT and
- * the engine stays usable.  0 disarms.  Nothing faults, traps or hangs. */
+ * stage; site 3: the next many-rows launch of vb_paged_attn outside a stream
+ * capture -- its first CTA never has all of its q.  The kernel records the
+ * timeout, lets its own copies and MMAs land, releases its tensor memory and
+ * returns; the call returns VB_ERR_TIMEOUT (vb_paged_attn, which does not wait:
+ * VB_PAGED_TIMEOUT in the batch's status word) and the engine stays usable.
+ * 0 disarms.  Nothing faults, traps or hangs. */
 VB_API vb_status vb_debug_arm_fault(int site);
 
 /* ------------------------------------------------------------------------ */
@@ -232,7 +235,8 @@ enum {
     VB_PAGED_BAD_ROWS = 1, /* a sequence's rows are not within 0..tokens, or more than max_new */
     VB_PAGED_BAD_LEN = 2,  /* a length is negative or above max_len */
     VB_PAGED_BAD_PAGE = 4, /* a page id outside 0..num_pages-1 */
-    VB_PAGED_TIMEOUT = 8   /* a bounded wait in a kernel gave up: the outputs are not valid */
+    VB_PAGED_TIMEOUT = 8   /* a bounded wait in a kernel gave up: the outputs are not valid (the
+                              lse of its rows is NaN, which shows it without a status word) */
 };
 
 /* New tokens of `batch` sequences, packed: sequence b owns rows

@@ -73,6 +73,7 @@ bool fault_take(int site) {
     int want = site;
     return site != kFaultNone && g_fault_site.compare_exchange_strong(want, kFaultNone);
 }
+bool fault_armed_for(int site) { return g_fault_site.load(std::memory_order_relaxed) == site; }
 }  // namespace vb
 
 using namespace vb;
@@ -84,7 +85,7 @@ const char* vb_last_error(void) { return g_last_error.c_str(); }
 const char* vb_version(void) { return "verbum-b200 0.1 (sm_100a)"; }
 
 vb_status vb_debug_arm_fault(int site) {
-    if (site < kFaultNone || site > kFaultGemmStage) return fail(VB_ERR_ARG, "fault site must be 0, 1 or 2");
+    if (site < kFaultNone || site > kFaultPagedQ) return fail(VB_ERR_ARG, "fault site must be 0, 1, 2 or 3");
     g_fault_site.store(site);
     return VB_OK;
 }

@@ -82,6 +82,7 @@ struct AttnView {
     bool after_many;    // the few-rows kernel of this call follows its many-rows kernel
     unsigned* ready;    // then: 1 once what came before the call can be read, by the many-rows kernel; else NULL
     int box;            // rows of a page that one TMA copy brings (many rows); 0: no tensor maps
+    bool stall;         // test hook (vb_debug_arm_fault): block 0 of the many-rows kernel never has all of its q
     float* part;        // [split][token][head][D] sums of a split, relative to its maximum
     float2* part_ml;    // [split][token][head] (maximum in base 2, sum of weights)
     float* strm;        // the same of the shared keys: [block][2][tile row][D]
@@ -150,6 +151,7 @@ __device__ __forceinline__ void cp_async16(unsigned dst, const void* src, bool r
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
@@ -1132,7 +1134,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
                            real);
             }
         }
-        cp_async_arrive(smem_addr(&q_full));
+        if (!(a.stall && blockIdx.x == 0 && t == 0)) cp_async_arrive(smem_addr(&q_full));
         const float sc = fabsf(a.scale_log2);
         const bool flip = a.scale_log2 < 0.f;
         float m = -INFINITY, l = 0.f;  // m: the maximum the sums are relative to; l: this half's sum
@@ -1220,10 +1222,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             l += f2sum(sum[0]) + f2sum(sum[1]);
         }
         if (n > 0) ok = tc_wait(smem_addr(&o_full[i]), 0u, &failed) && ok;
-        ok = __all_sync(0xffffffffu, ok);
+        ok = ok && !*(volatile int*)&failed;  // (where another wait gave up the products behind it were left out)
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");  // the last maximum has been read
-        l += other(l);
+        l += other(ok ? l : nanf(""));  // rows of which a wait gave up are NaN, not what the output held
+        if (!ok) l = nanf("");
+        cp_async_wait_all();  // q's, had nobody waited for them
         const bool last = a.many.splits == 1;
         const float inv = last ? 1.f / l : 1.f;
         const int rr = min(r, rows - 1);
@@ -1239,7 +1243,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
 #pragma unroll
                 for (int e = 0; e < 32; e++) o[e] = 0.f;
             }
-            if (live && ok) {
+            if (live) {
                 const int d = (D / 2) * hf + c;
 #pragma unroll
                 for (int e = 0; e < 32; e++) o[e] = l == 0.f ? 0.f : o[e] * inv;
@@ -1252,7 +1256,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
                 }
             }
         }
-        if (live && ok && hf == 0) {
+        if (live && hf == 0) {
             if (!last)
                 a.part_ml[pth] = make_float2(l == 0.f ? -INFINITY : m, l);
             else if (a.lse)
@@ -1560,7 +1564,7 @@ __global__ void __launch_bounds__(ExCfg<KV, D>::kThreads, 1)
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_addr(&q_full), 1);
+        if (lane == 0 && !(a.stall && blockIdx.x == 0 && t == 0)) mbar_arrive(smem_addr(&q_full), 1);
 
         const unsigned lanes = (unsigned)(32 * (warp & 3)) << 16;
         const unsigned tPV = tm + C::kPV + (D / 2) * hf + lanes;
@@ -1640,14 +1644,15 @@ __global__ void __launch_bounds__(ExCfg<KV, D>::kThreads, 1)
             alpha = f;
         }
         if (n > 0) fold(n - 1);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = ok && !*(volatile int*)&failed;  // (see the kernel above)
         asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");  // the last maximum has been read
-        l += other(l, 0);
+        l += other(ok ? l : nanf(""), 0);
+        if (!ok) l = nanf("");
         const bool last = a.many.splits == 1;
         const float inv = last ? 1.f / l : 1.f;
         const int64_t th = (int64_t)token * a.heads + head;
         const int64_t pth = (int64_t)split * a.p.tokens * a.heads + th;
-        if (live && ok) {
+        if (live) {
             float* dst = last ? reinterpret_cast<float*>(a.out + token * a.o_row + head * a.o_head) : a.part + pth * D;
 #pragma unroll
             for (int d = 0; d < D / 2; d += 8) {
@@ -2059,6 +2064,11 @@ vb_status launch_attn(const AttnView& a, cudaStream_t s) {
             if (e != cudaSuccess) return cuda_fail(e, "paged_attn_clear_kernel");
         }
         AttnView b = a;
+        if (fault_armed_for(kFaultPagedQ)) {  // failure-path test: never a launch that is being captured
+            cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+            VB_CUDA_TRY(cudaStreamIsCapturing(s, &cs));
+            b.stall = cs == cudaStreamCaptureStatusNone && fault_take(kFaultPagedQ);
+        }
         CUtensorMap mk{}, mv{};
         if constexpr (sizeof(KV) == 2) {
             b.box = page_map(a.p, a.p.k, D, std::is_same<KV, __half>::value, &mk);

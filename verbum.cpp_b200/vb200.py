@@ -199,7 +199,7 @@ def synth_normal(n: int, seed: int, std: float = 0.02) -> np.ndarray:
 
 def debug_arm_fault(site: int):
     """Arms the failure-path test hook for one launch (1 = clustered step,
-    2 = tensor-core GEMM; 0 disarms)."""
+    2 = tensor-core GEMM, 3 = paged attention of many rows; 0 disarms)."""
     check(lib().vb_debug_arm_fault(int(site)))
 
 
