@@ -235,8 +235,8 @@ enum {
     VB_PAGED_BAD_ROWS = 1, /* a sequence's rows are not within 0..tokens, or more than max_new */
     VB_PAGED_BAD_LEN = 2,  /* a length is negative or above max_len */
     VB_PAGED_BAD_PAGE = 4, /* a page id outside 0..num_pages-1 */
-    VB_PAGED_TIMEOUT = 8   /* a bounded wait in a kernel gave up: the outputs are not valid (the
-                              lse of its rows is NaN, which shows it without a status word) */
+    VB_PAGED_TIMEOUT = 8   /* a bounded wait in a kernel gave up: the outputs are not valid (what
+                              could not be computed again is NaN, never what was there before) */
 };
 
 /* New tokens of `batch` sequences, packed: sequence b owns rows

@@ -1,10 +1,11 @@
 """Calls of the paged operators at the edges of what their interface allows."""
+import math
 import time
 
 import pytest
 
 import vb200
-from test_gpu_paged import PAIRS, Setup, attn_reference, check_attn
+from test_gpu_paged import PAIRS, U, Setup, attn_reference, check_attn
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -59,6 +60,119 @@ def test_every_bad_sequence_is_reported(call, kind):
         assert _status(s, call, max_new=max(news) - 1) == rows
 
 
+# ------------------------------------------------- values that are not finite
+
+def formula(s, window=0):
+    """out in 64 bits, in the sense of limits: a weight of 0 silences whatever stands there, any
+    other passes an infinity on.  And the error bound of its finite elements."""
+    out = torch.zeros(s.T, s.H, s.D, dtype=torch.float64, device="cuda")
+    tol = torch.zeros_like(out)
+    lse = torch.full((s.T, s.H), -math.inf, dtype=torch.float64, device="cuda")  # NaN under a score of +inf, as out
+    for b in range(len(s.news)):
+        k, v = s.gather(b)
+        pos, r = s.pos(b), s.rows(b)
+        q = s.q[r].double().reshape(-1, s.KVH, s.G, s.D)
+        j = torch.arange(k.shape[0], device="cuda")
+        see = j <= pos[:, None]
+        if window:
+            see &= j > pos[:, None] - window
+        a = torch.einsum("nhgd,lhd->nhgl", q, k.nan_to_num(0, 0, 0)) * s.D**-0.5
+        size = torch.einsum("nhgd,lhd->nhgl", q.abs(), k.abs().nan_to_num(0, 0, 0)) * s.D**-0.5
+        for n, h, d in torch.nonzero(~torch.isfinite(k)).tolist():  # (one element of a key at most)
+            x = q[:, h, :, d] * k[n, h, d]
+            a[:, h, :, n] = torch.where(torch.isnan(x) | torch.isinf(x), x, a[:, h, :, n])
+        a = a.masked_fill(~see[:, None, None], -math.inf)
+        p = torch.softmax(a, -1)
+        fin = torch.isfinite(v)
+        y = torch.einsum("nhgl,lhd->nhgd", p, torch.where(fin, v, 0))
+        mass = torch.einsum("nhgl,lhd->nhgd", p, torch.where(fin, v, 0).abs())
+        for n, h, d in torch.nonzero(~fin).tolist():
+            y[:, h, :, d] += torch.where(p[:, h, :, n] == 0, 0, v[n, h, d])
+        size = size.masked_fill(~see[:, None, None], 0).amax(-1)[..., None]
+        u = U[s.io]
+        out[r] = y.reshape(-1, s.H, s.D)
+        lse[r] = torch.where((a == math.inf).any(-1), math.nan, torch.logsumexp(a, -1)).reshape(-1, s.H)
+        tol[r] = ((2 * size * 2.0**-19 + 2.0**-20 + (u if s.io != "f32" else 0)) * mass + u * y.abs() + 1e-30 +
+                  (2.0**-24 if s.io == "f16" else 0)).reshape(-1, s.H, s.D)
+    return out, tol, lse
+
+
+def check_formula(s, window=0):
+    want, tol, wl = formula(s, window)
+    out, lse = s.out(), torch.full((s.T, s.H), 55.0, device="cuda")
+    vb200.paged_attn(s.pc, s.pb, s.q, out, lse=lse, window=window)
+    fin = torch.isfinite(want)
+    assert torch.equal(out.double()[~fin].nan_to_num(7.0), want[~fin].nan_to_num(7.0))
+    assert ((out.double() - want).abs()[fin] <= tol[fin]).all()
+    assert torch.equal(torch.isnan(lse), torch.isnan(wl))
+    fin = torch.isfinite(wl)
+    assert ((lse.double() - wl).abs()[fin] <= 1e-3).all()
+    return out
+
+
+@pytest.mark.parametrize("io,cache", PAIRS)
+@pytest.mark.parametrize("n", [2, 40, 300])
+def test_an_infinity_that_rows_of_a_chunk_see(io, cache, n):
+    s = Setup([n, 1, n], [n + 500, 60, n], io, cache, seed=n)
+    for b, pos, head, d, value in ((0, 3, 0, 5, math.inf), (0, 400, 1, 9, -math.inf), (2, n - 1, 0, 1, math.inf),
+                                   (0, 500 + n // 2, 1, 7, math.nan)):
+        s.v[s.table[b, pos // s.page].long(), pos % s.page, head, d] = value
+    check_formula(s)
+    check_formula(s, window=n + 90)
+
+
+@pytest.mark.parametrize("n", [2, 40, 300])
+def test_an_infinity_under_a_weight_that_f16_has_not(n):
+    s = Setup([n, 1], [n + 200, 90], "f16", "f16", H=4, KVH=2, seed=n)
+    slot = s.table[0, 2].long(), 1  # position 33, seen by all rows of sequence 0
+    s.q[:n, :, 0] = 8.0
+    s.k[..., 0] = 0.0
+    s.k[slot[0], slot[1], :, 0] = -40.0  # 40 * 8 / sqrt(128) = 28 below the others: 2^-40
+    s.v[slot[0], slot[1], 0, 3] = math.inf
+    out = check_formula(s)
+    assert (out[:n, :2, 3] == math.inf).all()
+
+
+def _time(call, n=5):
+    call()
+    t = []
+    for _ in range(n):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        call()
+        b.record()
+        torch.cuda.synchronize()
+        t.append(a.elapsed_time(b))
+    return sorted(t)[n // 2]
+
+
+@pytest.mark.parametrize("io,cache", PAIRS)
+@pytest.mark.parametrize("what", ["v", "k", "v element"])
+@pytest.mark.parametrize("where", ["first", "own"])
+def test_a_nan_that_rows_see_costs_little(io, cache, what, where):
+    """One bad row of the cache makes every later output NaN: no reason for a call to take many
+    times as long and hold up the other sequences of its batch."""
+    n = 4096
+    s = Setup([n, 1], [n, 70], io, cache, H=16, KVH=8, seed=1, page=64)
+    ws, out = vb200.paged_attn_workspace(s.pc, s.pb, s.H), s.out()
+    call = lambda: vb200.paged_attn(s.pc, s.pb, s.q, out, workspace=ws)
+    clean = _time(call)
+    keep = out.clone()
+    x = s.k if what == "k" else s.v
+    pos = 0 if where == "first" else n - 130
+    dims = slice(9, 10) if what == "v element" else slice(None)
+    x[s.table[0, pos // 64].long(), pos % 64, :, dims] = math.nan
+    bad = _time(call)
+    assert torch.isnan(out[pos:n, :, dims]).all()
+    assert torch.equal(out[:pos], keep[:pos]) or (torch.isfinite(out[:pos]).all() and
+                                                  (out[:pos].float() - keep[:pos].float()).abs().max() < 0.02)
+    if what == "v element":
+        assert torch.isfinite(out[:n, :, :9]).all() and torch.isfinite(out[:n, :, 10:]).all()
+    assert torch.equal(out[n:], keep[n:])
+    print(f"{io} {cache} {what} {where}: {clean:.3f} -> {bad:.3f} ms")
+    assert bad < 4 * clean + 1.0, (clean, bad)
+
+
 # ------------------------------------------------------ a wait that gives up
 
 @pytest.mark.parametrize("io,cache", PAIRS)
@@ -84,12 +198,13 @@ def test_a_wait_runs_out(io, cache, news, lens, D, status):
     if status:
         assert int(s.status) == vb200.PAGED_TIMEOUT
         s.status.zero_()
-    lost = torch.isnan(lse)
-    assert lost.any() and not lost[:, 2:].any() and not lost[:s.T - news[-1]].any()
-    assert torch.equal(lse[~lost], wl[~lost]) and torch.equal(out[~lost], want[~lost])
+    hit = torch.zeros_like(lse, dtype=torch.bool)
+    hit[s.T - news[-1]:, :2] = True
+    assert torch.equal(lse[~hit], wl[~hit]) and torch.equal(out[~hit], want[~hit])
     # NaN, or taken again from the keys themselves: never what the output or a workspace held before
-    left = out[lost].float()
-    assert (torch.isnan(left) | ((left - want[lost].float()).abs() < 0.02)).all()
+    for x, w in ((lse, wl), (out, want)):
+        x, w = x[hit].float(), w[hit].float()
+        assert (torch.isnan(x) | ((x - w).abs() < 0.02)).all()
     out, lse = call()  # one launch only
     assert torch.equal(out, want) and torch.equal(lse, wl)
     assert not status or int(s.status) == 0

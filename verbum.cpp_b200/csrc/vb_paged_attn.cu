@@ -83,6 +83,7 @@ struct AttnView {
     unsigned* ready;    // then: 1 once what came before the call can be read, by the many-rows kernel; else NULL
     int box;            // rows of a page that one TMA copy brings (many rows); 0: no tensor maps
     bool stall;         // test hook (vb_debug_arm_fault): block 0 of the many-rows kernel never has all of its q
+    int* hint;          // [sequence][KV head] where a row that was taken again met a NaN (redo_row); -1 at first
     float* part;        // [split][token][head][D] sums of a split, relative to its maximum
     float2* part_ml;    // [split][token][head] (maximum in base 2, sum of weights)
     float* strm;        // the same of the shared keys: [block][2][tile row][D]
@@ -638,6 +639,10 @@ __global__ void paged_attn_clear_kernel(unsigned* ready) {
     pdl_trigger();
     *ready = 0;
 }
+__device__ __forceinline__ void clear_hints(const AttnView& a) {
+    if (a.hint && blockIdx.x == 0)
+        for (int i = threadIdx.x; i < a.p.batch * a.p.kv_heads; i += blockDim.x) a.hint[i] = -1;
+}
 __device__ __forceinline__ void release_ready(const AttnView& a) {
     if (a.ready && blockIdx.x == 0 && threadIdx.x == 0)
         asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(a.ready), "r"(1u) : "memory");
@@ -664,6 +669,7 @@ __global__ void __launch_bounds__(FewCfg<KV, D, NR>::kWarps * 32) paged_attn_few
         pdl_wait();
     }
     pdl_trigger();
+    if (!a.after_many) clear_hints(a);
     struct AtEnd {
         bool wait;
         __device__ ~AtEnd() {
@@ -1060,6 +1066,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     pdl_wait();
     release_ready(a);
     pdl_trigger();
+    clear_hints(a);
     int64_t idx = blockIdx.x;
     const int split = (int)(idx % a.many.splits);
     idx /= a.many.splits;
@@ -1486,6 +1493,7 @@ __global__ void __launch_bounds__(ExCfg<KV, D>::kThreads, 1)
     pdl_wait();
     release_ready(a);
     pdl_trigger();
+    clear_hints(a);
     int64_t idx = blockIdx.x;
     const int split = (int)(idx % a.many.splits);
     idx /= a.many.splits;
@@ -1873,11 +1881,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const 
 }
 
 // A tile's rows of several tokens see different keys, and a weight of 0 times an infinity or
-// NaN in a v that a row does not see is NaN.  So rows that came out non-finite are taken
-// again, key by key over what they do see.  A warp looks at 2 KB of (token, head) rows, 16
-// bytes a lane and load, and where all is finite that is all it does: 5 us after a prompt of
-// 8192 tokens (295 us with it, 290 without, in turns) as after 1500 rows, so a launch and its
-// wait more than the 33 MB out of L2; by 2-byte loads it was 14 us.
+// NaN in a v that a row does not see is NaN.  So rows that came out non-finite are looked at
+// again (redo_row).  A warp looks at 2 KB of (token, head) rows, 16 bytes a lane and load, and
+// where all is finite that is all it does: 5 us after a prompt of 8192 tokens (295 us with it,
+// 290 without, in turns) as after 1500 rows, so a launch and its wait more than the 33 MB out of
+// L2; by 2-byte loads it was 14 us.
 constexpr int kCheckLoads = 4;
 template <typename IO, int D>
 constexpr int check_rows() { return kCheckLoads * 512 / (D * (int)sizeof(IO)); }
@@ -1895,65 +1903,246 @@ __device__ __forceinline__ bool any_nonfinite16(uint4 c, unsigned e) {
 __device__ __forceinline__ bool any_nonfinite(uint4 c, __nv_bfloat16) { return any_nonfinite16(c, 0x7f80u); }
 __device__ __forceinline__ bool any_nonfinite(uint4 c, __half) { return any_nonfinite16(c, 0x7c00u); }
 
+// N neighbouring elements of a row
+template <typename T, int N>
+struct __align__(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Few {
+    T v[N];
+};
+
+// base + off, or zeros where off is negative (without a branch between an unrolled loop's loads)
+template <typename T, int N>
+__device__ __forceinline__ Few<T, N> row_or_zeros(const char* base, int64_t off) {
+    Few<T, N> x = *reinterpret_cast<const Few<T, N>*>(base + max(off, (int64_t)0));
+#pragma unroll
+    for (int e = 0; e < N; e++) x.v[e] = off < 0 ? (T)0.f : x.v[e];
+    return x;
+}
+
+// Places of keys key0 .. key0 + 31 of sequence b, one a lane; -1 beyond `last` and on a bad page.
+__device__ __forceinline__ int64_t places(const AttnView& a, int b, int key0, int last, int lane) {
+    return key0 + lane <= last ? paged_offset(a.p, b, key0 + lane) : -1;
+}
+
+// The rows of those keys (zeros where there is no place), 16 bytes a lane, through f: a lane has
+// dims kDims * (lane % kLanes) .. of every row it sees.
+template <typename KV, int D>
+struct Chunks {
+    static constexpr int kDims = 16 / (int)sizeof(KV), kLanes = D / kDims, kRows = 32 / kLanes;
+    template <typename F>
+    static __device__ __forceinline__ void each(const char* base, int64_t off, int lane, F f) {
+#pragma unroll
+        for (int j = 0; j < 32 / kRows; j++) {
+            const int64_t o = __shfl_sync(0xffffffffu, off, j * kRows + lane / kLanes);
+            f(row_or_zeros<KV, kDims>(base + lane % kLanes * 16, o));
+        }
+    }
+    template <typename F>  // bit e: test(element e)
+    static __device__ __forceinline__ unsigned bits(const Few<KV, kDims>& x, F test) {
+        unsigned m = 0;
+#pragma unroll
+        for (int e = 0; e < kDims; e++) m |= test((float)x.v[e]) ? 1u << e : 0u;
+        return m;
+    }
+};
+
+// Takes a row with NaN again, by the block's WARPS (an even number, at least 4) warps, each 32
+// keys at a time over what the row sees, in 32 bits as the formula has it: an infinity that is seen
+// stays one, where the products of terms (f32) or of f16 weights made it NaN.  Other elements stay.
+//
+// What is NaN for good is found soon.  The first and the last 32 keys are looked at before all else
+// (a bad prefix has its NaN there, a sequence that went wrong at the row's own position), and those
+// where another row of the sequence and KV head met its NaN (`hint`, verified like the others: any
+// value will do); further keys come from both ends by turns, and the block leaves when the sum of the
+// weights is NaN or every element in question is.  And bf16 products treat what a row sees as the
+// formula does, so a bf16 row is not taken again unless a v of its tile that it does not see is the
+// cause.
+// 16/8 heads, a call without NaN -> with one in the v of (a) the first of 4096 positions of a prompt,
+// (b) one of the last, which 2000 rows of its tile do not see, (c) the middle of 65536 under a chunk of
+// 512: bf16 0.10 -> 0.62, 1.05, 0.38 -> 0.70 ms; f16 0.10 -> 0.58, 1.02, 0.38 -> 20; f32 0.43 -> 0.84,
+// 0.90, 1.7 -> 19 (each row walked by a warp, a key at a time: (a) 36, 36 and 21).  What is left is a row's
+// way through all its keys, 0.3 us a key, paid once a KV head; by every row in an f32 call that sees
+// an infinity and no NaN.
+template <typename IO, typename KV, int D, int WARPS>
+__device__ __forceinline__ void redo_row(const AttnView& a, int token, int head, float (*sums)[D], float2* ml, int* done,
+                                         bool hints) {
+    constexpr int E = D / 32;
+    using C = Chunks<KV, D>;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b = paged_find_seq(a.p.q_start, a.p.batch, token, lane);
+    const PagedSeq s = paged_seq(a.p, b);
+    const int pos = s.len - s.n + token - s.start;
+    if (!s.ok || token < s.start || token >= s.start + s.n || pos < 0) return;  // not a row of this call, or an empty one
+    const int lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
+    const int64_t head_off = (int64_t)(head / a.group) * a.p.stride_head, th = (int64_t)token * a.heads + head;
+    const bool need_l = a.lse && isnan(a.lse[th]);
+    IO* const row = reinterpret_cast<IO*>(a.out + token * a.o_row + head * a.o_head);
+    Few<IO, E> out = *reinterpret_cast<const Few<IO, E>*>(row + lane * E);
+    const Few<IO, C::kDims> part = *reinterpret_cast<const Few<IO, C::kDims>*>(row + lane % C::kLanes * C::kDims);
+    unsigned bad = 0, bad_c = 0;  // elements that are NaN: of `out`, and of the chunk
+#pragma unroll
+    for (int e = 0; e < E; e++) bad |= isnan((float)out.v[e]) ? 1u << e : 0u;
+#pragma unroll
+    for (int e = 0; e < C::kDims; e++) bad_c |= isnan((float)part.v[e]) ? 1u << e : 0u;
+    if (!__any_sync(0xffffffffu, bad != 0)) return;  // (an infinity in a sum is a seen one's)
+    int* const hint = hints ? a.hint + b * a.p.kv_heads + head / a.group : nullptr;
+
+    bool nan_for_good = false;
+    const int met = hint ? *(volatile int*)hint : -1;
+    for (int i = warp; i < 6; i += WARPS) {  // v and k of the first keys, of the last ones, of those from `met` on
+        const int key0 = i < 2 ? lo : i < 4 ? max(lo, pos - 31) : met;
+        if (key0 < lo || key0 > pos) continue;
+        unsigned seen = 0;
+        C::each((i & 1 ? a.p.k : a.p.v) + head_off, places(a, b, key0, pos, lane), lane,
+                [&](const auto& x) { seen |= C::bits(x, [](float y) { return isnan(y); }); });
+#pragma unroll
+        for (int o = C::kLanes; o < 32; o <<= 1) seen |= __shfl_xor_sync(0xffffffffu, seen, o);
+        nan_for_good |= i & 1 ? __any_sync(0xffffffffu, seen != 0) : !need_l && __all_sync(0xffffffffu, (bad_c & ~seen) == 0);
+    }
+    auto leave_nan = [&] {
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            if (bad >> e & 1) out.v[e] = (IO)nanf("");
+        if (warp == 0) *reinterpret_cast<Few<IO, E>*>(row + lane * E) = out;
+    };
+    if (__syncthreads_or(nan_for_good)) {
+        leave_nan();
+        return;
+    }
+    if constexpr (std::is_same<IO, __nv_bfloat16>::value) {
+        const int rows = s.n * a.group, r = (token - s.start) * a.group + head % a.group;
+        const KeyRange kr =
+            rows > a.few_rows ? key_range(a, s, r / a.many.rows * a.many.rows, a.many) : key_range(a, s, 0, a.few);
+        bool hit = false;
+        auto unseen = [&](int first, int last) {
+            for (int key0 = first + warp * 32; key0 <= last && !hit; key0 += WARPS * 32) {
+                C::each(a.p.v + head_off, places(a, b, key0, last, lane), lane,
+                        [&](const auto& x) { hit |= (C::bits(x, [](float y) { return !isfinite(y); }) & bad_c) != 0; });
+                hit = __any_sync(0xffffffffu, hit);
+            }
+        };
+        unseen(pos + 1, kr.hi - 1);
+        unseen(kr.lo, lo - 1);
+        if (!__syncthreads_or(hit)) return;
+    }
+    const Few<IO, E> q8 = *reinterpret_cast<const Few<IO, E>*>(a.q + token * a.q_row + head * a.q_head + lane * E * sizeof(IO));
+    float q[E], o[E] = {}, m = -INFINITY, l = 0.f;  // l: of this lane's keys
+#pragma unroll
+    for (int e = 0; e < E; e++) q[e] = (float)q8.v[e];
+    if (threadIdx.x == 0) *done = 0;
+    __syncthreads();
+    const int n = (pos - lo) / 32 + 1;
+    for (int i = warp; i < n; i += WARPS) {
+        if (*(volatile int*)done) break;
+        const int key0 = lo + 32 * (i & 1 ? n - 1 - (i >> 1) : i >> 1);
+        const int64_t off = places(a, b, key0, pos, lane);
+        const int64_t mine = head_off + (int64_t)lane * E * sizeof(KV);
+        float x = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float d[16];
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const int64_t at = __shfl_sync(0xffffffffu, off, 16 * h + j);
+                const Few<KV, E> k = row_or_zeros<KV, E>(a.p.k + mine, at);
+                d[j] = 0.f;
+#pragma unroll
+                for (int e = 0; e < E; e++) d[j] = fmaf(q[e], (float)k.v[e], d[j]);
+            }
+            const float sum = __shfl_sync(0xffffffffu, warp_sum_scatter<16>(d, lane), 2 * (lane & 15));
+            if (lane >> 4 == h) x = sum;
+        }
+        x = key0 + lane <= pos ? x * a.scale_log2 : -INFINITY;
+        const float mn = fmaxf(m, warp_max(x)), mb = mn == -INFINITY ? 0.f : mn;
+        const float f = ex2_approx(m - mb), w = ex2_approx(x - mb);
+        m = mn;
+        l = fmaf(l, f, w);
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] *= f;
+#pragma unroll 16
+        for (int j = 0; j < 32; j++) {
+            const int64_t at = __shfl_sync(0xffffffffu, off, j);
+            const float wj = __shfl_sync(0xffffffffu, w, j);
+            const Few<KV, E> v = row_or_zeros<KV, E>(a.p.v + mine, at);
+#pragma unroll
+            for (int e = 0; e < E; e++) o[e] = fmaf(wj, (float)v.v[e], o[e]);
+        }
+        bool open = need_l;
+#pragma unroll
+        for (int e = 0; e < E; e++) open |= (bad >> e & 1) && !isnan(o[e]);
+        if (__any_sync(0xffffffffu, isnan(l)) || !__any_sync(0xffffffffu, open)) {
+            if (lane == 0) {
+                *(volatile int*)done = 1;
+                if (hint) *(volatile int*)hint = key0;
+            }
+            break;
+        }
+    }
+    l = warp_sum(l);
+    if (lane == 0) ml[warp] = make_float2(m, l);
+#pragma unroll
+    for (int e = 0; e < E; e++) sums[warp][lane * E + e] = o[e];
+    __syncthreads();
+    if (*done) {
+        leave_nan();
+    } else if (warp == 0) {
+        float M = -INFINITY, L = 0.f, y[E] = {};
+        for (int x = 0; x < WARPS; x++) M = fmaxf(M, ml[x].x);
+        for (int x = 0; x < WARPS; x++) {
+            const float w = ex2_approx(ml[x].x - (M == -INFINITY ? 0.f : M));
+            L = fmaf(ml[x].y, w, L);
+#pragma unroll
+            for (int e = 0; e < E; e++) y[e] = fmaf(w, sums[x][lane * E + e], y[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            if (bad >> e & 1) out.v[e] = (IO)(L == 0.f ? 0.f : y[e] / L);
+        *reinterpret_cast<Few<IO, E>*>(row + lane * E) = out;
+        if (need_l && lane == 0)
+            a.lse[th] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
+    }
+    __syncthreads();  // the shared memory is free for the next row
+}
+
 template <typename IO, typename KV, int D>
-__global__ void __launch_bounds__(128) paged_attn_check_kernel(const __grid_constant__ AttnView a) {
-    constexpr int E = D / 32, kLanes = D * sizeof(IO) / 16, kPass = 32 / kLanes;  // lanes a row, rows a load
+__global__ void __launch_bounds__(128, 8) paged_attn_check_kernel(const __grid_constant__ AttnView a) {
+    constexpr int kLanes = D * sizeof(IO) / 16, kPass = 32 / kLanes, R = check_rows<IO, D>();  // lanes a row, rows a load
+    __shared__ float sums[4][D];
+    __shared__ float2 ml[4];
+    __shared__ unsigned rows[4];
+    __shared__ int done;
     pdl_wait();
     pdl_trigger();
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const unsigned all = (unsigned)(a.p.tokens * (int64_t)a.heads);  // below 2^31
-    const unsigned first = (blockIdx.x * 4 + (threadIdx.x >> 5)) * check_rows<IO, D>();
+    // A load takes kPass rows; those of a block lie far apart, so that the rows of one bad tile are spread over
+    // many blocks.
+    auto row_of = [&](int w, int r) {
+        return ((unsigned)(r / kPass * 4 + w) * gridDim.x + blockIdx.x) * kPass + r % kPass;
+    };
     uint4 y[kCheckLoads];
 #pragma unroll
     for (int i = 0; i < kCheckLoads; i++) {
-        const unsigned th = min(first + i * kPass + lane / kLanes, all - 1), token = th / a.heads, head = th - token * a.heads;
+        const unsigned th = min(row_of(warp, i * kPass) + lane / kLanes, all - 1), token = th / a.heads,
+                       head = th - token * a.heads;
         y[i] = *reinterpret_cast<const uint4*>(a.out + token * a.o_row + head * a.o_head + lane % kLanes * 16);
     }
     unsigned bad[kCheckLoads], any = 0;
 #pragma unroll
     for (int i = 0; i < kCheckLoads; i++) any |= bad[i] = __ballot_sync(0xffffffffu, any_nonfinite(y[i], IO(0.f)));
-    if (any == 0) return;
+    if (!__syncthreads_or(any != 0)) return;
+    unsigned bits = 0;
+#pragma unroll
+    for (int r = 0; r < R; r++)
+        if (bad[r / kPass] >> (r % kPass * kLanes) & (kLanes == 32 ? ~0u : (1u << kLanes % 32) - 1)) bits |= 1u << r;
+    if (lane == 0) rows[warp] = bits;
+    __syncthreads();
 #pragma unroll 1
-    for (int r = 0; r < check_rows<IO, D>(); r++) {
-        unsigned of = 0;
-#pragma unroll
-        for (int i = 0; i < kCheckLoads; i++) of = r / kPass == i ? bad[i] : of;
-        if ((of >> (r % kPass * kLanes) & (kLanes == 32 ? ~0u : (1u << kLanes % 32) - 1)) == 0 || first + r >= all) continue;
-        const int token = (int)((first + r) / a.heads), head = (int)((first + r) % a.heads);
-        const int b = paged_find_seq(a.p.q_start, a.p.batch, token, lane);
-        const PagedSeq s = paged_seq(a.p, b);
-        if (!s.ok || token < s.start || token >= s.start + s.n) continue;  // not a row of this call
-        const int pos = s.len - s.n + token - s.start;
-        const IO* qp = reinterpret_cast<const IO*>(a.q + token * a.q_row + head * a.q_head) + lane * E;
-        const int64_t at = (int64_t)(head / a.group) * a.p.stride_head + (int64_t)lane * E * sizeof(KV);
-        float q[E], o[E] = {}, m = -INFINITY, l = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; e++) q[e] = (float)qp[e];
-        for (int key = a.window > 0 ? max(pos - a.window + 1, 0) : 0; key <= pos; key++) {
-            const int64_t off = paged_offset(a.p, b, key);
-            float k[E] = {}, v[E] = {};
-            if (off >= 0) {
-#pragma unroll
-                for (int e = 0; e < E; e++) {
-                    k[e] = (float)reinterpret_cast<const KV*>(a.p.k + off + at)[e];
-                    v[e] = (float)reinterpret_cast<const KV*>(a.p.v + off + at)[e];
-                }
-            }
-            float x = 0.f;
-#pragma unroll
-            for (int e = 0; e < E; e++) x = fmaf(q[e], k[e], x);
-            x = warp_sum(x) * a.scale_log2;
-            const float mn = fmaxf(m, x), mb = mn == -INFINITY ? 0.f : mn;
-            const float f = ex2_approx(m - mb), w = ex2_approx(x - mb);
-            m = mn;
-            l = fmaf(l, f, w);
-#pragma unroll
-            for (int e = 0; e < E; e++) o[e] = fmaf(o[e], f, w * v[e]);
+    for (int w = 0; w < 4; w++)
+#pragma unroll 1
+        for (unsigned left = rows[w]; left; left &= left - 1) {
+            const unsigned th = row_of(w, __ffs(left) - 1);
+            if (th < all) redo_row<IO, KV, D, 4>(a, (int)(th / a.heads), (int)(th % a.heads), sums, ml, &done, true);
         }
-        IO* dst = reinterpret_cast<IO*>(a.out + token * a.o_row + head * a.o_head) + lane * E;
-#pragma unroll
-        for (int e = 0; e < E; e++) dst[e] = (IO)(l == 0.f ? 0.f : o[e] / l);
-    }
 }
 
 // How the work is cut up: from the host's bounds alone, so that a captured
@@ -2002,14 +2191,16 @@ Plan make_plan(const PagedView& p, int io, int cache, int heads, int D, int wind
     pl.max_splits = tc ? (int)std::min<int64_t>(want, (all + 511) / 512) : 1;
     return pl;
 }
-// The workspace: first the shared-out tiles' pieces, then the splits', then (both kernels) 16 bytes for `ready`.
+// The workspace: first the shared-out tiles' pieces, then the splits', then the hints (4 bytes a sequence and KV
+// head; none for single tokens) and (both kernels) 16 bytes for `ready`.
 bool both_kernels(const Plan& pl) { return pl.few_rows && pl.few_rows != 0x7fffffff; }
 size_t stream_floats(const Plan& pl, int D) { return pl.few_rows ? (size_t)kStreamMost * 2 * pl.few.rows * (D + 2) : 0; }
 size_t split_floats(const Plan& pl, const PagedView& p, int heads, int D) {
     return pl.max_splits > 1 ? (size_t)pl.max_splits * p.tokens * heads * (D + 2) : 0;
 }
+size_t hint_ints(const PagedView& p) { return p.max_new > 1 ? ((size_t)p.batch * p.kv_heads + 3) / 4 * 4 : 0; }
 size_t plan_bytes(const Plan& pl, const PagedView& p, int heads, int D) {
-    return 4 * (stream_floats(pl, D) + split_floats(pl, p, heads, D) + (both_kernels(pl) ? 4 : 0));
+    return 4 * (stream_floats(pl, D) + split_floats(pl, p, heads, D) + hint_ints(p) + (both_kernels(pl) ? 4 : 0));
 }
 
 // Tensor map of a pool as [page][kv head][position][dim], boxes of one page's rows (128 at
@@ -2191,7 +2382,9 @@ extern "C" vb_status vb_paged_attn(const vb_paged_cache* cache, const vb_paged_b
     a.strm_ml = reinterpret_cast<float2*>(a.strm + parts * D);
     a.part = a.strm + stream_floats(pl, D);
     a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)pl.max_splits * a.p.tokens * heads * D);
-    if (both_kernels(pl)) a.ready = reinterpret_cast<unsigned*>(a.part + split_floats(pl, a.p, heads, D));
+    int* const words = reinterpret_cast<int*>(a.part + split_floats(pl, a.p, heads, D));
+    if (hint_ints(a.p)) a.hint = words;
+    if (both_kernels(pl)) a.ready = reinterpret_cast<unsigned*>(words + hint_ints(a.p));
     return D == 128 ? launch_attn<128>(a, io, cache->dtype, as_stream(stream))
                     : launch_attn<64>(a, io, cache->dtype, as_stream(stream));
 }
