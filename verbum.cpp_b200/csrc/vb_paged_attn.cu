@@ -83,7 +83,7 @@ struct AttnView {
     unsigned* ready;    // then: 1 once what came before the call can be read, by the many-rows kernel; else NULL
     int box;            // rows of a page that one TMA copy brings (many rows); 0: no tensor maps
     bool stall;         // test hook (vb_debug_arm_fault): block 0 of the many-rows kernel never has all of its q
-    int* hint;          // [sequence][KV head] where a row that was taken again met a NaN (redo_row); -1 at first
+    int* hint;          // calls of many rows: [sequence][KV head] where a row that was taken again met a NaN (redo_row)
     float* part;        // [split][token][head][D] sums of a split, relative to its maximum
     float2* part_ml;    // [split][token][head] (maximum in base 2, sum of weights)
     float* strm;        // the same of the shared keys: [block][2][tile row][D]
@@ -639,6 +639,7 @@ __global__ void paged_attn_clear_kernel(unsigned* ready) {
     pdl_trigger();
     *ready = 0;
 }
+// (By the many-rows kernel: a loop in the few-rows kernel, reached or not, cost every call of it 4 us.)
 __device__ __forceinline__ void clear_hints(const AttnView& a) {
     if (a.hint && blockIdx.x == 0)
         for (int i = threadIdx.x; i < a.p.batch * a.p.kv_heads; i += blockDim.x) a.hint[i] = -1;
@@ -669,7 +670,6 @@ __global__ void __launch_bounds__(FewCfg<KV, D, NR>::kWarps * 32) paged_attn_few
         pdl_wait();
     }
     pdl_trigger();
-    if (!a.after_many) clear_hints(a);
     struct AtEnd {
         bool wait;
         __device__ ~AtEnd() {
@@ -1984,7 +1984,7 @@ __device__ __forceinline__ void redo_row(const AttnView& a, int token, int head,
 #pragma unroll
     for (int e = 0; e < C::kDims; e++) bad_c |= isnan((float)part.v[e]) ? 1u << e : 0u;
     if (!__any_sync(0xffffffffu, bad != 0)) return;  // (an infinity in a sum is a seen one's)
-    int* const hint = hints ? a.hint + b * a.p.kv_heads + head / a.group : nullptr;
+    int* const hint = hints && a.hint ? a.hint + b * a.p.kv_heads + head / a.group : nullptr;
 
     bool nan_for_good = false;
     const int met = hint ? *(volatile int*)hint : -1;
@@ -2191,16 +2191,18 @@ Plan make_plan(const PagedView& p, int io, int cache, int heads, int D, int wind
     pl.max_splits = tc ? (int)std::min<int64_t>(want, (all + 511) / 512) : 1;
     return pl;
 }
-// The workspace: first the shared-out tiles' pieces, then the splits', then the hints (4 bytes a sequence and KV
-// head; none for single tokens) and (both kernels) 16 bytes for `ready`.
+// The workspace: first the shared-out tiles' pieces, then the splits', then the hints (many rows: 4 bytes a sequence
+// and KV head) and (both kernels) 16 bytes for `ready`.
 bool both_kernels(const Plan& pl) { return pl.few_rows && pl.few_rows != 0x7fffffff; }
 size_t stream_floats(const Plan& pl, int D) { return pl.few_rows ? (size_t)kStreamMost * 2 * pl.few.rows * (D + 2) : 0; }
 size_t split_floats(const Plan& pl, const PagedView& p, int heads, int D) {
     return pl.max_splits > 1 ? (size_t)pl.max_splits * p.tokens * heads * (D + 2) : 0;
 }
-size_t hint_ints(const PagedView& p) { return p.max_new > 1 ? ((size_t)p.batch * p.kv_heads + 3) / 4 * 4 : 0; }
+size_t hint_ints(const Plan& pl, const PagedView& p) {
+    return pl.few_rows != 0x7fffffff ? ((size_t)p.batch * p.kv_heads + 3) / 4 * 4 : 0;
+}
 size_t plan_bytes(const Plan& pl, const PagedView& p, int heads, int D) {
-    return 4 * (stream_floats(pl, D) + split_floats(pl, p, heads, D) + hint_ints(p) + (both_kernels(pl) ? 4 : 0));
+    return 4 * (stream_floats(pl, D) + split_floats(pl, p, heads, D) + hint_ints(pl, p) + (both_kernels(pl) ? 4 : 0));
 }
 
 // Tensor map of a pool as [page][kv head][position][dim], boxes of one page's rows (128 at
@@ -2383,8 +2385,8 @@ extern "C" vb_status vb_paged_attn(const vb_paged_cache* cache, const vb_paged_b
     a.part = a.strm + stream_floats(pl, D);
     a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)pl.max_splits * a.p.tokens * heads * D);
     int* const words = reinterpret_cast<int*>(a.part + split_floats(pl, a.p, heads, D));
-    if (hint_ints(a.p)) a.hint = words;
-    if (both_kernels(pl)) a.ready = reinterpret_cast<unsigned*>(words + hint_ints(a.p));
+    if (hint_ints(pl, a.p)) a.hint = words;
+    if (both_kernels(pl)) a.ready = reinterpret_cast<unsigned*>(words + hint_ints(pl, a.p));
     return D == 128 ? launch_attn<128>(a, io, cache->dtype, as_stream(stream))
                     : launch_attn<64>(a, io, cache->dtype, as_stream(stream));
 }
