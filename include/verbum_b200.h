@@ -303,7 +303,9 @@ VB_API vb_status vb_paged_append(const vb_paged_cache* cache, const vb_paged_bat
  * before): row with position p sees positions j <= p, with window > 0 only
  * j > p - window.  Places that a row does not see -- later tokens of its chunk,
  * positions before its window, behind its sequence's length -- may hold
- * anything, infinities and NaN too.
+ * anything, infinities and NaN too.  What it does see is taken as the formula
+ * has it, in 32 bits: an infinity in v comes out, a score of -inf weighs 0, a
+ * score of +inf or NaN makes the row and its lse NaN.
  * out [tokens][heads][D] = softmax(scale * q.k) v; an empty
  * row gives zeros.  lse (f32 [tokens][heads], may be NULL) gets the natural
  * logarithm of the sum of exp(scale * q.k), -inf for an empty row.  heads is a

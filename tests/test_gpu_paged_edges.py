@@ -110,6 +110,43 @@ def check_formula(s, window=0):
     return out
 
 
+# B sequences of one new token: clusters; shared-out keys; shared-out keys of a long sequence; the
+# kernels of many rows (more query heads a KV head than the other takes)
+SEEN = [(2, 300, 16, 8), (50, 700, 16, 8), (1, 9000, 16, 8), (3, 500, 20, 1), (3, 500, 66, 2)]
+
+
+@pytest.mark.parametrize("io,cache", PAIRS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,ctx,H,KVH", SEEN)
+def test_an_infinity_that_a_decoding_row_sees(io, cache, B, ctx, H, KVH, D):
+    s = Setup([1] * B, [ctx - 3 * b for b in range(B)], io, cache, H=H, KVH=KVH, D=D, seed=B)
+
+    def put(x, b, pos, head, d, value):
+        x[s.table[b, pos // s.page].long(), pos % s.page, head, d] = value
+
+    put(s.v, 0, ctx // 3, 0, 5, math.inf)
+    put(s.v, 0, ctx // 2, 0, 9, -math.inf)
+    put(s.v, B - 1, 0, KVH - 1, D - 1, math.inf)
+    put(s.v, B - 1, 1, KVH - 1, D - 1, -math.inf)  # both: NaN
+    put(s.v, B - 1, 2, KVH - 1, 0, math.nan)
+    put(s.v, B // 2, 7, 0, 2, -math.inf)
+    out = check_formula(s)
+    assert out[0, 0, 5] == math.inf and out[0, 0, 9] == -math.inf and torch.isnan(out[B - 1, H - 1, D - 1])
+    assert torch.isfinite(out[0, 0, 3:5]).all()
+
+
+@pytest.mark.parametrize("io,cache", PAIRS)
+@pytest.mark.parametrize("B,ctx,H,KVH", SEEN)
+def test_a_key_of_minus_infinity(io, cache, B, ctx, H, KVH):
+    # scores of -inf where q is positive: no weight; of +inf (and NaN) where it is negative
+    s = Setup([1] * B, [ctx - 3 * b for b in range(B)], io, cache, H=H, KVH=KVH, seed=B + 1)
+    s.k[s.table[0, 1].long(), 3, 0, 4] = -math.inf
+    s.q[0, :, 4] = s.q[0, :, 4].abs() + 0.5
+    s.q[0, 1, 4] *= -1
+    out = check_formula(s)
+    assert torch.isfinite(out[0, 0]).all() and torch.isnan(out[0, 1]).all()
+
+
 @pytest.mark.parametrize("io,cache", PAIRS)
 @pytest.mark.parametrize("n", [2, 40, 300])
 def test_an_infinity_that_rows_of_a_chunk_see(io, cache, n):
@@ -121,7 +158,7 @@ def test_an_infinity_that_rows_of_a_chunk_see(io, cache, n):
     check_formula(s, window=n + 90)
 
 
-@pytest.mark.parametrize("n", [2, 40, 300])
+@pytest.mark.parametrize("n", [1, 2, 40, 300])
 def test_an_infinity_under_a_weight_that_f16_has_not(n):
     s = Setup([n, 1], [n + 200, 90], "f16", "f16", H=4, KVH=2, seed=n)
     slot = s.table[0, 2].long(), 1  # position 33, seen by all rows of sequence 0

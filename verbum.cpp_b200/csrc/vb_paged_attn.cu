@@ -79,6 +79,8 @@ struct AttnView {
     int few_rows;       // sequences with at most this many rows a KV head run in the few-rows kernel
     Cut few, many;
     int stream;         // blocks that share all keys of the few-rows kernel evenly; 0: clusters of blocks, one a tile
+    bool redo;          // single tokens of a type whose products do not treat what is seen as the formula does:
+                        // no last pass, the few-rows kernel and its join look at their own rows
     bool after_many;    // the few-rows kernel of this call follows its many-rows kernel
     unsigned* ready;    // then: 1 once what came before the call can be read, by the many-rows kernel; else NULL
     int box;            // rows of a page that one TMA copy brings (many rows); 0: no tensor maps
@@ -250,6 +252,216 @@ __device__ __forceinline__ uint32_t mat_t(uint32_t a) {
 // reference, whatever it is.
 template <typename T>
 constexpr float kLift = std::is_same<T, __half>::value ? 6.f : 0.f;
+
+// ------------------------------------------------------------- rows taken again
+// N neighbouring elements of a row
+template <typename T, int N>
+struct __align__(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Few {
+    T v[N];
+};
+
+// base + off, or zeros where off is negative (without a branch between an unrolled loop's loads)
+template <typename T, int N>
+__device__ __forceinline__ Few<T, N> row_or_zeros(const char* base, int64_t off) {
+    Few<T, N> x = *reinterpret_cast<const Few<T, N>*>(base + max(off, (int64_t)0));
+#pragma unroll
+    for (int e = 0; e < N; e++) x.v[e] = off < 0 ? (T)0.f : x.v[e];
+    return x;
+}
+
+// Places of keys key0 .. key0 + 31 of sequence b, one a lane; -1 beyond `last` and on a bad page.
+__device__ __forceinline__ int64_t places(const AttnView& a, int b, int key0, int last, int lane) {
+    return key0 + lane <= last ? paged_offset(a.p, b, key0 + lane) : -1;
+}
+
+// The rows of those keys (zeros where there is no place), 16 bytes a lane, through f: a lane has
+// dims kDims * (lane % kLanes) .. of every row it sees.
+template <typename KV, int D>
+struct Chunks {
+    static constexpr int kDims = 16 / (int)sizeof(KV), kLanes = D / kDims, kRows = 32 / kLanes;
+    template <typename F>
+    static __device__ __forceinline__ void each(const char* base, int64_t off, int lane, F f) {
+#pragma unroll
+        for (int j = 0; j < 32 / kRows; j++) {
+            const int64_t o = __shfl_sync(0xffffffffu, off, j * kRows + lane / kLanes);
+            f(row_or_zeros<KV, kDims>(base + lane % kLanes * 16, o));
+        }
+    }
+    template <typename F>  // bit e: test(element e)
+    static __device__ __forceinline__ unsigned bits(const Few<KV, kDims>& x, F test) {
+        unsigned m = 0;
+#pragma unroll
+        for (int e = 0; e < kDims; e++) m |= test((float)x.v[e]) ? 1u << e : 0u;
+        return m;
+    }
+};
+
+// The products treat what a row sees as the formula does: bf16 weights are 0 only where f32's are.
+template <typename IO>
+constexpr bool kAsSeen = std::is_same<IO, __nv_bfloat16>::value;
+
+// Takes a row with NaN again, by the block's WARPS (an even number, at least 4) warps, each 32
+// keys at a time over what the row sees, in 32 bits as the formula has it: an infinity that is seen
+// stays one, where the products of terms (f32) or of f16 weights made it NaN.  Other elements stay.
+//
+// What is NaN for good is found soon.  The first and the last 32 keys are looked at before all else
+// (a bad prefix has its NaN there, a sequence that went wrong at the row's own position), and those
+// where another row of the sequence and KV head met its NaN (`hint`, verified like the others: any
+// value will do); further keys come from both ends by turns, and the block leaves when the sum of the
+// weights is NaN or every element in question is.  And bf16 products treat what a row sees as the
+// formula does, so a bf16 row is not taken again unless a v of its tile that it does not see is the
+// cause.
+// 16/8 heads, a call without NaN -> with one in the v of (a) the first of 4096 positions of a prompt,
+// (b) one of the last, which 2000 rows of its tile do not see, (c) the middle of 65536 under a chunk of
+// 512: bf16 0.10 -> 0.62, 1.05, 0.38 -> 0.70 ms; f16 0.10 -> 0.58, 1.02, 0.38 -> 20; f32 0.43 -> 0.84,
+// 0.90, 1.7 -> 19 (each row walked by a warp, a key at a time: (a) 36, 36 and 21).  What is left is a row's
+// way through all its keys, 0.3 us a key, paid once a KV head; by every row in an f32 call that sees
+// an infinity and no NaN.
+template <typename IO, typename KV, int D, int WARPS>
+__device__ __forceinline__ void redo_row(const AttnView& a, int token, int head, float (*sums)[D], float2* ml, int* done) {
+    constexpr int E = D / 32;
+    using C = Chunks<KV, D>;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b = paged_find_seq(a.p.q_start, a.p.batch, token, lane);
+    const PagedSeq s = paged_seq(a.p, b);
+    const int pos = s.len - s.n + token - s.start;
+    if (!s.ok || token < s.start || token >= s.start + s.n || pos < 0) return;  // not a row of this call, or an empty one
+    const int lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
+    const int64_t head_off = (int64_t)(head / a.group) * a.p.stride_head, th = (int64_t)token * a.heads + head;
+    const bool need_l = a.lse && isnan(a.lse[th]);
+    IO* const row = reinterpret_cast<IO*>(a.out + token * a.o_row + head * a.o_head);
+    Few<IO, E> out = *reinterpret_cast<const Few<IO, E>*>(row + lane * E);
+    const Few<IO, C::kDims> part = *reinterpret_cast<const Few<IO, C::kDims>*>(row + lane % C::kLanes * C::kDims);
+    unsigned bad = 0, bad_c = 0;  // elements that are NaN: of `out`, and of the chunk
+#pragma unroll
+    for (int e = 0; e < E; e++) bad |= isnan((float)out.v[e]) ? 1u << e : 0u;
+#pragma unroll
+    for (int e = 0; e < C::kDims; e++) bad_c |= isnan((float)part.v[e]) ? 1u << e : 0u;
+    if (!__any_sync(0xffffffffu, bad != 0)) return;  // (an infinity in a sum is a seen one's)
+    int* const hint = a.hint ? a.hint + b * a.p.kv_heads + head / a.group : nullptr;
+
+    bool nan_for_good = false;
+    const int met = hint ? *(volatile int*)hint : -1;
+    for (int i = warp; i < 6; i += WARPS) {  // v and k of the first keys, of the last ones, of those from `met` on
+        const int key0 = i < 2 ? lo : i < 4 ? max(lo, pos - 31) : met;
+        if (key0 < lo || key0 > pos) continue;
+        unsigned seen = 0;
+        C::each((i & 1 ? a.p.k : a.p.v) + head_off, places(a, b, key0, pos, lane), lane,
+                [&](const auto& x) { seen |= C::bits(x, [](float y) { return isnan(y); }); });
+#pragma unroll
+        for (int o = C::kLanes; o < 32; o <<= 1) seen |= __shfl_xor_sync(0xffffffffu, seen, o);
+        nan_for_good |= i & 1 ? __any_sync(0xffffffffu, seen != 0) : !need_l && __all_sync(0xffffffffu, (bad_c & ~seen) == 0);
+    }
+    auto leave_nan = [&] {
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            if (bad >> e & 1) out.v[e] = (IO)nanf("");
+        if (warp == 0) *reinterpret_cast<Few<IO, E>*>(row + lane * E) = out;
+    };
+    if (__syncthreads_or(nan_for_good)) {
+        leave_nan();
+        return;
+    }
+    if constexpr (kAsSeen<IO>) {
+        const int rows = s.n * a.group, r = (token - s.start) * a.group + head % a.group;
+        const KeyRange kr =
+            rows > a.few_rows ? key_range(a, s, r / a.many.rows * a.many.rows, a.many) : key_range(a, s, 0, a.few);
+        bool hit = false;
+        auto unseen = [&](int first, int last) {
+            for (int key0 = first + warp * 32; key0 <= last && !hit; key0 += WARPS * 32) {
+                C::each(a.p.v + head_off, places(a, b, key0, last, lane), lane,
+                        [&](const auto& x) { hit |= (C::bits(x, [](float y) { return !isfinite(y); }) & bad_c) != 0; });
+                hit = __any_sync(0xffffffffu, hit);
+            }
+        };
+        unseen(pos + 1, kr.hi - 1);
+        unseen(kr.lo, lo - 1);
+        if (!__syncthreads_or(hit)) return;
+    }
+    const Few<IO, E> q8 = *reinterpret_cast<const Few<IO, E>*>(a.q + token * a.q_row + head * a.q_head + lane * E * sizeof(IO));
+    float q[E], o[E] = {}, m = -INFINITY, l = 0.f;  // l: of this lane's keys
+#pragma unroll
+    for (int e = 0; e < E; e++) q[e] = (float)q8.v[e];
+    if (threadIdx.x == 0) *done = 0;
+    __syncthreads();
+    const int n = (pos - lo) / 32 + 1;
+    for (int i = warp; i < n; i += WARPS) {
+        if (*(volatile int*)done) break;
+        const int key0 = lo + 32 * (i & 1 ? n - 1 - (i >> 1) : i >> 1);
+        const int64_t off = places(a, b, key0, pos, lane);
+        const int64_t mine = head_off + (int64_t)lane * E * sizeof(KV);
+        float x = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float d[16];
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const int64_t at = __shfl_sync(0xffffffffu, off, 16 * h + j);
+                const Few<KV, E> k = row_or_zeros<KV, E>(a.p.k + mine, at);
+                d[j] = 0.f;
+#pragma unroll
+                for (int e = 0; e < E; e++) d[j] = fmaf(q[e], (float)k.v[e], d[j]);
+            }
+            const float sum = __shfl_sync(0xffffffffu, warp_sum_scatter<16>(d, lane), 2 * (lane & 15));
+            if (lane >> 4 == h) x = sum;
+        }
+        x = key0 + lane <= pos ? x * a.scale_log2 : -INFINITY;
+        const float mn = fmaxf(m, warp_max(x)), mb = mn == -INFINITY ? 0.f : mn;
+        const float f = ex2_approx(m - mb), w = ex2_approx(x - mb);
+        m = mn;
+        l = fmaf(l, f, w);
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] *= f;
+#pragma unroll 16
+        for (int j = 0; j < 32; j++) {
+            const int64_t at = __shfl_sync(0xffffffffu, off, j);
+            const float wj = __shfl_sync(0xffffffffu, w, j);
+            const Few<KV, E> v = row_or_zeros<KV, E>(a.p.v + mine, at);
+#pragma unroll
+            for (int e = 0; e < E; e++) o[e] = fmaf(wj, (float)v.v[e], o[e]);
+        }
+        bool open = need_l;
+#pragma unroll
+        for (int e = 0; e < E; e++) open |= (bad >> e & 1) && !isnan(o[e]);
+        if (__any_sync(0xffffffffu, isnan(l)) || !__any_sync(0xffffffffu, open)) {
+            if (lane == 0) {
+                *(volatile int*)done = 1;
+                if (hint) *(volatile int*)hint = key0;
+            }
+            break;
+        }
+    }
+    l = warp_sum(l);
+    if (lane == 0) ml[warp] = make_float2(m, l);
+#pragma unroll
+    for (int e = 0; e < E; e++) sums[warp][lane * E + e] = o[e];
+    __syncthreads();
+    if (*done) {
+        leave_nan();
+    } else if (warp == 0) {
+        float M = -INFINITY, L = 0.f, y[E] = {};
+        for (int x = 0; x < WARPS; x++) M = fmaxf(M, ml[x].x);
+        for (int x = 0; x < WARPS; x++) {
+            const float w = ex2_approx(ml[x].x - (M == -INFINITY ? 0.f : M));
+            L = fmaf(ml[x].y, w, L);
+#pragma unroll
+            for (int e = 0; e < E; e++) y[e] = fmaf(w, sums[x][lane * E + e], y[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            if (bad >> e & 1) out.v[e] = (IO)(L == 0.f ? 0.f : y[e] / L);
+        *reinterpret_cast<Few<IO, E>*>(row + lane * E) = out;
+        if (need_l && lane == 0)
+            a.lse[th] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
+    }
+    __syncthreads();  // the shared memory is free for the next row
+}
+
+// The same out of line, for kernels that have their registers for something else.
+template <typename IO, typename KV, int D, int WARPS>
+__device__ __noinline__ void redo_row_apart(const AttnView& a, int token, int head, float (*sums)[D], float2* ml, int* done) {
+    redo_row<IO, KV, D, WARPS>(a, token, head, sums, ml, done);
+}
 
 // ------------------------------------------------------------- few rows
 // The same by cutting the bits off: cheaper, for the operand whose other one is rounded
@@ -678,6 +890,7 @@ __global__ void __launch_bounds__(FewCfg<KV, D, NR>::kWarps * 32) paged_attn_few
     } at_end{a.after_many};
     if constexpr (CLUSTER) {
         __shared__ float2 kept[C::kRows];
+        __shared__ int again_done;
         const int rank = (int)cl_rank(), tile = (int)blockIdx.x / kCl;
         const int kvh = tile % a.p.kv_heads, b = tile / a.p.kv_heads;
         const PagedSeq s = paged_seq(a.p, b);
@@ -689,6 +902,7 @@ __global__ void __launch_bounds__(FewCfg<KV, D, NR>::kWarps * 32) paged_attn_few
         const Sink sink{false, true, nullptr, nullptr};
         few_piece<IO, KV, D, NR>(a, s, b, kvh, kr, k_begin, k_end, sink, smem, ml, kept);
         cluster_sync_all();
+        bool again = false;
         for (int it = rank * C::kWarps * 32 + threadIdx.x; it < C::kRows * (D / 4); it += kCl * C::kWarps * 32) {
             const int row = it / (D / 4), d = it % (D / 4) * 4;
             if (row >= rows) break;
@@ -714,10 +928,19 @@ __global__ void __launch_bounds__(FewCfg<KV, D, NR>::kWarps * 32) paged_attn_few
             IO* dst = reinterpret_cast<IO*>(a.out + token * a.o_row + head * a.o_head) + d;
             if (L != 0.f) y.x *= inv, y.y *= inv, y.z *= inv, y.w *= inv;
             dst[0] = (IO)y.x, dst[1] = (IO)y.y, dst[2] = (IO)y.z, dst[3] = (IO)y.w;
+            again |= isnan(y.x + y.y + y.z + y.w);
             if (d == 0 && a.lse)
                 a.lse[(int64_t)token * a.heads + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
         }
         cluster_sync_all();  // no block leaves while others read its shared memory
+        if constexpr (!kAsSeen<IO>) {
+            constexpr int kBlockRows = C::kWarps * 128 / D;  // rows of a block in each turn of the loop
+            if (a.redo && __syncthreads_or(again))
+                for (int i = rank * kBlockRows; i < rows; i += kCl * kBlockRows)
+                    for (int row = i; row < min(i + kBlockRows, rows); row++)
+                        redo_row_apart<IO, KV, D, C::kWarps>(a, s.start + row / a.group, kvh * a.group + row % a.group,
+                                                       reinterpret_cast<float(*)[D]>(smem), ml[0], &again_done);
+        }
     } else {
         // this block's units, piece by piece: a piece is what it has of one tile
         const int lane = threadIdx.x & 31;
@@ -1819,10 +2042,12 @@ __global__ void __launch_bounds__(128) paged_attn_merge_kernel(const __grid_cons
 // block where there are few blocks (a long sequence has dozens of pieces), eight otherwise
 // (every block adds up the batch's lengths).
 constexpr int kJoinWarps = 8;
-template <typename IO, int D, int ROWS>
-__global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const __grid_constant__ AttnView a, int groups) {
+template <typename IO, typename KV, int D, int ROWS>
+__global__ void __launch_bounds__(kJoinWarps * 32, 5) paged_attn_join_kernel(const __grid_constant__ AttnView a, int groups) {
     constexpr int W = kJoinWarps / ROWS;  // warps of a row
     __shared__ float sums[kJoinWarps][D];
+    __shared__ float2 ml[kJoinWarps];
+    __shared__ int done;
     pdl_wait();
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1838,8 +2063,30 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const 
     const int blocks = min(a.stream, all);
     const int c0 = (int)(((int64_t)(u0 + 1) * blocks - 1) / all), c1 = (int)(((int64_t)(u0 + n) * blocks - 1) / all);
     const int used = c1 - c0 + 1;
-    if (used == 1) return;  // written by the kernel itself
     const bool live = r < s.n * a.group;
+    // the block's rows, once they are written: taken again where one has a NaN
+    auto look = [&](bool again) {
+        if constexpr (!kAsSeen<IO>) {
+            const int first = r - warp / W;
+            if (__syncthreads_or(again) && a.redo)
+                for (int row = first; row < min(first + ROWS, s.n * a.group); row++)
+                    redo_row_apart<IO, KV, D, kJoinWarps>(a, s.start + row / a.group, kvh * a.group + row % a.group, sums, ml,
+                                                          &done);
+        }
+    };
+    if (used == 1) {  // written by the kernel itself
+        if constexpr (!kAsSeen<IO>) {
+            bool again = false;
+            if (live && a.redo && warp % W == 0) {
+                const int token = s.start + r / a.group, head = kvh * a.group + r % a.group;
+                const IO* y = reinterpret_cast<const IO*>(a.out + token * a.o_row + head * a.o_head);
+#pragma unroll
+                for (int e = 0; e < D / 32; e++) again |= isnan((float)y[lane + 32 * e]);
+            }
+            look(again);
+        }
+        return;
+    }
     // slot 1 of block c0, then slot 0 of the next ones
     auto at = [&](int x) { return ((int64_t)(c0 + x) * 2 + (x == 0)) * a.few.rows + r; };
     float M = -INFINITY, L = 0.f;
@@ -1865,19 +2112,23 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const 
 #pragma unroll
     for (int e = 0; e < E; e++) sums[warp][lane * E + e] = y[e];
     __syncthreads();
-    if (!live || warp % W) return;
-    const int token = s.start + r / a.group, head = kvh * a.group + r % a.group;
-    const float inv = 1.f / L;
-    IO* dst = reinterpret_cast<IO*>(a.out + token * a.o_row + head * a.o_head);
+    bool again = false;
+    if (live && warp % W == 0) {
+        const int token = s.start + r / a.group, head = kvh * a.group + r % a.group;
+        const float inv = 1.f / L;
+        IO* dst = reinterpret_cast<IO*>(a.out + token * a.o_row + head * a.o_head);
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        float z = 0.f;
+        for (int e = 0; e < E; e++) {
+            float z = 0.f;
 #pragma unroll
-        for (int x = 0; x < W; x++) z += sums[warp + x][lane + 32 * e];
-        dst[lane + 32 * e] = (IO)(L == 0.f ? 0.f : z * inv);
+            for (int x = 0; x < W; x++) z += sums[warp + x][lane + 32 * e];
+            dst[lane + 32 * e] = (IO)(L == 0.f ? 0.f : z * inv);
+            again |= isnan(z * inv) && L != 0.f;
+        }
+        if (a.lse && lane == 0)
+            a.lse[(int64_t)token * a.heads + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
     }
-    if (a.lse && lane == 0)
-        a.lse[(int64_t)token * a.heads + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
+    look(again);
 }
 
 // A tile's rows of several tokens see different keys, and a weight of 0 times an infinity or
@@ -1902,206 +2153,6 @@ __device__ __forceinline__ bool any_nonfinite16(uint4 c, unsigned e) {
 }
 __device__ __forceinline__ bool any_nonfinite(uint4 c, __nv_bfloat16) { return any_nonfinite16(c, 0x7f80u); }
 __device__ __forceinline__ bool any_nonfinite(uint4 c, __half) { return any_nonfinite16(c, 0x7c00u); }
-
-// N neighbouring elements of a row
-template <typename T, int N>
-struct __align__(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Few {
-    T v[N];
-};
-
-// base + off, or zeros where off is negative (without a branch between an unrolled loop's loads)
-template <typename T, int N>
-__device__ __forceinline__ Few<T, N> row_or_zeros(const char* base, int64_t off) {
-    Few<T, N> x = *reinterpret_cast<const Few<T, N>*>(base + max(off, (int64_t)0));
-#pragma unroll
-    for (int e = 0; e < N; e++) x.v[e] = off < 0 ? (T)0.f : x.v[e];
-    return x;
-}
-
-// Places of keys key0 .. key0 + 31 of sequence b, one a lane; -1 beyond `last` and on a bad page.
-__device__ __forceinline__ int64_t places(const AttnView& a, int b, int key0, int last, int lane) {
-    return key0 + lane <= last ? paged_offset(a.p, b, key0 + lane) : -1;
-}
-
-// The rows of those keys (zeros where there is no place), 16 bytes a lane, through f: a lane has
-// dims kDims * (lane % kLanes) .. of every row it sees.
-template <typename KV, int D>
-struct Chunks {
-    static constexpr int kDims = 16 / (int)sizeof(KV), kLanes = D / kDims, kRows = 32 / kLanes;
-    template <typename F>
-    static __device__ __forceinline__ void each(const char* base, int64_t off, int lane, F f) {
-#pragma unroll
-        for (int j = 0; j < 32 / kRows; j++) {
-            const int64_t o = __shfl_sync(0xffffffffu, off, j * kRows + lane / kLanes);
-            f(row_or_zeros<KV, kDims>(base + lane % kLanes * 16, o));
-        }
-    }
-    template <typename F>  // bit e: test(element e)
-    static __device__ __forceinline__ unsigned bits(const Few<KV, kDims>& x, F test) {
-        unsigned m = 0;
-#pragma unroll
-        for (int e = 0; e < kDims; e++) m |= test((float)x.v[e]) ? 1u << e : 0u;
-        return m;
-    }
-};
-
-// Takes a row with NaN again, by the block's WARPS (an even number, at least 4) warps, each 32
-// keys at a time over what the row sees, in 32 bits as the formula has it: an infinity that is seen
-// stays one, where the products of terms (f32) or of f16 weights made it NaN.  Other elements stay.
-//
-// What is NaN for good is found soon.  The first and the last 32 keys are looked at before all else
-// (a bad prefix has its NaN there, a sequence that went wrong at the row's own position), and those
-// where another row of the sequence and KV head met its NaN (`hint`, verified like the others: any
-// value will do); further keys come from both ends by turns, and the block leaves when the sum of the
-// weights is NaN or every element in question is.  And bf16 products treat what a row sees as the
-// formula does, so a bf16 row is not taken again unless a v of its tile that it does not see is the
-// cause.
-// 16/8 heads, a call without NaN -> with one in the v of (a) the first of 4096 positions of a prompt,
-// (b) one of the last, which 2000 rows of its tile do not see, (c) the middle of 65536 under a chunk of
-// 512: bf16 0.10 -> 0.62, 1.05, 0.38 -> 0.70 ms; f16 0.10 -> 0.58, 1.02, 0.38 -> 20; f32 0.43 -> 0.84,
-// 0.90, 1.7 -> 19 (each row walked by a warp, a key at a time: (a) 36, 36 and 21).  What is left is a row's
-// way through all its keys, 0.3 us a key, paid once a KV head; by every row in an f32 call that sees
-// an infinity and no NaN.
-template <typename IO, typename KV, int D, int WARPS>
-__device__ __forceinline__ void redo_row(const AttnView& a, int token, int head, float (*sums)[D], float2* ml, int* done,
-                                         bool hints) {
-    constexpr int E = D / 32;
-    using C = Chunks<KV, D>;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int b = paged_find_seq(a.p.q_start, a.p.batch, token, lane);
-    const PagedSeq s = paged_seq(a.p, b);
-    const int pos = s.len - s.n + token - s.start;
-    if (!s.ok || token < s.start || token >= s.start + s.n || pos < 0) return;  // not a row of this call, or an empty one
-    const int lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
-    const int64_t head_off = (int64_t)(head / a.group) * a.p.stride_head, th = (int64_t)token * a.heads + head;
-    const bool need_l = a.lse && isnan(a.lse[th]);
-    IO* const row = reinterpret_cast<IO*>(a.out + token * a.o_row + head * a.o_head);
-    Few<IO, E> out = *reinterpret_cast<const Few<IO, E>*>(row + lane * E);
-    const Few<IO, C::kDims> part = *reinterpret_cast<const Few<IO, C::kDims>*>(row + lane % C::kLanes * C::kDims);
-    unsigned bad = 0, bad_c = 0;  // elements that are NaN: of `out`, and of the chunk
-#pragma unroll
-    for (int e = 0; e < E; e++) bad |= isnan((float)out.v[e]) ? 1u << e : 0u;
-#pragma unroll
-    for (int e = 0; e < C::kDims; e++) bad_c |= isnan((float)part.v[e]) ? 1u << e : 0u;
-    if (!__any_sync(0xffffffffu, bad != 0)) return;  // (an infinity in a sum is a seen one's)
-    int* const hint = hints && a.hint ? a.hint + b * a.p.kv_heads + head / a.group : nullptr;
-
-    bool nan_for_good = false;
-    const int met = hint ? *(volatile int*)hint : -1;
-    for (int i = warp; i < 6; i += WARPS) {  // v and k of the first keys, of the last ones, of those from `met` on
-        const int key0 = i < 2 ? lo : i < 4 ? max(lo, pos - 31) : met;
-        if (key0 < lo || key0 > pos) continue;
-        unsigned seen = 0;
-        C::each((i & 1 ? a.p.k : a.p.v) + head_off, places(a, b, key0, pos, lane), lane,
-                [&](const auto& x) { seen |= C::bits(x, [](float y) { return isnan(y); }); });
-#pragma unroll
-        for (int o = C::kLanes; o < 32; o <<= 1) seen |= __shfl_xor_sync(0xffffffffu, seen, o);
-        nan_for_good |= i & 1 ? __any_sync(0xffffffffu, seen != 0) : !need_l && __all_sync(0xffffffffu, (bad_c & ~seen) == 0);
-    }
-    auto leave_nan = [&] {
-#pragma unroll
-        for (int e = 0; e < E; e++)
-            if (bad >> e & 1) out.v[e] = (IO)nanf("");
-        if (warp == 0) *reinterpret_cast<Few<IO, E>*>(row + lane * E) = out;
-    };
-    if (__syncthreads_or(nan_for_good)) {
-        leave_nan();
-        return;
-    }
-    if constexpr (std::is_same<IO, __nv_bfloat16>::value) {
-        const int rows = s.n * a.group, r = (token - s.start) * a.group + head % a.group;
-        const KeyRange kr =
-            rows > a.few_rows ? key_range(a, s, r / a.many.rows * a.many.rows, a.many) : key_range(a, s, 0, a.few);
-        bool hit = false;
-        auto unseen = [&](int first, int last) {
-            for (int key0 = first + warp * 32; key0 <= last && !hit; key0 += WARPS * 32) {
-                C::each(a.p.v + head_off, places(a, b, key0, last, lane), lane,
-                        [&](const auto& x) { hit |= (C::bits(x, [](float y) { return !isfinite(y); }) & bad_c) != 0; });
-                hit = __any_sync(0xffffffffu, hit);
-            }
-        };
-        unseen(pos + 1, kr.hi - 1);
-        unseen(kr.lo, lo - 1);
-        if (!__syncthreads_or(hit)) return;
-    }
-    const Few<IO, E> q8 = *reinterpret_cast<const Few<IO, E>*>(a.q + token * a.q_row + head * a.q_head + lane * E * sizeof(IO));
-    float q[E], o[E] = {}, m = -INFINITY, l = 0.f;  // l: of this lane's keys
-#pragma unroll
-    for (int e = 0; e < E; e++) q[e] = (float)q8.v[e];
-    if (threadIdx.x == 0) *done = 0;
-    __syncthreads();
-    const int n = (pos - lo) / 32 + 1;
-    for (int i = warp; i < n; i += WARPS) {
-        if (*(volatile int*)done) break;
-        const int key0 = lo + 32 * (i & 1 ? n - 1 - (i >> 1) : i >> 1);
-        const int64_t off = places(a, b, key0, pos, lane);
-        const int64_t mine = head_off + (int64_t)lane * E * sizeof(KV);
-        float x = 0.f;
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            float d[16];
-#pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const int64_t at = __shfl_sync(0xffffffffu, off, 16 * h + j);
-                const Few<KV, E> k = row_or_zeros<KV, E>(a.p.k + mine, at);
-                d[j] = 0.f;
-#pragma unroll
-                for (int e = 0; e < E; e++) d[j] = fmaf(q[e], (float)k.v[e], d[j]);
-            }
-            const float sum = __shfl_sync(0xffffffffu, warp_sum_scatter<16>(d, lane), 2 * (lane & 15));
-            if (lane >> 4 == h) x = sum;
-        }
-        x = key0 + lane <= pos ? x * a.scale_log2 : -INFINITY;
-        const float mn = fmaxf(m, warp_max(x)), mb = mn == -INFINITY ? 0.f : mn;
-        const float f = ex2_approx(m - mb), w = ex2_approx(x - mb);
-        m = mn;
-        l = fmaf(l, f, w);
-#pragma unroll
-        for (int e = 0; e < E; e++) o[e] *= f;
-#pragma unroll 16
-        for (int j = 0; j < 32; j++) {
-            const int64_t at = __shfl_sync(0xffffffffu, off, j);
-            const float wj = __shfl_sync(0xffffffffu, w, j);
-            const Few<KV, E> v = row_or_zeros<KV, E>(a.p.v + mine, at);
-#pragma unroll
-            for (int e = 0; e < E; e++) o[e] = fmaf(wj, (float)v.v[e], o[e]);
-        }
-        bool open = need_l;
-#pragma unroll
-        for (int e = 0; e < E; e++) open |= (bad >> e & 1) && !isnan(o[e]);
-        if (__any_sync(0xffffffffu, isnan(l)) || !__any_sync(0xffffffffu, open)) {
-            if (lane == 0) {
-                *(volatile int*)done = 1;
-                if (hint) *(volatile int*)hint = key0;
-            }
-            break;
-        }
-    }
-    l = warp_sum(l);
-    if (lane == 0) ml[warp] = make_float2(m, l);
-#pragma unroll
-    for (int e = 0; e < E; e++) sums[warp][lane * E + e] = o[e];
-    __syncthreads();
-    if (*done) {
-        leave_nan();
-    } else if (warp == 0) {
-        float M = -INFINITY, L = 0.f, y[E] = {};
-        for (int x = 0; x < WARPS; x++) M = fmaxf(M, ml[x].x);
-        for (int x = 0; x < WARPS; x++) {
-            const float w = ex2_approx(ml[x].x - (M == -INFINITY ? 0.f : M));
-            L = fmaf(ml[x].y, w, L);
-#pragma unroll
-            for (int e = 0; e < E; e++) y[e] = fmaf(w, sums[x][lane * E + e], y[e]);
-        }
-#pragma unroll
-        for (int e = 0; e < E; e++)
-            if (bad >> e & 1) out.v[e] = (IO)(L == 0.f ? 0.f : y[e] / L);
-        *reinterpret_cast<Few<IO, E>*>(row + lane * E) = out;
-        if (need_l && lane == 0)
-            a.lse[th] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
-    }
-    __syncthreads();  // the shared memory is free for the next row
-}
 
 template <typename IO, typename KV, int D>
 __global__ void __launch_bounds__(128, 8) paged_attn_check_kernel(const __grid_constant__ AttnView a) {
@@ -2141,7 +2192,7 @@ __global__ void __launch_bounds__(128, 8) paged_attn_check_kernel(const __grid_c
 #pragma unroll 1
         for (unsigned left = rows[w]; left; left &= left - 1) {
             const unsigned th = row_of(w, __ffs(left) - 1);
-            if (th < all) redo_row<IO, KV, D, 4>(a, (int)(th / a.heads), (int)(th % a.heads), sums, ml, &done, true);
+            if (th < all) redo_row<IO, KV, D, 4>(a, (int)(th / a.heads), (int)(th % a.heads), sums, ml, &done);
         }
 }
 
@@ -2301,8 +2352,8 @@ vb_status launch_attn(const AttnView& a, cudaStream_t s) {
         const int groups = one ? rows : (rows + 7) / 8;
         if (heads * groups > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
         const dim3 grid((unsigned)(heads * groups)), block(kJoinWarps * 32);
-        e = one ? launch_pdl(paged_attn_join_kernel<IO, D, 1>, grid, block, 0, s, a, groups)
-                : launch_pdl(paged_attn_join_kernel<IO, D, 8>, grid, block, 0, s, a, groups);
+        e = one ? launch_pdl(paged_attn_join_kernel<IO, KV, D, 1>, grid, block, 0, s, a, groups)
+                : launch_pdl(paged_attn_join_kernel<IO, KV, D, 8>, grid, block, 0, s, a, groups);
         if (e != cudaSuccess) return cuda_fail(e, "paged_attn_join_kernel");
     }
     if (a.many.splits > 1) {
@@ -2311,7 +2362,7 @@ vb_status launch_attn(const AttnView& a, cudaStream_t s) {
         e = launch_pdl(paged_attn_merge_kernel<IO, D>, dim3((unsigned)grid), dim3(128), 0, s, a);
         if (e != cudaSuccess) return cuda_fail(e, "paged_attn_merge_kernel");
     }
-    if (a.p.max_new > 1) {
+    if (a.p.max_new > 1 || (a.few_rows != 0x7fffffff && !kAsSeen<IO>)) {  // (see AttnView::redo)
         constexpr int kBlockRows = 4 * check_rows<IO, D>();
         const int64_t grid = ((int64_t)a.p.tokens * a.heads + kBlockRows - 1) / kBlockRows;
         e = launch_pdl(paged_attn_check_kernel<IO, KV, D>, dim3((unsigned)grid), dim3(128), 0, s, a);
@@ -2376,6 +2427,7 @@ extern "C" vb_status vb_paged_attn(const vb_paged_cache* cache, const vb_paged_b
     a.scale_log2 = (scale == 0.f ? 1.17549435e-38f : scale) * 1.44269504088896341f;
     a.window = window;
     a.few_rows = pl.few_rows;
+    a.redo = a.p.max_new == 1 && pl.few_rows == 0x7fffffff;
     a.few = pl.few;
     a.many = pl.many;
     a.stream = pl.stream;
