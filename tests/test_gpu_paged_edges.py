@@ -1,4 +1,5 @@
 """Calls of the paged operators at the edges of what their interface allows."""
+import ctypes as C
 import math
 import time
 
@@ -208,6 +209,34 @@ def test_a_nan_that_rows_see_costs_little(io, cache, what, where):
     assert torch.equal(out[n:], keep[n:])
     print(f"{io} {cache} {what} {where}: {clean:.3f} -> {bad:.3f} ms")
     assert bad < 4 * clean + 1.0, (clean, bad)
+
+
+# ---------------------------------------------------------------- launches
+
+def launches(call):
+    """How many nodes a call captures as."""
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    n = C.c_size_t()
+    assert C.CDLL("libcuda.so.1").cuGraphGetNodes(C.c_void_p(graph.raw_cuda_graph()), None, C.byref(n)) == 0
+    return n.value
+
+
+@pytest.mark.parametrize("io,cache", PAIRS)
+def test_one_long_prompt_launches_no_join(io, cache):
+    # one sequence alone has no keys that are shared out, however many it has
+    def count(ctx):
+        s = Setup([300], [ctx], io, cache, H=16, KVH=8, seed=1)
+        ws, out = vb200.paged_attn_workspace(s.pc, s.pb, s.H), s.out()
+        return launches(lambda: vb200.paged_attn(s.pc, s.pb, s.q, out, workspace=ws))
+
+    assert count(5000) == count(4000) >= 2
 
 
 # ------------------------------------------------------ a wait that gives up

@@ -2345,7 +2345,7 @@ vb_status launch_attn(const AttnView& a, cudaStream_t s) {
         }
         if (st) return st;
     }
-    if (a.stream > 1) {
+    if (a.few_rows && a.stream) {  // (one sequence alone on the many-rows kernel has nothing shared out)
         const int rows = (int)std::min<int64_t>(a.few.rows, (int64_t)a.p.max_new * a.group);
         const int64_t heads = (int64_t)a.p.batch * a.p.kv_heads;
         const bool one = heads * rows <= 2048;
