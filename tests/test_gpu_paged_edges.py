@@ -239,6 +239,20 @@ def test_one_long_prompt_launches_no_join(io, cache):
     assert count(5000) == count(4000) >= 2
 
 
+@pytest.mark.parametrize("io,cache", PAIRS)
+@pytest.mark.parametrize("D", [64, 128])
+def test_clusters_are_used_while_all_fit_the_card(io, cache, D):
+    # one launch; shared-out keys take a second one, the join
+    def count(B):
+        s = Setup([1] * B, [300] * B, io, cache, H=2, KVH=1, D=D, seed=B)
+        check_attn(s)
+        ws, out = vb200.paged_attn_workspace(s.pc, s.pb, s.H), s.out()
+        return launches(lambda: vb200.paged_attn(s.pc, s.pb, s.q, out, workspace=ws))
+
+    most = 15 if cache == "f32" and D == 128 else 37
+    assert count(most) == 1 and count(most + 1) == 2
+
+
 # ------------------------------------------------------ a wait that gives up
 
 @pytest.mark.parametrize("io,cache", PAIRS)

@@ -2228,8 +2228,10 @@ Plan make_plan(const PagedView& p, int io, int cache, int heads, int D, int wind
     const int64_t keys = span(pl.few.rows, 16);
     // Clusters where all fit the card at once and a block's share is at most 512 keys: one token of
     // one sequence of 777 keys takes one launch and 7.2 us of its caller instead of two and 9.8.
-    // Else as many blocks as the card runs at a time.
-    if ((int64_t)p.batch * p.kv_heads * kCl > 148 * 2 || keys > kCl * 512)
+    // Else as many blocks as the card runs at a time.  37 clusters fit (bf16, 37 tiles of 2000 keys:
+    // 8.4 us against 12.2 shared out); of f32 at D = 128, a block an SM, 15 (15 tiles of 2000 keys:
+    // 10.1 against 16.7; 16, in two waves: 18.8 against 16.3, of 4000: 31.0 against 21.2).
+    if ((int64_t)p.batch * p.kv_heads > (cache == VB_F32 && D == 128 ? 15 : 37) || keys > kCl * 512)
         pl.stream = (int)std::min<int64_t>(cache == VB_F32 && D == 128 ? 148 : kStreamMost,
                                            (int64_t)p.batch * p.kv_heads * ((keys + kUnit - 1) / kUnit));
     // many rows: one CTA for each SM, of at least 512 keys
