@@ -308,7 +308,8 @@ VB_API vb_status vb_paged_append(const vb_paged_cache* cache, const vb_paged_bat
  * score of +inf or NaN makes the row and its lse NaN.
  * out [tokens][heads][D] = softmax(scale * q.k) v; an empty
  * row gives zeros.  lse (f32 [tokens][heads], may be NULL) gets the natural
- * logarithm of the sum of exp(scale * q.k), -inf for an empty row.  heads is a
+ * logarithm of the sum of exp(scale * q.k), -inf for an empty row.  out and lse
+ * must not overlap q.  heads is a
  * multiple of kv_heads; query heads h*G .. h*G + G-1 read KV head h.  io as in
  * vb_paged_append.  workspace: vb_paged_attn_workspace_bytes() bytes (the same
  * for every io and window), 16-byte aligned, no initial contents; calls that

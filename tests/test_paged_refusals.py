@@ -132,6 +132,12 @@ def test_logits_arguments():
     assert vb200.lib().vb_logits_process(A, 100, A, 100, 0, 2, 100, None, None) == -1
 
 
+def test_attention_does_not_run_in_place():
+    # a row with an infinity or NaN in it is taken again from its q
+    assert attn(q=A, out=A) == -1
+    assert b"place" in vb200.lib().vb_last_error()
+
+
 def test_python_faces_refuse_what_is_not_on_the_device():
     torch = pytest.importorskip("torch")
     k = torch.zeros(4, 16, 2, 128)

@@ -2419,6 +2419,8 @@ extern "C" vb_status vb_paged_attn(const vb_paged_cache* cache, const vb_paged_b
     const size_t need = plan_bytes(pl, a.p, heads, D);
     if (need > workspace_bytes || (need && !workspace))
         return fail(VB_ERR_ARG, "paged_attn: the workspace is too small");
+    // (a row that is taken again reads its q when the output has been written)
+    if (q == out) return fail(VB_ERR_ARG, "paged_attn: not in place");
     a.q = static_cast<const char*>(q);
     a.out = static_cast<char*>(out);
     a.q_row = q_row * es, a.q_head = q_head * es, a.o_row = o_row * es, a.o_head = o_head * es;
