@@ -138,6 +138,20 @@ def test_attention_does_not_run_in_place():
     assert b"place" in vb200.lib().vb_last_error()
 
 
+def test_addresses_that_do_not_fit_their_elements():
+    # refused here: on the device an access at such an address is a fault
+    for n in ("q_start", "lens", "table", "status"):
+        assert attn(b=batch(**{n: A + 2})) == -9 and append(b=batch(**{n: A + 1})) == -9, n
+    assert attn(lse=A + 2) == -9
+    for dtype, off in ((0, 2), (0, 1), (1, 1), (2, 1)):
+        assert logits(dtype=dtype, p=A + off) == -9 and logits(dtype=dtype, out=2 * A + off) == -9
+    lists = dict(hist_start=A, hist_ids=A, hist_total=4, prompt_len=A, repetition=A, frequency=A, presence=A, bias_start=A,
+                 bias_ids=A, bias_vals=A, bias_total=4, mask=A, mask_stride=4)
+    for n, v in lists.items():
+        if v == A:
+            assert logits(**dict(lists, **{n: A + 2})) == -9, n
+
+
 def test_python_faces_refuse_what_is_not_on_the_device():
     torch = pytest.importorskip("torch")
     k = torch.zeros(4, 16, 2, 128)

@@ -239,6 +239,10 @@ extern "C" vb_status vb_logits_process(const void* logits, int64_t stride_in, vo
         return fail(VB_ERR_ARG, "null pointer");
     if (r.mask && rows > 1 && r.mask_stride < (vocab + 31) / 32)
         return fail(VB_ERR_ARG, "logits_process: mask rows overlap");
+    if ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) % es ||
+        !paged_words({r.hist_start, r.hist_ids, r.prompt_len, r.repetition, r.frequency, r.presence, r.bias_start, r.bias_ids,
+                      r.bias_vals, r.mask}))
+        return fail(VB_ERR_UNSUPPORTED, "logits_process: arrays aligned to their elements required");
     LogitsArgs a{};
     a.in = static_cast<const char*>(logits);
     a.out = static_cast<char*>(out);

@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <initializer_list>
+
 #include "vb_common.cuh"
 
 namespace vb {
@@ -29,6 +31,11 @@ inline int paged_elem_bytes(int dtype) { return dtype == VB_F32 ? 4 : dtype == V
 // Checks of what the host can see; fills the view (vb_paged_attn.cu).
 vb_status paged_view(const vb_paged_cache* cache, const vb_paged_batch* batch, int io, int heads, const char* who,
                      PagedView* out);
+inline bool paged_words(std::initializer_list<const void*> p) {  // addresses (or NULL) of 4-byte elements
+    uintptr_t bits = 0;
+    for (const void* x : p) bits |= reinterpret_cast<uintptr_t>(x);
+    return (bits & 3u) == 0;
+}
 inline bool paged_aligned(const void* p, int64_t row, int64_t head, int elem) {
     return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(row * elem) | (uintptr_t)(head * elem)) & 15u) == 0;
 }

@@ -32,6 +32,8 @@ vb_status paged_view(const vb_paged_cache* c, const vb_paged_batch* b, int io, i
         return refuse(VB_ERR_UNSUPPORTED, "16-byte alignment required");
     if (b->batch < 0 || b->tokens < 0 || b->max_new < 0 || b->max_len < 0 || b->table_stride < 0)
         return refuse(VB_ERR_ARG, "negative size");
+    if (!paged_words({b->q_start, b->lens, b->table, b->status}))
+        return refuse(VB_ERR_UNSUPPORTED, "4-byte alignment required");
     if (b->batch && b->tokens) {
         if (!b->q_start || !b->lens || (b->max_len && !b->table)) return refuse(VB_ERR_ARG, "null pointer");
         if (b->max_len > (int64_t)b->table_stride * c->page_size)
@@ -2411,6 +2413,7 @@ extern "C" vb_status vb_paged_attn(const vb_paged_cache* cache, const vb_paged_b
     const int es = paged_elem_bytes(io), D = cache->head_dim;
     if (!paged_aligned(q, q_row, q_head, es) || !paged_aligned(out, o_row, o_head, es) || !paged_aligned(workspace, 0, 0, 1))
         return fail(VB_ERR_UNSUPPORTED, "paged_attn: 16-byte alignment required");
+    if (!paged_words({lse})) return fail(VB_ERR_UNSUPPORTED, "paged_attn: 4-byte alignment required");
     if ((int64_t)batch->tokens * heads > 0x7fffffff) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
     const Plan pl = make_plan(a.p, io, cache->dtype, heads, D, window);
     // the units of shared-out keys are counted in 32 bits
