@@ -310,7 +310,7 @@ VB_API vb_status vb_paged_append(const vb_paged_cache* cache, const vb_paged_bat
  * row gives zeros.  lse (f32 [tokens][heads], may be NULL) gets the natural
  * logarithm of the sum of exp(scale * q.k), -inf for an empty row.  out and lse
  * must not overlap q.  heads is a
- * multiple of kv_heads; query heads h*G .. h*G + G-1 read KV head h.  io as in
+ * multiple of kv_heads, max_len at most 2^30; query heads h*G .. h*G + G-1 read KV head h.  io as in
  * vb_paged_append.  workspace: vb_paged_attn_workspace_bytes() bytes (the same
  * for every io and window), 16-byte aligned, no initial contents; calls that
  * may overlap need their own. */

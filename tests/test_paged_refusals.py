@@ -152,6 +152,13 @@ def test_addresses_that_do_not_fit_their_elements():
             assert logits(**dict(lists, **{n: A + 2})) == -9, n
 
 
+def test_positions_stay_far_from_32_bits():
+    # tiles of keys are counted past the last position
+    b = batch(max_len=(1 << 30) + 1, table_stride=1 << 30)
+    assert attn(b=b) == -9 and b"keys" in vb200.lib().vb_last_error()
+    assert attn(b=batch(max_len=0x7fffffff, table_stride=1 << 30)) == -9
+
+
 def test_python_faces_refuse_what_is_not_on_the_device():
     torch = pytest.importorskip("torch")
     k = torch.zeros(4, 16, 2, 128)

@@ -2416,8 +2416,9 @@ extern "C" vb_status vb_paged_attn(const vb_paged_cache* cache, const vb_paged_b
     if (!paged_words({lse})) return fail(VB_ERR_UNSUPPORTED, "paged_attn: 4-byte alignment required");
     if ((int64_t)batch->tokens * heads > 0x7fffffff) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
     const Plan pl = make_plan(a.p, io, cache->dtype, heads, D, window);
-    // the units of shared-out keys are counted in 32 bits
-    if ((int64_t)a.p.batch * a.p.kv_heads * ((int64_t)a.p.max_len / kUnit + 1) > 0x3fffffff)
+    // positions up to a tile past the last one, and the units of shared-out keys, are counted in 32 bits
+    if (a.p.max_len > 0x40000000 ||
+        (int64_t)a.p.batch * a.p.kv_heads * ((int64_t)a.p.max_len / kUnit + 1) > 0x3fffffff)
         return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many keys");
     const size_t need = plan_bytes(pl, a.p, heads, D);
     if (need > workspace_bytes || (need && !workspace))
