@@ -61,6 +61,28 @@ def test_every_bad_sequence_is_reported(call, kind):
         assert _status(s, call, max_new=max(news) - 1) == rows
 
 
+def test_python_faces_refuse_with_their_own_error():
+    i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32, device="cuda")
+    f32 = lambda *shape: torch.zeros(shape, device="cuda")
+    s = Setup([1, 2], [20, 30], "bf16", "bf16", seed=1)
+    out = s.out()
+    x, y = f32(2, 500), f32(2, 500)
+    for call in (lambda: vb200.LogitsRules(mask=i32(16)), lambda: vb200.LogitsRules(mask=i32()),
+                 lambda: vb200.LogitsRules(mask=i32(2, 4, 4)), lambda: vb200.LogitsRules(prompt_len=i32()),
+                 lambda: vb200.LogitsRules(hist_start=i32(3), hist_ids=i32(2, 2)),
+                 lambda: vb200.LogitsRules(bias_start=i32(3), bias_ids=i32(4), bias_vals=f32(5)),
+                 lambda: vb200.logits_process(x[0], y[0], vb200.LogitsRules()),
+                 lambda: vb200.logits_process(x, y[:1], vb200.LogitsRules()),
+                 lambda: vb200.paged_attn(s.pc, s.pb, s.q[:, 0], out), lambda: vb200.paged_attn(s.pc, s.pb, s.q, s.q),
+                 lambda: vb200.paged_attn(s.pc, s.pb, s.q, out, lse=f32(3)),
+                 lambda: vb200.paged_attn(s.pc, s.pb, s.q, out, workspace=torch.zeros(8, dtype=torch.uint8)),
+                 lambda: vb200.paged_append(s.pc, s.pb, s.kn[:, 0], s.vn), lambda: vb200.PagedCache(s.k[0], s.v[0]),
+                 lambda: vb200.PagedBatch(s.q_start, s.lens, s.table[0], max_new=2, max_len=30, tokens=3),
+                 lambda: vb200.PagedBatch(s.q_start, s.lens[0], s.table, max_new=2, max_len=30, tokens=3)):
+        with pytest.raises(vb200.VBError):
+            call()
+
+
 # ------------------------------------------------- values that are not finite
 
 def formula(s, window=0):

@@ -779,7 +779,7 @@ class LogitsRules:
         d = self.index
         self.keep = (hist_start, hist_ids, prompt_len, repetition, frequency, presence, bias_start, bias_ids,
                      bias_vals, mask)
-        self.words = None if mask is None else mask.shape[1]
+        self.words = None if mask is None else mask.shape[-1] if mask.dim() else 0
         self.s = VBLogitsRules(
             _array(hist_start, _I32, d, "hist_start"), _array(hist_ids, _I32, d, "hist_ids"),
             0 if hist_ids is None else hist_ids.numel(), _array(prompt_len, _I32, d, "prompt_len"),
