@@ -1,6 +1,7 @@
 """Calls of the paged operators at the edges of what their interface allows."""
 import ctypes as C
 import math
+import random
 import time
 
 import pytest
@@ -86,12 +87,15 @@ def test_python_faces_refuse_with_their_own_error():
 # ------------------------------------------------- values that are not finite
 
 def formula(s, window=0):
-    """out in 64 bits, in the sense of limits: a weight of 0 silences whatever stands there, any
-    other passes an infinity on.  And the error bound of its finite elements."""
+    """out in 64 bits, the error bound of its finite elements, and lse.  What is seen is multiplied by its
+    weight, an infinity by a weight of 0 (a score of -inf) being NaN; what is not seen is not there.
+    A row whose scores are all -inf is empty."""
     out = torch.zeros(s.T, s.H, s.D, dtype=torch.float64, device="cuda")
     tol = torch.zeros_like(out)
     lse = torch.full((s.T, s.H), -math.inf, dtype=torch.float64, device="cuda")  # NaN under a score of +inf, as out
     for b in range(len(s.news)):
+        if not s.news[b]:
+            continue
         k, v = s.gather(b)
         pos, r = s.pos(b), s.rows(b)
         q = s.q[r].double().reshape(-1, s.KVH, s.G, s.D)
@@ -105,12 +109,14 @@ def formula(s, window=0):
             x = q[:, h, :, d] * k[n, h, d]
             a[:, h, :, n] = torch.where(torch.isnan(x) | torch.isinf(x), x, a[:, h, :, n])
         a = a.masked_fill(~see[:, None, None], -math.inf)
-        p = torch.softmax(a, -1)
+        empty = (a == -math.inf).all(-1, keepdim=True)
+        p = torch.where(empty, 0, torch.softmax(a, -1))
         fin = torch.isfinite(v)
         y = torch.einsum("nhgl,lhd->nhgd", p, torch.where(fin, v, 0))
         mass = torch.einsum("nhgl,lhd->nhgd", p, torch.where(fin, v, 0).abs())
         for n, h, d in torch.nonzero(~fin).tolist():
-            y[:, h, :, d] += torch.where(p[:, h, :, n] == 0, 0, v[n, h, d])
+            y[:, h, :, d] += torch.where(see[:, n, None], p[:, h, :, n] * v[n, h, d], 0)
+        y = torch.where(empty, 0, y)
         size = size.masked_fill(~see[:, None, None], 0).amax(-1)[..., None]
         u = U[s.io]
         out[r] = y.reshape(-1, s.H, s.D)
@@ -191,6 +197,27 @@ def test_an_infinity_under_a_weight_that_f16_has_not(n):
     s.v[slot[0], slot[1], 0, 3] = math.inf
     out = check_formula(s)
     assert (out[:n, :2, 3] == math.inf).all()
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_random_batches_with_values_that_are_not_finite(seed):
+    r = random.Random(seed)
+    io, cache = r.choice(PAIRS)
+    kvh, group = r.choice([1, 2, 4, 8]), r.choice([1, 2, 2, 4, 5, 8, 9, 16, 17, 20, 33])
+    most = r.choice([1, 1, r.randint(2, 20), r.randint(2, 300)])
+    B = min(int(2 ** r.uniform(0, 5)), max(1, 12000 // (most * group * kvh)))
+    news = [r.choice([1, most, r.randint(0, most)]) for _ in range(B)]
+    news[0] = most
+    s = Setup(news, [n + r.randint(0, 600) for n in news], io, cache, H=kvh * group, KVH=kvh, D=r.choice([64, 128]),
+              page=r.choice([1, 5, 8, 16, 32, 64, 128]), order=r.choice(["phd", "hpd"]), seed=seed)
+    for _ in range(r.randint(0, 6)):
+        b = r.randrange(B)
+        if s.lens_h[b]:
+            p, h = r.randrange(s.lens_h[b]), r.randrange(kvh)
+            x = r.choice([s.k, s.v, s.v])[s.table[b, p // s.page].long(), p % s.page, h]
+            if torch.isfinite(x).all():
+                x[r.randrange(s.D)] = r.choice([math.nan, math.inf, -math.inf])
+    check_formula(s, window=r.choice([0, 0, 1, 7, 64, 300]))
 
 
 def _time(call, n=5):
