@@ -2042,9 +2042,10 @@ __global__ void __launch_bounds__(128) paged_attn_merge_kernel(const __grid_cons
 // Joins the pieces of a shared-out tile's rows: grid over (sequence, KV head, group of ROWS
 // tile rows), 8 warps, 8 / ROWS of them for a row, taking turns at its pieces.  One row a
 // block where there are few blocks (a long sequence has dozens of pieces), eight otherwise
-// (every block adds up the batch's lengths).
+// (every block adds up the batch's lengths).  REDO: looks at the rows (AttnView::redo; the code for it,
+// reached or not, cost a mixed batch 2 us).
 constexpr int kJoinWarps = 8;
-template <typename IO, typename KV, int D, int ROWS>
+template <typename IO, typename KV, int D, int ROWS, bool REDO>
 __global__ void __launch_bounds__(kJoinWarps * 32, 5) paged_attn_join_kernel(const __grid_constant__ AttnView a, int groups) {
     constexpr int W = kJoinWarps / ROWS;  // warps of a row
     __shared__ float sums[kJoinWarps][D];
@@ -2068,18 +2069,18 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 5) paged_attn_join_kernel(con
     const bool live = r < s.n * a.group;
     // the block's rows, once they are written: taken again where one has a NaN
     auto look = [&](bool again) {
-        if constexpr (!kAsSeen<IO>) {
+        if constexpr (REDO) {
             const int first = r - warp / W;
-            if (__syncthreads_or(again) && a.redo)
+            if (__syncthreads_or(again))
                 for (int row = first; row < min(first + ROWS, s.n * a.group); row++)
                     redo_row_apart<IO, KV, D, kJoinWarps>(a, s.start + row / a.group, kvh * a.group + row % a.group, sums, ml,
                                                           &done);
         }
     };
     if (used == 1) {  // written by the kernel itself
-        if constexpr (!kAsSeen<IO>) {
+        if constexpr (REDO) {
             bool again = false;
-            if (live && a.redo && warp % W == 0) {
+            if (live && warp % W == 0) {
                 const int token = s.start + r / a.group, head = kvh * a.group + r % a.group;
                 const IO* y = reinterpret_cast<const IO*>(a.out + token * a.o_row + head * a.o_head);
 #pragma unroll
@@ -2356,8 +2357,13 @@ vb_status launch_attn(const AttnView& a, cudaStream_t s) {
         const int groups = one ? rows : (rows + 7) / 8;
         if (heads * groups > 0x7fffffffll) return fail(VB_ERR_UNSUPPORTED, "paged_attn: too many rows");
         const dim3 grid((unsigned)(heads * groups)), block(kJoinWarps * 32);
-        e = one ? launch_pdl(paged_attn_join_kernel<IO, KV, D, 1>, grid, block, 0, s, a, groups)
-                : launch_pdl(paged_attn_join_kernel<IO, KV, D, 8>, grid, block, 0, s, a, groups);
+        constexpr bool kRedo = !kAsSeen<IO>;
+        if (a.redo && kRedo)
+            e = one ? launch_pdl(paged_attn_join_kernel<IO, KV, D, 1, kRedo>, grid, block, 0, s, a, groups)
+                    : launch_pdl(paged_attn_join_kernel<IO, KV, D, 8, kRedo>, grid, block, 0, s, a, groups);
+        else
+            e = one ? launch_pdl(paged_attn_join_kernel<IO, KV, D, 1, false>, grid, block, 0, s, a, groups)
+                    : launch_pdl(paged_attn_join_kernel<IO, KV, D, 8, false>, grid, block, 0, s, a, groups);
         if (e != cudaSuccess) return cuda_fail(e, "paged_attn_join_kernel");
     }
     if (a.many.splits > 1) {
