@@ -245,8 +245,9 @@ enum {
  * the page of its positions j*page_size .. (j+1)*page_size-1.  Row i of a
  * sequence with n new tokens has position p = lens[b] - n + i.  A row with
  * p < 0 (left padding, or a sequence of length 0) has no position: nothing is
- * appended for it and its attention is empty.  Rows behind the last sequence's
- * are left as they were in every output.
+ * appended for it, its q_out is left as it was, and its attention is empty.
+ * Rows behind the last sequence's are left as they were in every output.  A call
+ * whose batch, tokens or (attention) max_new is 0 does nothing.
  * q_start [batch+1], lens [batch] and table are device arrays, read by the
  * kernels only (a captured graph replays with their contents of that moment);
  * max_new and max_len bound what they say.  The kernels check them: a sequence
@@ -309,8 +310,11 @@ VB_API vb_status vb_paged_append(const vb_paged_cache* cache, const vb_paged_bat
  * out [tokens][heads][D] = softmax(scale * q.k) v; an empty
  * row gives zeros.  lse (f32 [tokens][heads], may be NULL) gets the natural
  * logarithm of the sum of exp(scale * q.k), -inf for an empty row.  out and lse
- * must not overlap q.  heads is a
- * multiple of kv_heads, max_len at most 2^30; query heads h*G .. h*G + G-1 read KV head h.  io as in
+ * must not overlap q.  Of 16-bit rows the softmax weights are rounded to the
+ * rows' type before they multiply v (by half a step each at most, relative:
+ * 2^-8 of bf16, 2^-11 of f16), their sum is not, and out is rounded once more;
+ * f32 rows are computed to f32.  heads is a multiple of kv_heads, max_len at
+ * most 2^30; query heads h*G .. h*G + G-1 read KV head h.  io as in
  * vb_paged_append.  workspace: vb_paged_attn_workspace_bytes() bytes (the same
  * for every io and window), 16-byte aligned, no initial contents; calls that
  * may overlap need their own. */

@@ -514,8 +514,8 @@ struct Sink {
 // accumulation truncates, which over thousands of keys would show.  16-bit rows: the
 // weights are rounded to the cache's type (what the tensor cores take; half a step of
 // each, relative, and of both signs), their sum is not.
-// 64 sequences of up to 4096 keys, bf16, 16/8 heads: 88 us, 5.6 TB/s, 0.85 of the measured
-// copy rate; 64 x 2112 f32 192 us, 0.88; 2 x up to 131072 f16 72.5 us, 0.89.
+// 64 sequences of up to 4096 keys, bf16, 16/8 heads: 92 us, 5.3 TB/s, 0.81 of the measured
+// copy rate; 64 x 2112 f32 191-207 us from card to card, 0.82-0.88; 2 x up to 131072 f16 74-77 us, 0.84-0.87.
 //
 // The rows of KV head kvh of sequence b over keys k_begin .. k_end - 1, by the block.
 template <typename IO, typename KV, int D, int NR>
@@ -1021,8 +1021,8 @@ __global__ void __launch_bounds__(FewCfg<KV, D, NR>::kWarps * 32) paged_attn_few
 // to the cache's 16 bits as the products take them, their sum is not.
 // Of the two tiles' 128 x 128 scores the exponentials take 2048 clocks (16 a
 // clock on an SM) and, at D = 128, the products as many.  A prompt of 8192
-// tokens, 16/8 heads, bf16: 254 us, 1083 TFLOP/s, 0.66 of the measured bf16 rate;
-// a key tile of the pair takes about 3000 clocks, bound by the chain scores ->
+// tokens, 16/8 heads, bf16: 287 us (293 with the last pass: 938 TFLOP/s, 0.57 of the
+// measured bf16 rate), at 1700 MHz under the power cap; bound by the chain scores ->
 // weights -> P.V -> next scores of one tile.
 constexpr int kTcThreads = 640;
 constexpr int kTcProducers = 96;
@@ -1605,8 +1605,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
 // which the softmax threads hold, by FMAs: the tensor cores' own accumulation cuts bits off.
 // Tensor memory: scores 2 x 128 columns, over which the high and middle terms of the
 // weights go; P.V 128; the low terms 2 x 64.
-// A prompt of 4096 tokens, 16/8 heads: f32 cache 361 us (3214 us by 16-row tiles of the
-// few-rows kernel).  Two chunks of 512 beside 31 decodes, bf16 cache: 119 us in all (348).
+// A prompt of 4096 tokens, 16/8 heads: f32 cache 400 us (3214 us by 16-row tiles of the
+// few-rows kernel), bf16 cache 180.  Two chunks of 512 beside 31 decodes, bf16 cache: 125 us in all (348).
 constexpr int kExRows = 128;
 
 template <typename KV, int D>
@@ -2137,8 +2137,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 5) paged_attn_join_kernel(con
 // A tile's rows of several tokens see different keys, and a weight of 0 times an infinity or
 // NaN in a v that a row does not see is NaN.  So rows that came out non-finite are looked at
 // again (redo_row).  A warp looks at 2 KB of (token, head) rows, 16 bytes a lane and load, and
-// where all is finite that is all it does: 5 us after a prompt of 8192 tokens (295 us with it,
-// 290 without, in turns) as after 1500 rows, so a launch and its wait more than the 33 MB out of
+// where all is finite that is all it does: 6 us after a prompt of 8192 tokens (293 us with it,
+// 287 without, in turns), 2 after 256 tokens, so a launch and its wait more than the 33 MB out of
 // L2; by 2-byte loads it was 14 us.
 constexpr int kCheckLoads = 4;
 template <typename IO, int D>
@@ -2215,8 +2215,12 @@ Plan make_plan(const PagedView& p, int io, int cache, int heads, int D, int wind
     const int64_t most = (int64_t)p.max_new * G, total = (int64_t)p.tokens * G;  // rows of a KV head
     // Batches that may hold more than 16 rows of a KV head a sequence (8 of f32; one decoded token's G
     // in any case) run on the tensor cores' tiles of 256 (128) rows, all but the sequences of a token
-    // or few.  64 x 4096 keys, bf16: 16 rows 252 us here and 391 there, 32 rows 464 and 344.  One
-    // sequence alone takes one kernel for all it may hold.
+    // or few.  Measured with all sequences alike, us, here and there: 64 x 4096 keys, D = 128, 16 rows: bf16
+    // 215 and 367, f16 217 and 369, f32 over bf16 338 and 337, f32 (2112 keys) 509 and 529; 32 rows: bf16 364 and
+    // 325, f16 372 and 328.  At D = 64 the products weigh less and the crossover lies higher, which the
+    // rule leaves alone: 16 rows f32 179 and 348, f32 over bf16 142 and 276; 32 rows bf16 218 and 282.  (All
+    // sequences would then run on the wider tiles for the longest one's sake: with 8 rows f32 125 us, with 12
+    // 177.)  One sequence alone takes one kernel for all it may hold.
     const int least = G <= 8 ? 8 : G <= 16 || io == VB_F32 ? 16 : 32, many_rows = io == VB_F32 ? kExRows : kTcRows;
     const bool tc = most > (io == VB_F32 ? least : std::max(least, 16));
     pl.few_rows = !tc ? 0x7fffffff : p.batch == 1 ? 0 : least;
