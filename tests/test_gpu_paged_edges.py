@@ -257,7 +257,7 @@ def test_a_nan_that_rows_see_costs_little(io, cache, what, where):
         assert torch.isfinite(out[:n, :, :9]).all() and torch.isfinite(out[:n, :, 10:]).all()
     assert torch.equal(out[n:], keep[n:])
     print(f"{io} {cache} {what} {where}: {clean:.3f} -> {bad:.3f} ms")
-    assert bad < 4 * clean + 1.0, (clean, bad)
+    assert bad < 4 * clean + 3.0, (clean, bad)  # 0.1-1.1 ms; 8-36 where every key was walked by one warp
 
 
 # ---------------------------------------------------------------- launches
